@@ -10,7 +10,7 @@ import os
 c_i32, c_i64, c_u32, c_u64 = ctypes.c_int32, ctypes.c_int64, ctypes.c_uint32, ctypes.c_uint64
 c_dbl, c_vp = ctypes.c_double, ctypes.c_void_p
 
-ABI_VERSION = 9
+ABI_VERSION = 10
 
 MODEL_V0, MODEL_V1, MODEL_V2, MODEL_V4 = 0, 1, 2, 4
 MODEL_V5, MODEL_V6, MODEL_V7, MODEL_V8, MODEL_V9, MODEL_V10, MODEL_V11 = 5, 6, 7, 8, 9, 10, 11
@@ -54,9 +54,21 @@ class FishingBuffers(ctypes.Structure):
     _fields_ = [(name, c_vp) for name in BUFFER_FIELDS]
 
 
+DTYPE_F32, DTYPE_BF16 = 0, 1
+
+
+class FishingDecayAttention(ctypes.Structure):
+    _fields_ = [("dtype", c_i32), ("heads", c_i32), ("dk", c_i32), ("dv", c_i32), ("batch", c_i64), ("steps", c_i64), ("scale", c_dbl),
+                ("q", c_vp), ("k", c_vp), ("v", c_vp), ("log_decay", c_vp), ("starts", c_vp), ("state", c_vp), ("out", c_vp), ("state_out", c_vp),
+                ("q_stride", c_i64 * 3), ("k_stride", c_i64 * 3), ("v_stride", c_i64 * 3), ("out_stride", c_i64 * 3), ("starts_stride", c_i64 * 2),
+                ("dout", c_vp), ("dstate_out", c_vp), ("dq", c_vp), ("dk_out", c_vp), ("dv_out", c_vp), ("dstate", c_vp),
+                ("dout_stride", c_i64 * 3), ("dq_stride", c_i64 * 3), ("dk_stride", c_i64 * 3), ("dv_stride", c_i64 * 3)]
+
+
 # symbol -> (restype, argtypes); must list every function include/fishing_hip.h declares
 _PP = ctypes.POINTER(FishingParams)
 _BP = ctypes.POINTER(FishingBuffers)
+_AP = ctypes.POINTER(FishingDecayAttention)
 SIGNATURES = {
     "fishing_abi_version": (c_i32, []),
     "fishing_error_string": (ctypes.c_char_p, [c_i32]),
@@ -90,6 +102,16 @@ SIGNATURES = {
     "fishing_step_normals_f32": (c_i32, [c_i64, c_i64, c_u64, c_u64, c_vp, c_vp]),
     "fishing_reset_normals_f32": (c_i32, [c_i64, c_i64, c_u64, c_u64, c_i32, c_vp, c_vp, c_vp]),
     "fishing_math_f64": (c_i32, [c_i64, c_i32, c_vp, c_vp, c_vp]),
+    "fishing_embedding_forward": (c_i32, [c_i32, c_i32, c_i64, c_i64, c_i64, c_vp, c_i64, c_vp, ctypes.c_float, c_vp, c_vp]),
+    "fishing_embedding_workspace": (c_i64, [c_i64, c_i64, c_i64]),
+    "fishing_embedding_backward": (c_i32, [c_i32, c_i32, c_i64, c_i64, c_i64, c_vp, c_i64, c_vp, ctypes.c_float, c_vp, c_vp, c_i64, c_vp]),
+    "fishing_decay_attention_step": (c_i32, [_AP, c_vp]),
+    "fishing_decay_attention_workspace": (c_i64, [_AP, c_i32]),
+    "fishing_decay_attention_forward": (c_i32, [_AP, c_vp, c_i64, c_vp]),
+    "fishing_decay_attention_backward": (c_i32, [_AP, c_vp, c_i64, c_vp]),
+    "fishing_cross_entropy_workspace": (c_i64, [c_i32, c_i64, c_i64, c_i64, c_i32]),
+    "fishing_cross_entropy_forward": (c_i32, [c_i32, c_i32, c_i64, c_i64, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_i64, c_vp]),
+    "fishing_cross_entropy_backward": (c_i32, [c_i32, c_i32, c_i64, c_i64, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_vp]),
     "fishing_step_floor_f32": (c_i32, [c_i32, c_i64, _BP, c_i32, c_vp]),
 }
 

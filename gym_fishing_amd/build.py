@@ -42,7 +42,10 @@ HIPCC_FLAGS = ["-O3", "--offload-arch=" + ARCH, "-ffp-contract=off", "-fPIC", "-
 # step 6.70 -> 6.40 us per step at N = 2^22, 1.25 -> 1.13 at 2^18; in-kernel-policy rollouts +2.5-6 %:
 # profiles/r03_rollout_no_slp.jsonl) -- its packed f32 operations save fewer issue slots than its re-ordering costs.
 TU_FLAGS = {"fishing_step.hip": ["-fno-slp-vectorize", "-mllvm", "-amdgpu-kernarg-preload-count=10"],
-            "fishing_rollout.hip": ["-fno-slp-vectorize"]}
+            "fishing_rollout.hip": ["-fno-slp-vectorize"],
+            # the sequence operators accumulate in float32 with fused multiply-adds: no NumPy rounding to reproduce there
+            "sequence_embedding.hip": ["-ffp-contract=fast"], "sequence_attention.hip": ["-ffp-contract=fast"],
+            "sequence_loss.hip": ["-ffp-contract=fast"]}
 
 
 def sources():

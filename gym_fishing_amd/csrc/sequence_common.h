@@ -1,0 +1,90 @@
+// sequence_common.h -- what the sequence operators' kernels share: element types, 16-byte accesses, the matrix-core tile
+// wrappers of gfx950 and the launch helper.  The operators serve an agent that remembers its episode: token embedding
+// (sequence_embedding.hip), linear attention with a decay per head (sequence_attention.hip), softmax cross entropy over the
+// quota levels (sequence_loss.hip).
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <tuple>
+
+#include "../../include/fishing_hip.h"
+
+namespace fishing {
+namespace seq {
+
+typedef __bf16 bf16;
+typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(bf16 x) { return (float)x; }
+// round to nearest even (v_cvt_pk_bf16_f32): the one rounding of an output's last step
+template <typename T>
+__device__ __forceinline__ T from_f32(float x) { return (T)x; }
+
+// N elements that move as one access (16 bytes for the vector forms, one element for the others)
+template <typename T, int N>
+struct alignas(sizeof(T) * N) Pack {
+    T e[N];
+};
+
+template <typename T>
+__host__ __device__ constexpr int vec_of() { return 16 / (int)sizeof(T); }
+
+static inline bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
+static inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+static inline int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
+
+// This launch's own status, as hipLaunchKernel returns it
+template <typename... P, typename... A>
+inline int launch(void (*kernel)(P...), dim3 grid, dim3 block, hipStream_t stream, A&&... args) {
+    std::tuple<P...> packed{static_cast<P>(args)...};
+    return std::apply(
+        [&](auto&... a) {
+            void* argv[] = {(void*)&a...};
+            return (int)hipLaunchKernel((const void*)kernel, grid, block, argv, 0, stream);
+        },
+        packed);
+}
+
+// Workspace carving: 256-byte aligned blocks in the caller's buffer
+struct Carve {
+    char* base;
+    int64_t used = 0;
+    explicit Carve(void* p) : base((char*)p) {}
+    template <typename T>
+    T* take(int64_t count) {
+        T* p = (T*)(base + used);
+        used = round_up(used + count * (int64_t)sizeof(T), 256);
+        return p;
+    }
+};
+
+// Matrix-core tiles.  16 x 16 outputs, lane l: the A operand's row / B operand's column is l % 16, its k indices are
+// (l / 16) * E .. + E - 1 (E = 8 for bf16 with k = 32, 1 for f32 with k = 4); the accumulator's column is l % 16, its four
+// rows (l / 16) * 4 .. + 3.
+template <typename T>
+struct Mma;
+template <>
+struct Mma<bf16> {
+    static constexpr int K = 32, E = 8;
+    typedef bf16x8 Frag;
+    static __device__ __forceinline__ f32x4 run(Frag a, Frag b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    }
+};
+template <>
+struct Mma<float> {
+    static constexpr int K = 4, E = 1;
+    typedef float Frag;
+    static __device__ __forceinline__ f32x4 run(Frag a, Frag b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
+    }
+};
+
+}  // namespace seq
+}  // namespace fishing

@@ -1,0 +1,355 @@
+// sequence_embedding.hip -- rows of a table for tokens, and the table's gradient by sorted tokens.
+#include "sequence_common.h"
+
+namespace fishing {
+namespace seq {
+
+// out[i] = scale * table[token[i]]; a token outside [0, vocab) is padding: a row of zeros.
+// A block owns 256 / vecs rows at a time (vecs accesses a row), four times over; bound by the rows written.
+template <typename T, typename I, int V>
+__global__ void __launch_bounds__(256) embedding_kernel(const T* table, int64_t table_stride, const I* token, int64_t n, int64_t vocab,
+                                                        int32_t vecs, float scale, T* out) {
+    const int per = vecs < 256 ? 256 / vecs : 1;
+    const int r = threadIdx.x / vecs < per ? threadIdx.x / vecs : -1;
+    const int c0 = vecs < 256 ? threadIdx.x % vecs : threadIdx.x;
+    if (vecs < 256 && r < 0) return;
+    const int64_t dim = (int64_t)vecs * V;
+#pragma unroll 4
+    for (int j = 0; j < 4; ++j) {
+        const int64_t i = ((int64_t)blockIdx.x * 4 + j) * per + (vecs < 256 ? r : 0);
+        if (i >= n) return;
+        const int64_t t = (int64_t)token[i];
+        const bool there = t >= 0 && t < vocab;
+        for (int c = c0; c < vecs; c += 256) {
+            Pack<T, V> x;
+            if (there) {
+                x = *(const Pack<T, V>*)(table + t * table_stride + (int64_t)c * V);
+#pragma unroll
+                for (int e = 0; e < V; ++e) x.e[e] = from_f32<T>(to_f32(x.e[e]) * scale);
+            } else {
+#pragma unroll
+                for (int e = 0; e < V; ++e) x.e[e] = from_f32<T>(0.0f);
+            }
+            *(Pack<T, V>*)(out + i * dim + (int64_t)c * V) = x;
+        }
+    }
+}
+
+// ---- the gradient: dtable[v] = scale * sum of dout[i] over the i with token[i] == v, in ascending i ----
+// A stable radix sort of (token, i) by up to 8 bits a pass puts a token's rows side by side; then chunks of the sorted order
+// are summed in float32 registers, and runs that cross a chunk's border leave a partial row that the last kernel adds in
+// chunk order.  No atomics: the same bits every time.
+constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64, kMaxDigits = 256;
+
+__device__ __forceinline__ uint32_t key_of(int64_t t, int64_t vocab) { return t >= 0 && t < vocab ? (uint32_t)t : (uint32_t)vocab; }
+
+template <typename I, bool FIRST>
+__global__ void __launch_bounds__(kSortThreads) sort_count_kernel(const I* token, const uint32_t* key, int64_t n, int64_t vocab, int64_t tile, int shift,
+                                                                  int digits, uint32_t* count) {
+    __shared__ uint32_t bin[kMaxDigits];
+    for (int d = threadIdx.x; d < digits; d += kSortThreads) bin[d] = 0;
+    __syncthreads();
+    const int64_t lo = (int64_t)blockIdx.x * tile, hi = lo + tile < n ? lo + tile : n;
+    for (int64_t i = lo + threadIdx.x; i < hi; i += kSortThreads) {
+        const uint32_t k = FIRST ? key_of((int64_t)token[i], vocab) : key[i];
+        atomicAdd(&bin[(k >> shift) & (digits - 1)], 1u);   // whole numbers: the order does not matter
+    }
+    __syncthreads();
+    for (int d = threadIdx.x; d < digits; d += kSortThreads) count[(int64_t)d * gridDim.x + blockIdx.x] = bin[d];
+}
+
+// exclusive sum over count[digits * blocks], one workgroup
+__global__ void __launch_bounds__(1024) sort_scan_kernel(uint32_t* count, int32_t n) {
+    __shared__ uint32_t sum[1024];
+    const int per = (n + 1023) / 1024, lo = threadIdx.x * per, hi = lo + per < n ? lo + per : n;
+    uint32_t s = 0;
+    for (int i = lo; i < hi; ++i) s += count[i];
+    sum[threadIdx.x] = s;
+    __syncthreads();
+    for (int d = 1; d < 1024; d <<= 1) {
+        const uint32_t x = threadIdx.x >= d ? sum[threadIdx.x - d] : 0;
+        __syncthreads();
+        sum[threadIdx.x] += x;
+        __syncthreads();
+    }
+    uint32_t run = sum[threadIdx.x] - s;
+    for (int i = lo; i < hi; ++i) {
+        const uint32_t x = count[i];
+        count[i] = run;
+        run += x;
+    }
+}
+
+template <typename I, bool FIRST>
+__global__ void __launch_bounds__(kSortThreads) sort_place_kernel(const I* token, const uint32_t* key, const uint32_t* row, int64_t n, int64_t vocab,
+                                                                  int64_t tile, int shift, int bits, const uint32_t* count, uint32_t* key_out, uint32_t* row_out) {
+    __shared__ uint32_t base[kMaxDigits];
+    __shared__ uint32_t in_wave[kSortWaves][kMaxDigits];
+    const int digits = 1 << bits, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    for (int d = threadIdx.x; d < digits; d += kSortThreads) base[d] = count[(int64_t)d * gridDim.x + blockIdx.x];
+    const int64_t lo = (int64_t)blockIdx.x * tile, hi = lo + tile < n ? lo + tile : n;
+    for (int64_t i0 = lo; i0 < hi; i0 += kSortThreads) {
+        for (int d = threadIdx.x; d < kSortWaves * digits; d += kSortThreads) in_wave[d >> bits][d & (digits - 1)] = 0;
+        __syncthreads();
+        const int64_t i = i0 + threadIdx.x;
+        const bool there = i < hi;
+        uint32_t k = 0, from = 0;
+        if (there) {
+            k = FIRST ? key_of((int64_t)token[i], vocab) : key[i];
+            from = FIRST ? (uint32_t)i : row[i];
+        }
+        const uint32_t d = (k >> shift) & (digits - 1);
+        uint64_t same = __ballot(there);
+        for (int b = 0; b < bits; ++b) {
+            const uint64_t set = __ballot((d >> b) & 1);
+            same &= (d >> b) & 1 ? set : ~set;
+        }
+        const uint32_t rank = __popcll(same & ((1ull << lane) - 1));
+        if (there && rank == 0) in_wave[wave][d] = __popcll(same);
+        __syncthreads();
+        for (int x = threadIdx.x; x < digits; x += kSortThreads) {
+            uint32_t run = base[x];
+            for (int w = 0; w < kSortWaves; ++w) {
+                const uint32_t c = in_wave[w][x];
+                in_wave[w][x] = run;
+                run += c;
+            }
+            base[x] = run;
+        }
+        __syncthreads();
+        if (there) {
+            const uint32_t at = in_wave[wave][d] + rank;
+            key_out[at] = k;
+            row_out[at] = from;
+        }
+        __syncthreads();
+    }
+}
+
+// start[v] = first sorted position with a key >= v, v = 0 .. vocab; written where the key changes, by the lanes of a group
+template <int G>
+__device__ __forceinline__ void mark_starts(uint32_t* start, int64_t from, int64_t to, uint32_t at, int lane) {
+    for (int64_t v = from + lane; v <= to; v += G) start[v] = at;
+}
+
+// A group of G lanes sums one chunk of the sorted order, V columns a lane; blockIdx.y walks the columns beyond G * V.
+template <typename T, int V, int G>
+__global__ void __launch_bounds__(256) embedding_sum_kernel(const T* dout, int64_t dout_stride, const uint32_t* key, const uint32_t* row, int64_t n, int64_t vocab,
+                                                            int32_t dim, int32_t chunk, float scale, T* dtable, float* partial, uint32_t* start) {
+    constexpr int U = 8;
+    const int lane = threadIdx.x % G;
+    const int64_t c = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
+    const int64_t p0 = c * chunk, p1 = p0 + chunk < n ? p0 + chunk : n;
+    if (p0 >= n) return;
+    const int col = (blockIdx.y * G + lane) * V;
+    const bool mine = col < dim, marks = blockIdx.y == 0;
+    const int64_t before = p0 > 0 ? (int64_t)key[p0 - 1] : -1, after = p1 < n ? (int64_t)key[p1] : -1;
+    float acc[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) acc[e] = 0.0f;
+    int64_t cur = key[p0];
+    bool first = true;
+    if (marks && cur != before) mark_starts<G>(start, before + 1, cur, (uint32_t)p0, lane);
+    auto flush = [&](bool last) {
+        if (cur < vocab && mine) {
+            const bool crosses = (first && cur == before) || (last && cur == after);
+            if (crosses) {
+                float* to = partial + (2 * c + (first ? 0 : 1)) * dim + col;
+#pragma unroll
+                for (int e = 0; e < V; ++e) to[e] = acc[e];
+            } else {
+                Pack<T, V> x;
+#pragma unroll
+                for (int e = 0; e < V; ++e) x.e[e] = from_f32<T>(acc[e] * scale);
+                *(Pack<T, V>*)(dtable + cur * dim + col) = x;
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc[e] = 0.0f;
+        first = false;
+    };
+    for (int64_t p = p0; p < p1; p += U) {
+        uint32_t k[U];
+        Pack<T, V> x[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t at = p + u < p1 ? p + u : p1 - 1;
+            k[u] = key[at];
+            if (mine && k[u] < vocab) x[u] = *(const Pack<T, V>*)(dout + (int64_t)row[at] * dout_stride + col);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (p + u < p1) {
+                if ((int64_t)k[u] != cur) {
+                    flush(false);
+                    if (marks) mark_starts<G>(start, cur + 1, k[u], (uint32_t)(p + u), lane);
+                    cur = k[u];
+                }
+                if (mine && k[u] < vocab) {
+#pragma unroll
+                    for (int e = 0; e < V; ++e) acc[e] += to_f32(x[u].e[e]);
+                }
+            }
+        }
+    }
+    flush(true);
+    if (marks && p1 == n) mark_starts<G>(start, cur + 1, vocab, (uint32_t)n, lane);
+}
+
+// the rows the chunks did not finish: tokens that were never met (zeros) and runs over several chunks (their partials' sum)
+template <typename T>
+__global__ void __launch_bounds__(256) embedding_join_kernel(const uint32_t* start, const float* partial, int64_t n, int64_t vocab, int32_t dim, int32_t chunk,
+                                                             float scale, T* dtable) {
+    const int64_t v = blockIdx.x;
+    const int64_t s = n ? start[v] : 0, e = n ? start[v + 1] : 0;
+    const int64_t a = s / chunk, b = e > s ? (e - 1) / chunk : a;
+    if (e > s && a == b) return;
+    for (int col = threadIdx.x; col < dim; col += 256) {
+        float acc = 0.0f;
+        if (e > s) {
+            acc = partial[(2 * a + (s == a * chunk ? 0 : 1)) * dim + col];
+#pragma unroll 8
+            for (int64_t c = a + 1; c <= b; ++c) acc += partial[2 * c * dim + col];
+        }
+        dtable[v * dim + col] = from_f32<T>(acc * scale);
+    }
+}
+
+struct SortPlan {
+    int bits, passes, digit_bits;
+    int64_t tile;
+    int blocks;
+    int32_t chunk;
+    int64_t chunks;
+};
+
+static SortPlan sort_plan(int64_t n, int64_t vocab) {
+    SortPlan s;
+    s.bits = 1;
+    while (((int64_t)1 << s.bits) <= vocab) ++s.bits;         // keys 0 .. vocab
+    s.passes = (s.bits + 7) / 8;
+    s.digit_bits = (s.bits + s.passes - 1) / s.passes;
+    s.tile = round_up(ceil_div(n > 0 ? n : 1, 512), 2 * kSortThreads);
+    s.blocks = (int)ceil_div(n > 0 ? n : 1, s.tile);
+    s.chunk = n >= (1 << 19) ? 256 : n >= (1 << 16) ? 64 : 16;
+    s.chunks = ceil_div(n, s.chunk);
+    return s;
+}
+
+struct EmbeddingWork {
+    uint32_t *key[2], *row[2], *count, *start;
+    float* partial;
+    int64_t bytes;
+};
+
+static EmbeddingWork embedding_work(const SortPlan& s, int64_t n, int64_t vocab, int64_t dim, void* at) {
+    Carve c(at);
+    EmbeddingWork w;
+    for (int k = 0; k < 2; ++k) {
+        w.key[k] = c.take<uint32_t>(n);
+        w.row[k] = c.take<uint32_t>(n);
+    }
+    w.count = c.take<uint32_t>((int64_t)s.blocks << s.digit_bits);
+    w.start = c.take<uint32_t>(vocab + 1);
+    w.partial = c.take<float>(2 * s.chunks * dim);
+    w.bytes = c.used;
+    return w;
+}
+
+static int embedding_check(int32_t dtype, int32_t index_bytes, int64_t n, int64_t vocab, int64_t dim) {
+    if (dtype != FISHING_DTYPE_F32 && dtype != FISHING_DTYPE_BF16) return FISHING_ERR_UNSUPPORTED;
+    if (index_bytes != 4 && index_bytes != 8) return FISHING_ERR_UNSUPPORTED;
+    if (n < 0 || n > 0x7fffffff || vocab < 1 || vocab > 0x7ffffffe || dim < 1 || dim > 65536) return FISHING_ERR_SIZE;
+    return FISHING_OK;
+}
+
+template <typename T, typename I>
+static int embedding_forward(int64_t n, int64_t vocab, int64_t dim, const T* table, int64_t table_stride, const I* token, float scale, T* out, hipStream_t stream) {
+    constexpr int V = vec_of<T>();
+    auto go = [&](auto kernel, int vecs) {
+        const int64_t per = vecs < 256 ? 256 / vecs : 1;
+        return launch(kernel, dim3((unsigned)ceil_div(n, 4 * per)), dim3(256), stream, table, table_stride, token, n, vocab, vecs, scale, out);
+    };
+    if (dim % V == 0 && table_stride % V == 0 && aligned16(table) && aligned16(out)) return go(embedding_kernel<T, I, V>, (int)(dim / V));
+    return go(embedding_kernel<T, I, 1>, (int)dim);
+}
+
+template <typename T, typename I>
+static int embedding_backward(int64_t n, int64_t vocab, int64_t dim, const T* dout, int64_t dout_stride, const I* token, float scale, T* dtable, void* workspace,
+                              hipStream_t stream) {
+    const SortPlan s = sort_plan(n, vocab);
+    const EmbeddingWork w = embedding_work(s, n, vocab, dim, workspace);
+    int rc = 0;
+    if (n > 0) {
+        for (int p = 0; p < s.passes && !rc; ++p) {
+            const int shift = p * s.digit_bits, digits = 1 << s.digit_bits;
+            const uint32_t *key = w.key[(p + 1) & 1], *row = w.row[(p + 1) & 1];
+            const dim3 grid(s.blocks), block(kSortThreads);
+            rc = p == 0 ? launch(sort_count_kernel<I, true>, grid, block, stream, token, key, n, vocab, s.tile, shift, digits, w.count)
+                        : launch(sort_count_kernel<I, false>, grid, block, stream, token, key, n, vocab, s.tile, shift, digits, w.count);
+            if (!rc) rc = launch(sort_scan_kernel, dim3(1), dim3(1024), stream, w.count, s.blocks << s.digit_bits);
+            if (!rc)
+                rc = p == 0 ? launch(sort_place_kernel<I, true>, grid, block, stream, token, key, row, n, vocab, s.tile, shift, s.digit_bits, w.count, w.key[0], w.row[0])
+                            : launch(sort_place_kernel<I, false>, grid, block, stream, token, key, row, n, vocab, s.tile, shift, s.digit_bits, w.count, w.key[p & 1], w.row[p & 1]);
+        }
+        if (rc) return rc;
+        const uint32_t *key = w.key[(s.passes - 1) & 1], *row = w.row[(s.passes - 1) & 1];
+        auto sum = [&](auto kernel, int V, int G) {
+            return launch(kernel, dim3((unsigned)ceil_div(s.chunks, 256 / G), (unsigned)ceil_div(dim, G * V)), dim3(256), stream, dout, dout_stride, key, row, n, vocab,
+                          (int32_t)dim, s.chunk, scale, dtable, w.partial, w.start);
+        };
+        constexpr int V = vec_of<T>();
+        if (dim % V == 0 && dout_stride % V == 0 && aligned16(dout) && aligned16(dtable)) {
+            const int64_t lanes = dim / V;
+            rc = lanes <= 8 ? sum(embedding_sum_kernel<T, V, 8>, V, 8) : lanes <= 16 ? sum(embedding_sum_kernel<T, V, 16>, V, 16)
+               : lanes <= 32 ? sum(embedding_sum_kernel<T, V, 32>, V, 32) : sum(embedding_sum_kernel<T, V, 64>, V, 64);
+        } else {
+            rc = sum(embedding_sum_kernel<T, 1, 64>, 1, 64);
+        }
+        if (rc) return rc;
+    }
+    return launch(embedding_join_kernel<T>, dim3((unsigned)vocab), dim3(256), stream, w.start, w.partial, n, vocab, (int32_t)dim, s.chunk, scale, dtable);
+}
+
+}  // namespace seq
+}  // namespace fishing
+
+using namespace fishing::seq;
+
+extern "C" {
+
+int fishing_embedding_forward(int32_t dtype, int32_t index_bytes, int64_t n, int64_t vocab, int64_t dim, const void* table, int64_t table_stride, const void* token,
+                              float scale, void* out, fishing_stream_t stream) {
+    if (int rc = embedding_check(dtype, index_bytes, n, vocab, dim)) return rc;
+    if (table_stride < dim) return FISHING_ERR_SIZE;
+    if (n == 0) return FISHING_OK;
+    if (!table || !token || !out) return FISHING_ERR_NULL;
+    hipStream_t st = (hipStream_t)stream;
+    if (dtype == FISHING_DTYPE_F32)
+        return index_bytes == 4 ? embedding_forward<float, int32_t>(n, vocab, dim, (const float*)table, table_stride, (const int32_t*)token, scale, (float*)out, st)
+                                : embedding_forward<float, int64_t>(n, vocab, dim, (const float*)table, table_stride, (const int64_t*)token, scale, (float*)out, st);
+    return index_bytes == 4 ? embedding_forward<bf16, int32_t>(n, vocab, dim, (const bf16*)table, table_stride, (const int32_t*)token, scale, (bf16*)out, st)
+                            : embedding_forward<bf16, int64_t>(n, vocab, dim, (const bf16*)table, table_stride, (const int64_t*)token, scale, (bf16*)out, st);
+}
+
+int64_t fishing_embedding_workspace(int64_t n, int64_t vocab, int64_t dim) {
+    if (int rc = embedding_check(FISHING_DTYPE_F32, 4, n, vocab, dim)) return rc;
+    return embedding_work(sort_plan(n, vocab), n, vocab, dim, nullptr).bytes;
+}
+
+int fishing_embedding_backward(int32_t dtype, int32_t index_bytes, int64_t n, int64_t vocab, int64_t dim, const void* dout, int64_t dout_stride, const void* token,
+                               float scale, void* dtable, void* workspace, int64_t workspace_bytes, fishing_stream_t stream) {
+    if (int rc = embedding_check(dtype, index_bytes, n, vocab, dim)) return rc;
+    if (n > 0 && dout_stride < dim) return FISHING_ERR_SIZE;
+    if (!dtable || !workspace || (n > 0 && (!dout || !token))) return FISHING_ERR_NULL;
+    if (!aligned16(workspace)) return FISHING_ERR_ALIGN;
+    if (workspace_bytes < fishing_embedding_workspace(n, vocab, dim)) return FISHING_ERR_SIZE;
+    hipStream_t st = (hipStream_t)stream;
+    if (dtype == FISHING_DTYPE_F32)
+        return index_bytes == 4 ? embedding_backward<float, int32_t>(n, vocab, dim, (const float*)dout, dout_stride, (const int32_t*)token, scale, (float*)dtable, workspace, st)
+                                : embedding_backward<float, int64_t>(n, vocab, dim, (const float*)dout, dout_stride, (const int64_t*)token, scale, (float*)dtable, workspace, st);
+    return index_bytes == 4 ? embedding_backward<bf16, int32_t>(n, vocab, dim, (const bf16*)dout, dout_stride, (const int32_t*)token, scale, (bf16*)dtable, workspace, st)
+                            : embedding_backward<bf16, int64_t>(n, vocab, dim, (const bf16*)dout, dout_stride, (const int64_t*)token, scale, (bf16*)dtable, workspace, st);
+}
+
+}  // extern "C"

@@ -32,12 +32,13 @@
 extern "C" {
 #endif
 
-/* 9: FISHING_FLAG_RESET_COUNTER_ON_DEVICE (the reset counter as a fourth word of FishingBuffers.counter, read and bumped by
+/* 10: the sequence operators (fishing_embedding_*, fishing_decay_attention_*, fishing_cross_entropy_*); everything else as in 9.
+ * 9: FISHING_FLAG_RESET_COUNTER_ON_DEVICE (the reset counter as a fourth word of FishingBuffers.counter, read and bumped by
  * fishing_reset_* itself: captured resets draw fresh parameters at every replay); fishing_math_f64 keeps fn 0-1 only.
  * 8: same entry points and structs as 7; fishing-v11's per-episode model choice is drawn from one Philox2x32-10 block per env
  * quad (four 16-bit draws) instead of a Philox4x32-10 block -- a run of a fishing-v11 batch continues with other model draws
  * than under ABI 7; the float64 zoo evaluates the growth functions' algebraic form (same 2e-14 bar). */
-#define FISHING_ABI_VERSION 9
+#define FISHING_ABI_VERSION 10
 
 typedef void* fishing_stream_t; /* hipStream_t */
 
@@ -378,6 +379,65 @@ int fishing_reset_normals_f32(int64_t n, int64_t env_offset, uint64_t seed, uint
 #define FISHING_MATH_LOG_F64 0
 #define FISHING_MATH_EXP_F64 1
 int fishing_math_f64(int64_t n, int32_t fn, const double* in, double* out, fishing_stream_t stream);
+
+/* ---- Sequence operators: what an agent that remembers its episode computes (gym_fishing_amd/sequence.py) ----------------
+ * The reference's agents come from stable-baselines3 (tests/test-PPO.py:10-21) and remember nothing; fishing-v4, -v10 and -v11
+ * draw parameters that only the episode's history shows.  Same conventions as above, with these differences: pointers need their
+ * element's alignment only (16-byte aligned, contiguous rows take the wide accesses), `workspace` is 16-byte aligned, holds at
+ * least what the matching *_workspace call returns (bytes, or a negative error code) and is free again when the call's launches are done.
+ * Values are float32 or bfloat16; sums, statistics and states are float32.  All results are the same bits at every call. */
+#define FISHING_DTYPE_F32 0
+#define FISHING_DTYPE_BF16 1
+
+/* out[i, :] = scale * table[token[i], :], i < n; zeros where token[i] is outside [0, vocab) (padding).  token: int32 / int64
+ * (index_bytes 4 / 8), contiguous; out: contiguous [n, dim]; table_stride: elements between the table's rows. */
+int fishing_embedding_forward(int32_t dtype, int32_t index_bytes, int64_t n, int64_t vocab, int64_t dim, const void* table, int64_t table_stride, const void* token,
+                              float scale, void* out, fishing_stream_t stream);
+/* dtable[v, :] = scale * sum of dout[i, :] over token[i] == v, for every v < vocab (zeros where none); contiguous [vocab, dim]. */
+int64_t fishing_embedding_workspace(int64_t n, int64_t vocab, int64_t dim);
+int fishing_embedding_backward(int32_t dtype, int32_t index_bytes, int64_t n, int64_t vocab, int64_t dim, const void* dout, int64_t dout_stride, const void* token,
+                               float scale, void* dtable, void* workspace, int64_t workspace_bytes, fishing_stream_t stream);
+
+/* Linear attention with a decay for each head.  For every batch row and head, over steps t:
+ *   S_t = a_t S_{t-1} + k_t v_t^T     a_t = exp(log_decay[h]), 0 where starts[batch, t] (an episode begins at t)
+ *   out_t = scale * q_t S_t
+ * q, k: [batch, steps, heads, dk], v, out: [batch, steps, heads, dv] with unit stride in the last axis and the element strides
+ * {batch, step, head} given; starts: bytes with strides {batch, step}, nullable; state, state_out: float32 [batch, heads, dk, dv]
+ * contiguous, nullable except for the single step.  dk, dv in 1 .. 128.  steps = 0 hands the state through. */
+typedef struct FishingDecayAttention {
+    int32_t dtype, heads, dk, dv;
+    int64_t batch, steps;
+    double scale;
+    const void *q, *k, *v;
+    const float* log_decay;   /* float32[heads] */
+    const uint8_t* starts;
+    const float* state;
+    void* out;
+    float* state_out;
+    int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3], starts_stride[2];
+    /* backward: gradients of out and (nullable) state_out in; of q, k, v and (nullable) state out */
+    const void* dout;
+    const float* dstate_out;
+    void *dq, *dk_out, *dv_out;
+    float* dstate;
+    int64_t dout_stride[3], dq_stride[3], dk_stride[3], dv_stride[3];
+} FishingDecayAttention;
+
+/* one step (the step stride is not read): state -> state_out (the same buffer, or one that does not overlap it), out */
+int fishing_decay_attention_step(const FishingDecayAttention* a, fishing_stream_t stream);
+int64_t fishing_decay_attention_workspace(const FishingDecayAttention* a, int32_t backward);
+int fishing_decay_attention_forward(const FishingDecayAttention* a, void* workspace, int64_t workspace_bytes, fishing_stream_t stream);
+int fishing_decay_attention_backward(const FishingDecayAttention* a, void* workspace, int64_t workspace_bytes, fishing_stream_t stream);
+
+/* Softmax cross entropy of rows of `hidden` [rows, dim] against `head` [levels, dim]: loss[r] = lse[r] - hidden[r] . head[target[r]],
+ * lse[r] = log sum_v exp(hidden[r] . head[v]); loss 0 and no gradient where target[r] is outside [0, levels).  The logits are
+ * never kept: the levels are taken in pieces.  Backward: grad[r] is loss[r]'s gradient; dhidden, dhead contiguous. */
+int64_t fishing_cross_entropy_workspace(int32_t dtype, int64_t rows, int64_t levels, int64_t dim, int32_t backward);
+int fishing_cross_entropy_forward(int32_t dtype, int32_t target_bytes, int64_t rows, int64_t levels, int64_t dim, const void* hidden, int64_t hidden_stride, const void* head,
+                                  int64_t head_stride, const void* target, float* loss, float* lse, void* workspace, int64_t workspace_bytes, fishing_stream_t stream);
+int fishing_cross_entropy_backward(int32_t dtype, int32_t target_bytes, int64_t rows, int64_t levels, int64_t dim, const void* hidden, int64_t hidden_stride, const void* head,
+                                   int64_t head_stride, const void* target, const float* lse, const float* grad, void* dhidden, void* dhead, void* workspace,
+                                   int64_t workspace_bytes, fishing_stream_t stream);
 
 #ifdef __cplusplus
 }
