@@ -3,200 +3,297 @@
 //   z = h W^T        lse = log sum_v exp(z_v)        loss = lse - z_y        (0 where the target y is outside [0, levels))
 //   dz = g (exp(z - lse) - [v == y])        dh = dz W        dW = dz^T h
 //
-// Forward: a workgroup computes the logits of a tile of rows against a range of levels and keeps each row's running maximum and sum;
-// the ranges' pairs are joined afterwards.  Backward: the logits are computed again, a piece of the levels at a time, turned into dz
-// in the operands' type (the factor of the two products' operands; sums stay in float32) and multiplied.
-#include "sequence_common.h"
+// Forward: one product whose epilogue reduces each row's tile of logits to a maximum and a sum of exponentials; the tiles' pairs are
+// joined afterwards.  Backward: per piece of the levels the logits are computed again and turned into dz (rounded to the operands'
+// type: it is a factor of the two products that follow; sums stay in float32), kept for the piece as dz^T [level][row], where four
+// rows of a lane's accumulator are one store, and multiplied twice: k-major for dh, k-contiguous for dW.
+#include "sequence_gemm.h"
 
 namespace fishing {
 namespace seq {
-
-// ---- a 64 x 64 tile of A B^T or its transposed forms; element (row, k) of an operand sits at row * ld + k, or k * ld + row ----
-template <typename T>
-struct Operand {
-    const T* p;
-    int64_t ld;
-    int64_t rows;
-    bool across;
-    const void* target = nullptr;   // where given: k runs over rows of `hidden`, and those of padded targets count as zeros, whatever they hold
-    int target_bytes = 0;
-    int64_t levels = 0;
-};
 
 __device__ __forceinline__ int64_t target_of(const void* target, int bytes, int64_t row) {
     return bytes == 4 ? (int64_t)((const int32_t*)target)[row] : ((const int64_t*)target)[row];
 }
 
-template <typename T>
-struct Tile {
-    static constexpr int BK = 32, PAD = 8;
-    T a[64][BK + PAD], b[64][BK + PAD];
-};
+constexpr float kLog2E = 1.4426950408889634f;
+__device__ __forceinline__ float exp_fast(float x) { return __builtin_amdgcn_exp2f(x * kLog2E); }
 
+// rows of `width` to rows of `padded`, zeros behind; rows of padded targets become zeros, whatever they hold (NaN times a zero dz is NaN)
 template <typename T>
-__device__ __forceinline__ void stage(T (*to)[Tile<T>::BK + Tile<T>::PAD], const Operand<T>& o, int64_t row0, int64_t k0, int64_t depth) {
-    constexpr int BK = Tile<T>::BK;
-    for (int x = threadIdx.x; x < 64 * BK; x += 256) {
-        const int r = o.across ? x % 64 : x / BK, k = o.across ? x / 64 : x % BK;
-        const int64_t row = row0 + r, kk = k0 + k;
-        T e = from_f32<T>(0.0f);
-        bool there = row < o.rows && kk < depth;
-        if (there && o.target) {
-            const int64_t y = target_of(o.target, o.target_bytes, kk);
-            there = y >= 0 && y < o.levels;
-        }
-        if (there) e = o.across ? o.p[kk * o.ld + row] : o.p[row * o.ld + kk];
-        to[r][k] = e;
+__global__ void __launch_bounds__(256) pad_kernel(const T* src, int64_t ld, int64_t rows, int32_t width, T* dst, int32_t padded, const void* target, int target_bytes,
+                                                  int64_t levels) {
+    constexpr int V = vec_of<T>();
+    const int per = padded / V;
+    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t row = at / per;
+    const int c = (int)(at - row * per) * V;
+    if (row >= rows) return;
+    bool there = true;
+    if (target) {
+        const int64_t y = target_of(target, target_bytes, row);
+        there = y >= 0 && y < levels;
     }
+    Pack<T, V> x;
+    const T* from = src + row * ld + c;
+    if (there && c + V <= width && ((uintptr_t)from & 15) == 0) {
+        x = *(const Pack<T, V>*)from;
+    } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) x.e[e] = there && c + e < width ? from[e] : from_f32<T>(0.0f);
+    }
+    *(Pack<T, V>*)(dst + row * padded + c) = x;
 }
 
-// four waves, each 32 x 32 as 2 x 2 matrix-core tiles
-template <typename T>
-__device__ __forceinline__ void multiply(Tile<T>& t, const Operand<T>& a, int64_t a0, const Operand<T>& b, int64_t b0, int64_t depth, f32x4 (&acc)[2][2]) {
-    typedef Mma<T> M;
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, wr = (wave >> 1) * 32, wc = (wave & 1) * 32;
+// ---- forward: top[part][row], sum[part][row] of BN / WN levels each; taken[row] = the target's logit ----
+template <typename T, typename G, int BM, int BN>
+__global__ void __launch_bounds__(G::THREADS, 2)
+    loss_part_kernel(Operand<T> h, Operand<T> w, int64_t k, const void* target, int target_bytes, int64_t tiles_m, int64_t tiles_n, float* top, float* sum, float* taken) {
+    __shared__ __attribute__((aligned(16))) char lds0[G::BYTES];
+    __shared__ __attribute__((aligned(16))) char lds1[G::BYTES];
+    const int64_t tile = xcd_tile(blockIdx.x, tiles_m * tiles_n);
+    const int64_t tm = tile % tiles_m, tn = tile / tiles_m;
+    f32x4 acc[G::MT][G::NT];
+    G::run(lds0, lds1, h, tm * BM, w, tn * BN, 0, k, acc);
+    const int lane = threadIdx.x & 63;
+    const int64_t left = w.count - tn * BN, rows_left = h.count - tm * BM, part = (tn * BN + G::col0()) / (G::NT * 16);
+    const int levels_here = left < BN ? (int)left : BN, rows_here = rows_left < BM ? (int)rows_left : BM, col = G::col0() + (lane & 15);
+    float *top_here = top + part * h.count + tm * BM, *sum_here = sum + part * h.count + tm * BM, *taken_here = taken + tm * BM;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < G::MT; ++i) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    for (int64_t k0 = 0; k0 < depth; k0 += Tile<T>::BK) {
-        __syncthreads();
-        stage<T>(t.a, a, a0, k0, depth);
-        stage<T>(t.b, b, b0, k0, depth);
-        __syncthreads();
+        for (int r = 0; r < 4; ++r) {
+            const int row = G::row0() + i * 16 + (lane >> 4) * 4 + r;
+            float m = -INFINITY;
 #pragma unroll
-        for (int k = 0; k < Tile<T>::BK; k += M::K) {
-            typename M::Frag fa[2], fb[2];
+            for (int j = 0; j < G::NT; ++j) m = col + j * 16 < levels_here ? fmaxf(m, acc[i][j][r]) : m;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                fa[i] = *(const typename M::Frag*)&t.a[wr + i * 16 + lane % 16][k + (lane / 16) * M::E];
-                fb[i] = *(const typename M::Frag*)&t.b[wc + i * 16 + lane % 16][k + (lane / 16) * M::E];
+            for (int d = 1; d < 16; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
+            float s = 0.0f;
+#pragma unroll
+            for (int j = 0; j < G::NT; ++j) s += col + j * 16 < levels_here ? exp_fast(acc[i][j][r] - m) : 0.0f;
+#pragma unroll
+            for (int d = 1; d < 16; d <<= 1) s += __shfl_xor(s, d);
+            if (row < rows_here) {
+                const int64_t y = target_of(target, target_bytes, tm * BM + row) - tn * BN;
+#pragma unroll
+                for (int j = 0; j < G::NT; ++j)
+                    if (y == col + j * 16 && col + j * 16 < levels_here) taken_here[row] = acc[i][j][r];
+                if ((lane & 15) == 0) {
+                    // (a part wholly behind the last level holds m = -inf, s = 0)
+                    top_here[row] = m;
+                    sum_here[row] = s;
+                }
             }
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) acc[i][j] = M::run(fa[i], fb[j], acc[i][j]);
         }
     }
 }
 
-template <typename F>
-__device__ __forceinline__ void each(f32x4 (&acc)[2][2], F f) {
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, wr = (wave >> 1) * 32, wc = (wave & 1) * 32;
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) f(wr + i * 16 + (lane / 16) * 4 + r, wc + j * 16 + lane % 16, acc[i][j][r]);
-}
-
-
-template <typename T>
-__global__ void __launch_bounds__(256) loss_part_kernel(Operand<T> h, Operand<T> w, int64_t dim, const void* target, int target_bytes, int64_t span, float* top, float* sum,
-                                                        float* taken) {
-    __shared__ Tile<T> t;
-    __shared__ float z[64][65];
-    const int64_t r0 = (int64_t)blockIdx.x * 64, lo = blockIdx.y * span, hi = lo + span < w.rows ? lo + span : w.rows;
-    float m = -INFINITY, s = 0.0f;          // thread r < 64 keeps row r's
-    for (int64_t v0 = lo; v0 < hi; v0 += 64) {
-        f32x4 acc[2][2];
-        multiply<T>(t, h, r0, w, v0, dim, acc);
-        each(acc, [&](int r, int c, float x) { z[r][c] = x; });
-        __syncthreads();
-        const int64_t row = r0 + threadIdx.x;
-        if (threadIdx.x < 64 && row < h.rows) {
-            const int n = hi - v0 < 64 ? (int)(hi - v0) : 64;
-            float now = m;
-            for (int c = 0; c < n; ++c) now = z[threadIdx.x][c] > now || z[threadIdx.x][c] != z[threadIdx.x][c] ? z[threadIdx.x][c] : now;
-            s = m == now ? s : s * expf(m - now);
-            for (int c = 0; c < n; ++c) s += z[threadIdx.x][c] == now && fabsf(now) == INFINITY ? 1.0f : expf(z[threadIdx.x][c] - now);
-            m = now;
-            const int64_t y = target_of(target, target_bytes, row);
-            if (y >= v0 && y < v0 + n) taken[row] = z[threadIdx.x][y - v0];
-        }
-    }
-    const int64_t row = r0 + threadIdx.x;
-    if (threadIdx.x < 64 && row < h.rows) {
-        top[blockIdx.y * h.rows + row] = m;
-        sum[blockIdx.y * h.rows + row] = s;
-    }
-}
-
+// a wave per 4 rows' parts: 16 lanes a row
 __global__ void __launch_bounds__(256) loss_join_kernel(const float* top, const float* sum, const float* taken, const void* target, int target_bytes, int64_t rows,
                                                         int64_t levels, int parts, float* loss, float* lse) {
-    const int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (row >= rows) return;
-    float m = -INFINITY;
-    for (int p = 0; p < parts; ++p) {
-        const float x = top[p * rows + row];
-        m = x > m || x != x ? x : m;
+    // 16 rows x 16 lanes: lane = row within the block's 16 for coalesced reads of [part][row]
+    __shared__ float ms[16][17], ss[16][17];
+    const int r = threadIdx.x & 15, p0 = threadIdx.x >> 4;
+    const int64_t row = (int64_t)blockIdx.x * 16 + r;
+    float m = -INFINITY, s = 0.0f;
+    if (row < rows) {
+        for (int p = p0; p < parts; p += 16) {
+            const float x = top[(int64_t)p * rows + row], y = sum[(int64_t)p * rows + row];
+            const float now = fmaxf(m, x);
+            s = (m == now ? s : s * exp_fast(m - now)) + (x == now ? y : y * exp_fast(x - now));
+            m = now;
+        }
     }
-    float s = 0.0f;
-    for (int p = 0; p < parts; ++p) s += top[p * rows + row] == m ? sum[p * rows + row] : sum[p * rows + row] * expf(top[p * rows + row] - m);
+    ms[p0][r] = m;
+    ss[p0][r] = s;
+    __syncthreads();
+    if (p0 || row >= rows) return;
+    for (int p = 1; p < 16; ++p) {
+        const float x = ms[p][r], y = ss[p][r];
+        const float now = fmaxf(m, x);
+        s = (m == now ? s : s * exp_fast(m - now)) + (x == now ? y : y * exp_fast(x - now));
+        m = now;
+    }
     const float l = m + logf(s);
     lse[row] = l;
-    const int64_t y = target_of(target, target_bytes, row);
-    loss[row] = y >= 0 && y < levels ? l - taken[row] : 0.0f;
+    const int64_t t = target_of(target, target_bytes, row);
+    loss[row] = t >= 0 && t < levels ? l - taken[row] : 0.0f;
 }
 
-// a piece of dz: rows x [v0, v0 + width)
+// ---- backward: dz^T of a piece of the levels, [width padded to BN][ld rows]; zeros behind the rows and the levels ----
+template <typename T, typename G, int BM, int BN>
+__global__ void __launch_bounds__(G::THREADS, 2)
+    loss_dz_kernel(Operand<T> h, Operand<T> w, int64_t k, const void* target, int target_bytes, int64_t levels, int64_t v0, int64_t tiles_m, int64_t tiles_n, const float* lse,
+                   const float* g, T* dzt, int64_t ld) {
+    __shared__ __attribute__((aligned(16))) char lds0[G::BYTES];
+    __shared__ __attribute__((aligned(16))) char lds1[G::BYTES];
+    const int64_t tile = xcd_tile(blockIdx.x, tiles_m * tiles_n);
+    const int64_t tm = tile % tiles_m, tn = tile / tiles_m;
+    f32x4 acc[G::MT][G::NT];
+    G::run(lds0, lds1, h, tm * BM, w, v0 + tn * BN, 0, k, acc);
+    const int lane = threadIdx.x & 63, col = G::col0() + (lane & 15);
+    const int64_t left = levels - v0 - tn * BN, rows_left = h.count - tm * BM, ld_left = ld - tm * BM;
+    const int levels_here = left < BN ? (int)left : BN, rows_here = rows_left < BM ? (int)rows_left : BM, ld_here = ld_left < BM ? (int)ld_left : BM;
+    T* to = dzt + (tn * BN + col) * ld + tm * BM;
+#pragma unroll
+    for (int i = 0; i < G::MT; ++i) {
+        const int row = G::row0() + i * 16 + (lane >> 4) * 4;
+        if (row >= ld_here) continue;
+        float l[4], gr[4];
+        int y[4];                                   // the target's column, or -1 (any other tile's)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int64_t at = tm * BM + row + r, t = row + r < rows_here ? target_of(target, target_bytes, at) : -1;
+            const bool there = t >= 0 && t < levels;
+            l[r] = there ? lse[at] : INFINITY;
+            gr[r] = there ? g[at] : 0.0f;
+            const int64_t rel = t - v0 - tn * BN;
+            y[r] = there && rel >= 0 && rel < BN ? (int)rel : -1;
+        }
+#pragma unroll
+        for (int j = 0; j < G::NT; ++j) {
+            Pack<T, 4> x;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float p = exp_fast(acc[i][j][r] - l[r]) - (y[r] == col + j * 16 ? 1.0f : 0.0f);
+                x.e[r] = from_f32<T>(l[r] == INFINITY || col + j * 16 >= levels_here ? 0.0f : gr[r] * p);
+            }
+            *(Pack<T, 4>*)(to + j * 16 * ld + row) = x;
+        }
+    }
+}
+
+// ---- out[n][m] (+)= sum_k A[m, k] B[n, k] over a share of k: float32 slabs (one per share, added to across pieces) or the type ----
+template <typename T, typename O, typename G, int BM, int BN>
+__global__ void __launch_bounds__(G::THREADS, 2)
+    product_kernel(Operand<T> a, Operand<T> b, int64_t k, int64_t share, int64_t m, int64_t n, int64_t tiles_m, int64_t tiles_n, bool add, O* out, int64_t ld, int64_t slab) {
+    __shared__ __attribute__((aligned(16))) char lds0[G::BYTES];
+    __shared__ __attribute__((aligned(16))) char lds1[G::BYTES];
+    const int64_t tile = xcd_tile(blockIdx.x, tiles_m * tiles_n);
+    const int64_t tm = tile % tiles_m, tn = tile / tiles_m;
+    const int64_t lo = blockIdx.y * share, hi = lo + share < k ? lo + share : k;
+    f32x4 acc[G::MT][G::NT];
+    G::run(lds0, lds1, a, tm * BM, b, tn * BN, lo, hi, acc);
+    const int64_t left_n = n - tn * BN, left_m = m - tm * BM;
+    const int n_here = left_n < BN ? (int)left_n : BN, m_here = left_m < BM ? (int)left_m : BM;
+    O* to = out + blockIdx.y * slab + tn * BN * ld + tm * BM;
+    const bool whole = (ld & 3) == 0 && (((uintptr_t)out) & (4 * sizeof(O) - 1)) == 0;
+    G::each(acc, [&](int r, int c, f32x4 x) {
+        if (c >= n_here || r >= m_here) return;
+        O* p = to + c * ld + r;
+        if (whole && r + 4 <= m_here) {
+            Pack<O, 4> y;
+            if (add) y = *(const Pack<O, 4>*)p;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y.e[e] = from_f32<O>(add ? to_f32(y.e[e]) + x[e] : x[e]);
+            *(Pack<O, 4>*)p = y;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (r + e < m_here) p[e] = from_f32<O>(add ? to_f32(p[e]) + x[e] : x[e]);
+        }
+    });
+}
+
+// out = the shares' slabs added in order
 template <typename T>
-__global__ void __launch_bounds__(256) loss_dz_kernel(Operand<T> h, Operand<T> w, int64_t dim, const void* target, int target_bytes, int64_t levels, int64_t v0,
-                                                      int64_t width, const float* lse, const float* g, T* dz) {
-    __shared__ Tile<T> t;
-    f32x4 acc[2][2];
-    const int64_t r0 = (int64_t)blockIdx.x * 64, c0 = (int64_t)blockIdx.y * 64;
-    multiply<T>(t, h, r0, w, v0 + c0, dim, acc);
-    each(acc, [&](int r, int c, float x) {
-        const int64_t row = r0 + r, col = c0 + c;
-        if (row >= h.rows || col >= width) return;
-        const int64_t y = target_of(target, target_bytes, row);
-        const float p = expf(x - lse[row]) - (y == v0 + col ? 1.0f : 0.0f);
-        dz[row * width + col] = from_f32<T>(y >= 0 && y < levels ? g[row] * p : 0.0f);
-    });
+__global__ void __launch_bounds__(256) slab_sum_kernel(const float* slabs, int64_t slab, int count, T* out, int64_t n) {
+    const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (at >= n) return;
+    if (at + 4 <= n) {
+        f32x4 s = *(const f32x4*)(slabs + at);
+#pragma unroll 8
+        for (int c = 1; c < count; ++c) s += *(const f32x4*)(slabs + c * slab + at);
+        Pack<T, 4> y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y.e[e] = from_f32<T>(s[e]);
+        if (((uintptr_t)(out + at) & (4 * sizeof(T) - 1)) == 0) {
+            *(Pack<T, 4>*)(out + at) = y;
+        } else {
+            for (int e = 0; e < 4; ++e) out[at + e] = y.e[e];
+        }
+        return;
+    }
+    for (int64_t i = at; i < n; ++i) {
+        float s = slabs[i];
+        for (int c = 1; c < count; ++c) s += slabs[c * slab + i];
+        out[i] = from_f32<T>(s);
+    }
 }
 
-// out (+)= A B^T over the depth; to float32 (kept between pieces) or to the type
-template <typename T, typename O, bool ADD>
-__global__ void __launch_bounds__(256) product_kernel(Operand<T> a, Operand<T> b, int64_t depth, const float* before, O* out, int64_t ld) {
-    __shared__ Tile<T> t;
-    f32x4 acc[2][2];
-    const int64_t r0 = (int64_t)blockIdx.x * 64, c0 = (int64_t)blockIdx.y * 64;
-    multiply<T>(t, a, r0, b, c0, depth, acc);
-    each(acc, [&](int r, int c, float x) {
-        const int64_t row = r0 + r, col = c0 + c;
-        if (row >= a.rows || col >= b.rows) return;
-        out[row * ld + col] = from_f32<O>(ADD ? before[row * ld + col] + x : x);
-    });
+template <typename T>
+__global__ void __launch_bounds__(256) zero_kernel(T* p, int64_t n) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i < n) p[i] = from_f32<T>(0.0f);
+}
+
+// ---- the plan: tile sizes, pieces, shares ----
+constexpr int64_t kCUs = 256;
+
+// 256 x 256 tiles read the operands half as often as 128 x 128 ones, but there must be enough of them to fill the chip
+static bool big_tiles(int64_t m, int64_t n) { return ceil_div(m, 256) * ceil_div(n, 256) >= kCUs; }
+
+// how often to split k so that the tiles fill the chip
+static int64_t shares_of(int64_t m, int64_t n, bool big, int64_t k_steps) {
+    const int64_t b = big ? 256 : 128, tiles = ceil_div(m, b) * ceil_div(n, b), slots = big ? kCUs : 2 * kCUs;
+    int64_t s = slots / tiles;
+    if (s < 1) s = 1;
+    const int64_t most = k_steps / 4 > 0 ? k_steps / 4 : 1;
+    return s < most ? s : most;
 }
 
 struct LossPlan {
-    int64_t span, piece;
+    int64_t bk, dim_p, rows_p, piece;       // elements of a staged k step; padded depth and row count; levels of a piece
+    bool big_z;
     int parts;
+    int64_t dh_share, dh_shares, dw_share, dw_shares;
+    bool big_dh, big_dw;
 };
 
-static LossPlan loss_plan(int64_t rows, int64_t levels) {
-    LossPlan p;
-    const int64_t want = ceil_div(2048, ceil_div(rows > 0 ? rows : 1, 64));
-    p.span = round_up(ceil_div(levels, want), 64);
-    p.parts = (int)ceil_div(levels, p.span);
-    p.piece = levels < 16384 ? levels : 16384;
+template <typename T>
+static LossPlan loss_plan(int64_t rows, int64_t levels, int64_t dim) {
+    LossPlan p{};
+    rows = rows > 0 ? rows : 1;
+    p.bk = 128 / (int64_t)sizeof(T);
+    p.dim_p = round_up(dim, p.bk);
+    p.rows_p = round_up(rows, p.bk);
+    const int64_t pieces = ceil_div(levels, 16384);
+    p.piece = pieces == 1 ? levels : round_up(ceil_div(levels, pieces), 256);
+    p.big_z = big_tiles(rows, p.piece);
+    p.parts = (int)(p.big_z ? ceil_div(levels, 256) * 4 : ceil_div(levels, 128) * 2);
+    const int64_t dh_k = round_up(p.piece, p.bk);
+    p.big_dh = ceil_div(dim, 256) * ceil_div(rows, 256) * (dh_k / p.bk / 8) >= kCUs && dim > 128;
+    p.dh_shares = shares_of(dim, rows, p.big_dh, dh_k / p.bk);
+    p.dh_share = round_up(ceil_div(dh_k, p.dh_shares), p.bk);
+    p.dh_shares = ceil_div(dh_k, p.dh_share);
+    p.big_dw = ceil_div(dim, 256) * ceil_div(p.piece, 256) * (p.rows_p / p.bk / 8) >= kCUs && dim > 128;
+    p.dw_shares = shares_of(dim, p.piece, p.big_dw, p.rows_p / p.bk);
+    p.dw_share = round_up(ceil_div(p.rows_p, p.dw_shares), p.bk);
+    p.dw_shares = ceil_div(p.rows_p, p.dw_share);
     return p;
 }
 
+template <typename T>
 struct LossWork {
-    float *top, *sum, *taken, *dh;
-    void* dz;
-    int64_t bytes;
+    float *top = nullptr, *sum = nullptr, *taken = nullptr, *dh = nullptr, *dw = nullptr;
+    T *h = nullptr, *w = nullptr, *dzt = nullptr;
+    int64_t dh_slab = 0, dw_slab = 0, bytes = 0;
 };
 
-static LossWork loss_work(const LossPlan& p, int64_t size, int64_t rows, int64_t levels, int64_t dim, bool backward, void* at) {
+// the padded copies are counted whether the operands need them or not: the caller asks before the pointers are known
+template <typename T>
+static LossWork<T> loss_work(const LossPlan& p, int64_t rows, int64_t levels, int64_t dim, bool backward, void* at) {
     Carve c(at);
-    LossWork w{};
+    LossWork<T> w;
+    w.h = c.take<T>(rows * p.dim_p);
+    w.w = c.take<T>(levels * p.dim_p);
     if (backward) {
-        w.dz = c.take<char>(rows * p.piece * size);
-        w.dh = c.take<float>(p.piece < levels ? rows * dim : 0);
+        w.dzt = c.take<T>(round_up(p.piece, 256) * p.rows_p);
+        w.dh_slab = round_up(rows * dim, 4);
+        w.dw_slab = round_up(p.piece * dim, 4);
+        if (p.dh_shares > 1 || p.piece < levels) w.dh = c.take<float>(p.dh_shares * w.dh_slab);
+        if (p.dw_shares > 1) w.dw = c.take<float>(p.dw_shares * w.dw_slab);
     } else {
         w.top = c.take<float>(rows * p.parts);
         w.sum = c.take<float>(rows * p.parts);
@@ -209,58 +306,94 @@ static LossWork loss_work(const LossPlan& p, int64_t size, int64_t rows, int64_t
 static int loss_check(int32_t dtype, int64_t rows, int64_t levels, int64_t dim) {
     if (dtype != FISHING_DTYPE_F32 && dtype != FISHING_DTYPE_BF16) return FISHING_ERR_UNSUPPORTED;
     if (rows < 0 || rows > 0x7fffffff || levels < 1 || levels > 0x7ffffff || dim < 1 || dim > 65536) return FISHING_ERR_SIZE;
+    if (ceil_div(rows, 128) * ceil_div(levels, 128) > 0x7fffffff || ceil_div(rows, 128) * ceil_div(dim, 128) > 0x7fffffff) return FISHING_ERR_SIZE;    // workgroups of a launch
     return FISHING_OK;
+}
+
+template <typename T>
+using Big = Gemm<T, 256, 256, 2, 4, false, false>;
+template <typename T>
+using Small = Gemm<T, 128, 128, 2, 2, false, false>;
+
+template <typename T>
+static int pad(const T* src, int64_t ld, int64_t rows, int64_t width, T* dst, int64_t padded, const void* target, int target_bytes, int64_t levels, hipStream_t stream) {
+    return launch(pad_kernel<T>, dim3((unsigned)ceil_div(rows * (padded / vec_of<T>()), 256)), dim3(256), stream, src, ld, rows, (int32_t)width, dst, (int32_t)padded, target,
+                  target_bytes, levels);
+}
+
+// the operand as it is where its rows are whole k steps at 16-byte addresses, its padded copy otherwise
+template <typename T>
+static int padded_operand(const LossPlan& p, const T* src, int64_t ld, int64_t rows, int64_t dim, T* copy, Operand<T>& o, hipStream_t stream) {
+    if (dim == p.dim_p && ld % vec_of<T>() == 0 && aligned16(src)) {
+        o = Operand<T>{src, ld, rows, rows};
+        return 0;
+    }
+    o = Operand<T>{copy, p.dim_p, rows, rows};
+    return pad<T>(src, ld, rows, dim, copy, p.dim_p, nullptr, 4, 0, stream);
 }
 
 template <typename T>
 static int loss_forward(int64_t rows, int64_t levels, int64_t dim, const T* h, int64_t h_ld, const T* w, int64_t w_ld, const void* target, int target_bytes, float* loss,
                         float* lse, void* workspace, hipStream_t stream) {
-    const LossPlan p = loss_plan(rows, levels);
-    const LossWork k = loss_work(p, sizeof(T), rows, levels, dim, false, workspace);
-    const Operand<T> a{h, h_ld, rows, false}, b{w, w_ld, levels, false};
-    int rc = launch(loss_part_kernel<T>, dim3((unsigned)ceil_div(rows, 64), (unsigned)p.parts), dim3(256), stream, a, b, dim, target, target_bytes, p.span, k.top, k.sum, k.taken);
+    const LossPlan p = loss_plan<T>(rows, levels, dim);
+    const LossWork<T> k = loss_work<T>(p, rows, levels, dim, false, workspace);
+    Operand<T> a, b;
+    int rc = padded_operand<T>(p, h, h_ld, rows, dim, k.h, a, stream);
+    if (!rc) rc = padded_operand<T>(p, w, w_ld, levels, dim, k.w, b, stream);
+    if (rc) return rc;
+    const int64_t t = p.big_z ? 256 : 128, tm = ceil_div(rows, t), tn = ceil_div(levels, t);
+    rc = p.big_z ? launch(loss_part_kernel<T, Big<T>, 256, 256>, dim3((unsigned)(tm * tn)), dim3(512), stream, a, b, p.dim_p, target, target_bytes, tm, tn, k.top, k.sum, k.taken)
+                 : launch(loss_part_kernel<T, Small<T>, 128, 128>, dim3((unsigned)(tm * tn)), dim3(256), stream, a, b, p.dim_p, target, target_bytes, tm, tn, k.top, k.sum, k.taken);
     if (!rc)
-        rc = launch(loss_join_kernel, dim3((unsigned)ceil_div(rows, 256)), dim3(256), stream, k.top, k.sum, k.taken, target, target_bytes, rows, levels, p.parts, loss, lse);
+        rc = launch(loss_join_kernel, dim3((unsigned)ceil_div(rows, 16)), dim3(256), stream, k.top, k.sum, k.taken, target, target_bytes, rows, levels, p.parts, loss, lse);
     return rc;
+}
+
+template <typename T, typename O, bool A_MAJOR, bool B_MAJOR>
+static int product(const Operand<T>& a, const Operand<T>& b, bool big, int64_t k, int64_t share, int64_t shares, int64_t m, int64_t n, bool add, O* out, int64_t ld, int64_t slab,
+                   hipStream_t stream) {
+    const int64_t t = big ? 256 : 128, tm = ceil_div(m, t), tn = ceil_div(n, t);
+    const dim3 grid((unsigned)(tm * tn), (unsigned)shares);
+    if (big)
+        return launch(product_kernel<T, O, Gemm<T, 256, 256, 2, 4, A_MAJOR, B_MAJOR>, 256, 256>, grid, dim3(512), stream, a, b, k, share, m, n, tm, tn, add, out, ld, slab);
+    return launch(product_kernel<T, O, Gemm<T, 128, 128, 2, 2, A_MAJOR, B_MAJOR>, 128, 128>, grid, dim3(256), stream, a, b, k, share, m, n, tm, tn, add, out, ld, slab);
 }
 
 template <typename T>
 static int loss_backward(int64_t rows, int64_t levels, int64_t dim, const T* h, int64_t h_ld, const T* w, int64_t w_ld, const void* target, int target_bytes, const float* lse,
                          const float* g, T* dh, T* dw, void* workspace, hipStream_t stream) {
-    const LossPlan p = loss_plan(rows, levels);
-    const LossWork k = loss_work(p, sizeof(T), rows, levels, dim, true, workspace);
-    T* dz = (T*)k.dz;
-    const Operand<T> a{h, h_ld, rows, false};
-    int rc = 0;
+    const LossPlan p = loss_plan<T>(rows, levels, dim);
+    const LossWork<T> k = loss_work<T>(p, rows, levels, dim, true, workspace);
+    Operand<T> a{k.h, p.dim_p, rows, rows}, b;
+    int rc = pad<T>(h, h_ld, rows, dim, k.h, p.dim_p, target, target_bytes, levels, stream);
+    if (!rc) rc = padded_operand<T>(p, w, w_ld, levels, dim, k.w, b, stream);
     for (int64_t v0 = 0; v0 < levels && !rc; v0 += p.piece) {
-        const int64_t width = levels - v0 < p.piece ? levels - v0 : p.piece;
-        const bool first = v0 == 0, last = v0 + width == levels;
-        const Operand<T> all{w, w_ld, levels, false}, rowwise{dz, width, rows, false}, levelwise{dz, width, width, true};
-        const Operand<T> w_dim{w + v0 * w_ld, w_ld, dim, true}, h_dim{h, h_ld, dim, true, target, target_bytes, levels};
-        rc = launch(loss_dz_kernel<T>, dim3((unsigned)ceil_div(rows, 64), (unsigned)ceil_div(width, 64)), dim3(256), stream, a, all, dim, target, target_bytes, levels, v0, width,
-                    lse, g, dz);
-        const dim3 grid((unsigned)ceil_div(rows, 64), (unsigned)ceil_div(dim, 64));
-        if (!rc) {
-            if (first && last)
-                rc = launch(product_kernel<T, T, false>, grid, dim3(256), stream, rowwise, w_dim, width, k.dh, dh, dim);
-            else if (first)
-                rc = launch(product_kernel<T, float, false>, grid, dim3(256), stream, rowwise, w_dim, width, k.dh, k.dh, dim);
-            else if (!last)
-                rc = launch(product_kernel<T, float, true>, grid, dim3(256), stream, rowwise, w_dim, width, k.dh, k.dh, dim);
-            else
-                rc = launch(product_kernel<T, T, true>, grid, dim3(256), stream, rowwise, w_dim, width, k.dh, dh, dim);
+        const int64_t width = levels - v0 < p.piece ? levels - v0 : p.piece, width_p = round_up(width, p.bk);
+        const int64_t t = p.big_z ? 256 : 128, tm = ceil_div(rows, t), tn = ceil_div(width, t);
+        rc = p.big_z ? launch(loss_dz_kernel<T, Big<T>, 256, 256>, dim3((unsigned)(tm * tn)), dim3(512), stream, a, b, p.dim_p, target, target_bytes, levels, v0, tm, tn, lse, g,
+                              k.dzt, p.rows_p)
+                     : launch(loss_dz_kernel<T, Small<T>, 128, 128>, dim3((unsigned)(tm * tn)), dim3(256), stream, a, b, p.dim_p, target, target_bytes, levels, v0, tm, tn, lse, g,
+                              k.dzt, p.rows_p);
+        if (rc) break;
+        // dh[r][d]: m = d, n = r, k = the piece's levels, both operands k-major; W's rows beyond the last meet zeros of dz
+        const Operand<T> wd{b.p + v0 * b.ld, b.ld, p.dim_p, width}, zr{k.dzt, p.rows_p, p.rows_p, width_p};
+        if (k.dh)
+            rc = product<T, float, true, true>(wd, zr, p.big_dh, width_p, p.dh_share, p.dh_shares, dim, rows, v0 > 0, k.dh, dim, k.dh_slab, stream);
+        else
+            rc = product<T, T, true, true>(wd, zr, p.big_dh, width_p, p.dh_share, 1, dim, rows, false, dh, dim, 0, stream);
+        if (rc) break;
+        // dW[v][d]: m = d, n = v, k = rows; h's rows beyond the last meet zeros of dz
+        const Operand<T> hd{k.h, p.dim_p, p.dim_p, rows}, zv{k.dzt, p.rows_p, width, width};
+        if (k.dw) {
+            rc = product<T, float, true, false>(hd, zv, p.big_dw, p.rows_p, p.dw_share, p.dw_shares, dim, width, false, k.dw, dim, k.dw_slab, stream);
+            if (!rc)
+                rc = launch(slab_sum_kernel<T>, dim3((unsigned)ceil_div(width * dim, 1024)), dim3(256), stream, k.dw, k.dw_slab, (int)p.dw_shares, dw + v0 * dim, width * dim);
+        } else {
+            rc = product<T, T, true, false>(hd, zv, p.big_dw, p.rows_p, p.dw_share, 1, dim, width, false, dw + v0 * dim, dim, 0, stream);
         }
-        if (!rc)
-            rc = launch(product_kernel<T, T, false>, dim3((unsigned)ceil_div(width, 64), (unsigned)ceil_div(dim, 64)), dim3(256), stream, levelwise, h_dim, rows, k.dh,
-                        dw + v0 * dim, dim);
     }
+    if (!rc && k.dh) rc = launch(slab_sum_kernel<T>, dim3((unsigned)ceil_div(rows * dim, 1024)), dim3(256), stream, k.dh, k.dh_slab, (int)p.dh_shares, dh, rows * dim);
     return rc;
-}
-
-template <typename T>
-__global__ void __launch_bounds__(256) zero_kernel(T* p, int64_t n) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i < n) p[i] = from_f32<T>(0.0f);
 }
 
 }  // namespace seq
@@ -272,7 +405,8 @@ extern "C" {
 
 int64_t fishing_cross_entropy_workspace(int32_t dtype, int64_t rows, int64_t levels, int64_t dim, int32_t backward) {
     if (int rc = loss_check(dtype, rows, levels, dim)) return rc;
-    return loss_work(loss_plan(rows, levels), dtype == FISHING_DTYPE_F32 ? 4 : 2, rows, levels, dim, backward != 0, nullptr).bytes;
+    return dtype == FISHING_DTYPE_F32 ? loss_work<float>(loss_plan<float>(rows, levels, dim), rows, levels, dim, backward != 0, nullptr).bytes
+                                      : loss_work<bf16>(loss_plan<bf16>(rows, levels, dim), rows, levels, dim, backward != 0, nullptr).bytes;
 }
 
 int fishing_cross_entropy_forward(int32_t dtype, int32_t target_bytes, int64_t rows, int64_t levels, int64_t dim, const void* hidden, int64_t hidden_stride, const void* head,
