@@ -19,6 +19,24 @@ __device__ __forceinline__ int64_t target_of(const void* target, int bytes, int6
 constexpr float kLog2E = 1.4426950408889634f;
 __device__ __forceinline__ float exp_fast(float x) { return __builtin_amdgcn_exp2f(x * kLog2E); }
 
+// over the 16 lanes of a row of the accumulator (DPP rotations: no trip through LDS)
+template <int N>
+__device__ __forceinline__ float rotated(float x) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x120 | N, 0xf, 0xf, false));
+}
+__device__ __forceinline__ float max16(float x) {
+    x = fmaxf(x, rotated<8>(x));
+    x = fmaxf(x, rotated<4>(x));
+    x = fmaxf(x, rotated<2>(x));
+    return fmaxf(x, rotated<1>(x));
+}
+__device__ __forceinline__ float sum16(float x) {
+    x += rotated<8>(x);
+    x += rotated<4>(x);
+    x += rotated<2>(x);
+    return x + rotated<1>(x);
+}
+
 // rows of `width` to rows of `padded`, zeros behind; rows of padded targets become zeros, whatever they hold (NaN times a zero dz is NaN)
 template <typename T>
 __global__ void __launch_bounds__(256) pad_kernel(const T* src, int64_t ld, int64_t rows, int32_t width, T* dst, int32_t padded, const void* target, int target_bytes,
@@ -53,68 +71,83 @@ __global__ void __launch_bounds__(G::THREADS, 2)
     __shared__ __attribute__((aligned(16))) char lds1[G::BYTES];
     const int64_t tile = xcd_tile(blockIdx.x, tiles_m * tiles_n);
     const int64_t tm = tile % tiles_m, tn = tile / tiles_m;
+    // the target's column in this tile, or -1; read behind the product's barriers
+    __shared__ int column[BM];
+    if (threadIdx.x < BM) {
+        const int64_t row = tm * BM + threadIdx.x;
+        const int64_t y = row < h.count ? target_of(target, target_bytes, row) - tn * BN : -1;
+        column[threadIdx.x] = y >= 0 && y < BN ? (int)y : -1;
+    }
     f32x4 acc[G::MT][G::NT];
     G::run(lds0, lds1, h, tm * BM, w, tn * BN, 0, k, acc);
     const int lane = threadIdx.x & 63;
     const int64_t left = w.count - tn * BN, rows_left = h.count - tm * BM, part = (tn * BN + G::col0()) / (G::NT * 16);
     const int levels_here = left < BN ? (int)left : BN, rows_here = rows_left < BM ? (int)rows_left : BM, col = G::col0() + (lane & 15);
     float *top_here = top + part * h.count + tm * BM, *sum_here = sum + part * h.count + tm * BM, *taken_here = taken + tm * BM;
+    const bool whole = levels_here == BN;
 #pragma unroll
     for (int i = 0; i < G::MT; ++i) {
+        const int row = G::row0() + i * 16 + (lane >> 4) * 4;
+        const int4 y = *(const int4*)&column[row];
+        const int ys[4] = {y.x, y.y, y.z, y.w};
+        float m[4], s[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int row = G::row0() + i * 16 + (lane >> 4) * 4 + r;
-            float m = -INFINITY;
+            if (!whole) {
 #pragma unroll
-            for (int j = 0; j < G::NT; ++j) m = col + j * 16 < levels_here ? fmaxf(m, acc[i][j][r]) : m;
+                for (int j = 0; j < G::NT; ++j) acc[i][j][r] = col + j * 16 < levels_here ? acc[i][j][r] : -INFINITY;
+            }
+            m[r] = acc[i][0][r];
 #pragma unroll
-            for (int d = 1; d < 16; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
-            float s = 0.0f;
+            for (int j = 1; j < G::NT; ++j) m[r] = fmaxf(m[r], acc[i][j][r]);
+            m[r] = max16(m[r]);
+            const float from = m[r] == -INFINITY ? 0.0f : m[r];      // (a part wholly behind the last level: m = -inf, s = 0)
+            s[r] = 0.0f;
 #pragma unroll
-            for (int j = 0; j < G::NT; ++j) s += col + j * 16 < levels_here ? exp_fast(acc[i][j][r] - m) : 0.0f;
+            for (int j = 0; j < G::NT; ++j) s[r] += exp_fast(acc[i][j][r] - from);
+            s[r] = sum16(s[r]);
 #pragma unroll
-            for (int d = 1; d < 16; d <<= 1) s += __shfl_xor(s, d);
-            if (row < rows_here) {
-                const int64_t y = target_of(target, target_bytes, tm * BM + row) - tn * BN;
+            for (int j = 0; j < G::NT; ++j)
+                if (ys[r] == col + j * 16) taken_here[row + r] = acc[i][j][r];
+        }
+        if ((lane & 15) == 0) {
 #pragma unroll
-                for (int j = 0; j < G::NT; ++j)
-                    if (y == col + j * 16 && col + j * 16 < levels_here) taken_here[row] = acc[i][j][r];
-                if ((lane & 15) == 0) {
-                    // (a part wholly behind the last level holds m = -inf, s = 0)
-                    top_here[row] = m;
-                    sum_here[row] = s;
+            for (int r = 0; r < 4; ++r) {
+                if (row + r < rows_here) {
+                    top_here[row + r] = m[r];
+                    sum_here[row + r] = s[r];
                 }
             }
         }
     }
 }
 
-// a wave per 4 rows' parts: 16 lanes a row
-__global__ void __launch_bounds__(256) loss_join_kernel(const float* top, const float* sum, const float* taken, const void* target, int target_bytes, int64_t rows,
-                                                        int64_t levels, int parts, float* loss, float* lse) {
-    // 16 rows x 16 lanes: lane = row within the block's 16 for coalesced reads of [part][row]
-    __shared__ float ms[16][17], ss[16][17];
-    const int r = threadIdx.x & 15, p0 = threadIdx.x >> 4;
-    const int64_t row = (int64_t)blockIdx.x * 16 + r;
+// (m, s) <- the pair of two parts
+__device__ __forceinline__ void join(float& m, float& s, float x, float y) {
+    const float now = fmaxf(m, x);
+    s = (m == now ? s : s * exp_fast(m - now)) + (x == now ? y : y * exp_fast(x - now));
+    m = now;
+}
+
+// R rows x L lanes a row: lane p0 joins parts p0, p0 + L, ..., the row's first lane the lanes'.  Many parts (few rows against many
+// levels) take many lanes: 17 rows, 1026 parts: 22.7 us with 16 lanes
+template <int R, int L>
+__global__ void __launch_bounds__(R* L) loss_join_kernel(const float* top, const float* sum, const float* taken, const void* target, int target_bytes, int64_t rows,
+                                                         int64_t levels, int parts, float* loss, float* lse) {
+    __shared__ float ms[L][R + 1], ss[L][R + 1];
+    const int r = threadIdx.x % R, p0 = threadIdx.x / R;
+    const int64_t row = (int64_t)blockIdx.x * R + r;
     float m = -INFINITY, s = 0.0f;
     if (row < rows) {
-        for (int p = p0; p < parts; p += 16) {
-            const float x = top[(int64_t)p * rows + row], y = sum[(int64_t)p * rows + row];
-            const float now = fmaxf(m, x);
-            s = (m == now ? s : s * exp_fast(m - now)) + (x == now ? y : y * exp_fast(x - now));
-            m = now;
-        }
+#pragma unroll 4
+        for (int p = p0; p < parts; p += L) join(m, s, top[(int64_t)p * rows + row], sum[(int64_t)p * rows + row]);
     }
     ms[p0][r] = m;
     ss[p0][r] = s;
     __syncthreads();
     if (p0 || row >= rows) return;
-    for (int p = 1; p < 16; ++p) {
-        const float x = ms[p][r], y = ss[p][r];
-        const float now = fmaxf(m, x);
-        s = (m == now ? s : s * exp_fast(m - now)) + (x == now ? y : y * exp_fast(x - now));
-        m = now;
-    }
+#pragma unroll 4
+    for (int p = 1; p < L; ++p) join(m, s, ms[p][r], ss[p][r]);
     const float l = m + logf(s);
     lse[row] = l;
     const int64_t t = target_of(target, target_bytes, row);
@@ -130,27 +163,31 @@ __global__ void __launch_bounds__(G::THREADS, 2)
     __shared__ __attribute__((aligned(16))) char lds1[G::BYTES];
     const int64_t tile = xcd_tile(blockIdx.x, tiles_m * tiles_n);
     const int64_t tm = tile % tiles_m, tn = tile / tiles_m;
+    // per row of the tile, read behind the product's barriers: lse (infinite for a padded target: a share of zero), the loss's
+    // gradient, the target's column or -1
+    __shared__ float row_lse[BM], row_g[BM];
+    __shared__ int row_y[BM];
+    if (threadIdx.x < BM) {
+        const int64_t row = tm * BM + threadIdx.x, t = row < h.count ? target_of(target, target_bytes, row) : -1;
+        const bool there = t >= 0 && t < levels;
+        const int64_t rel = t - v0 - tn * BN;
+        row_lse[threadIdx.x] = there ? lse[row] : INFINITY;
+        row_g[threadIdx.x] = there ? g[row] : 0.0f;
+        row_y[threadIdx.x] = there && rel >= 0 && rel < BN ? (int)rel : -1;
+    }
     f32x4 acc[G::MT][G::NT];
     G::run(lds0, lds1, h, tm * BM, w, v0 + tn * BN, 0, k, acc);
     const int lane = threadIdx.x & 63, col = G::col0() + (lane & 15);
-    const int64_t left = levels - v0 - tn * BN, rows_left = h.count - tm * BM, ld_left = ld - tm * BM;
-    const int levels_here = left < BN ? (int)left : BN, rows_here = rows_left < BM ? (int)rows_left : BM, ld_here = ld_left < BM ? (int)ld_left : BM;
+    const int64_t left = levels - v0 - tn * BN, ld_left = ld - tm * BM;
+    const int levels_here = left < BN ? (int)left : BN, ld_here = ld_left < BM ? (int)ld_left : BM;
     T* to = dzt + (tn * BN + col) * ld + tm * BM;
 #pragma unroll
     for (int i = 0; i < G::MT; ++i) {
         const int row = G::row0() + i * 16 + (lane >> 4) * 4;
         if (row >= ld_here) continue;
-        float l[4], gr[4];
-        int y[4];                                   // the target's column, or -1 (any other tile's)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int64_t at = tm * BM + row + r, t = row + r < rows_here ? target_of(target, target_bytes, at) : -1;
-            const bool there = t >= 0 && t < levels;
-            l[r] = there ? lse[at] : INFINITY;
-            gr[r] = there ? g[at] : 0.0f;
-            const int64_t rel = t - v0 - tn * BN;
-            y[r] = there && rel >= 0 && rel < BN ? (int)rel : -1;
-        }
+        const f32x4 l = *(const f32x4*)&row_lse[row], gr = *(const f32x4*)&row_g[row];
+        const int4 y4 = *(const int4*)&row_y[row];
+        const int y[4] = {y4.x, y4.y, y4.z, y4.w};
 #pragma unroll
         for (int j = 0; j < G::NT; ++j) {
             Pack<T, 4> x;
@@ -196,30 +233,40 @@ __global__ void __launch_bounds__(G::THREADS, 2)
     });
 }
 
-// out = the shares' slabs added in order
-template <typename T>
+// out = the shares' slabs added in order: L lanes take every L-th slab, their sums are added in the lanes' order
+template <typename T, int L>
 __global__ void __launch_bounds__(256) slab_sum_kernel(const float* slabs, int64_t slab, int count, T* out, int64_t n) {
-    const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
-    if (at >= n) return;
-    if (at + 4 <= n) {
-        f32x4 s = *(const f32x4*)(slabs + at);
+    constexpr int C = 256 / L;
+    __shared__ f32x4 lane_sum[L][C];
+    const int c = threadIdx.x % C, l = threadIdx.x / C;
+    const int64_t at = ((int64_t)blockIdx.x * C + c) * 4;
+    f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (at < n) {                                         // (a slab is padded to whole quads)
 #pragma unroll 8
-        for (int c = 1; c < count; ++c) s += *(const f32x4*)(slabs + c * slab + at);
+        for (int i = l; i < count; i += L) s += *(const f32x4*)(slabs + i * slab + at);
+    }
+    if (L > 1) {
+        lane_sum[l][c] = s;
+        __syncthreads();
+        if (l) return;
+#pragma unroll
+        for (int i = 1; i < L; ++i) s += lane_sum[i][c];
+    }
+    if (at >= n) return;
+    if (at + 4 <= n && ((uintptr_t)(out + at) & (4 * sizeof(T) - 1)) == 0) {
         Pack<T, 4> y;
 #pragma unroll
         for (int e = 0; e < 4; ++e) y.e[e] = from_f32<T>(s[e]);
-        if (((uintptr_t)(out + at) & (4 * sizeof(T) - 1)) == 0) {
-            *(Pack<T, 4>*)(out + at) = y;
-        } else {
-            for (int e = 0; e < 4; ++e) out[at + e] = y.e[e];
-        }
-        return;
+        *(Pack<T, 4>*)(out + at) = y;
+    } else {
+        for (int e = 0; e < 4 && at + e < n; ++e) out[at + e] = from_f32<T>(s[e]);
     }
-    for (int64_t i = at; i < n; ++i) {
-        float s = slabs[i];
-        for (int c = 1; c < count; ++c) s += slabs[c * slab + i];
-        out[i] = from_f32<T>(s);
-    }
+}
+
+template <typename T>
+static int slab_sum(const float* slabs, int64_t slab, int64_t count, T* out, int64_t n, hipStream_t stream) {
+    if (count >= 32) return launch(slab_sum_kernel<T, 16>, dim3((unsigned)ceil_div(n, 64)), dim3(256), stream, slabs, slab, (int)count, out, n);
+    return launch(slab_sum_kernel<T, 1>, dim3((unsigned)ceil_div(n, 1024)), dim3(256), stream, slabs, slab, (int)count, out, n);
 }
 
 template <typename T>
@@ -232,7 +279,7 @@ __global__ void __launch_bounds__(256) zero_kernel(T* p, int64_t n) {
 constexpr int64_t kCUs = 256;
 
 // 256 x 256 tiles read the operands half as often as 128 x 128 ones, but there must be enough of them to fill the chip
-static bool big_tiles(int64_t m, int64_t n) { return ceil_div(m, 256) * ceil_div(n, 256) >= kCUs; }
+static bool big_tiles(int64_t m, int64_t n) { return m > 128 && n > 128 && ceil_div(m, 256) * ceil_div(n, 256) >= kCUs; }
 
 // how often to split k so that the tiles fill the chip
 static int64_t shares_of(int64_t m, int64_t n, bool big, int64_t k_steps) {
@@ -344,9 +391,11 @@ static int loss_forward(int64_t rows, int64_t levels, int64_t dim, const T* h, i
     const int64_t t = p.big_z ? 256 : 128, tm = ceil_div(rows, t), tn = ceil_div(levels, t);
     rc = p.big_z ? launch(loss_part_kernel<T, Big<T>, 256, 256>, dim3((unsigned)(tm * tn)), dim3(512), stream, a, b, p.dim_p, target, target_bytes, tm, tn, k.top, k.sum, k.taken)
                  : launch(loss_part_kernel<T, Small<T>, 128, 128>, dim3((unsigned)(tm * tn)), dim3(256), stream, a, b, p.dim_p, target, target_bytes, tm, tn, k.top, k.sum, k.taken);
-    if (!rc)
-        rc = launch(loss_join_kernel, dim3((unsigned)ceil_div(rows, 16)), dim3(256), stream, k.top, k.sum, k.taken, target, target_bytes, rows, levels, p.parts, loss, lse);
-    return rc;
+    if (rc) return rc;
+    auto join_parts = [&](auto kernel, int r, int l) {
+        return launch(kernel, dim3((unsigned)ceil_div(rows, r)), dim3(r * l), stream, k.top, k.sum, k.taken, target, target_bytes, rows, levels, p.parts, loss, lse);
+    };
+    return p.parts <= 8 ? join_parts(loss_join_kernel<256, 1>, 256, 1) : p.parts <= 64 ? join_parts(loss_join_kernel<32, 8>, 32, 8) : join_parts(loss_join_kernel<16, 64>, 16, 64);
 }
 
 template <typename T, typename O, bool A_MAJOR, bool B_MAJOR>
@@ -387,12 +436,12 @@ static int loss_backward(int64_t rows, int64_t levels, int64_t dim, const T* h, 
         if (k.dw) {
             rc = product<T, float, true, false>(hd, zv, p.big_dw, p.rows_p, p.dw_share, p.dw_shares, dim, width, false, k.dw, dim, k.dw_slab, stream);
             if (!rc)
-                rc = launch(slab_sum_kernel<T>, dim3((unsigned)ceil_div(width * dim, 1024)), dim3(256), stream, k.dw, k.dw_slab, (int)p.dw_shares, dw + v0 * dim, width * dim);
+                rc = slab_sum<T>(k.dw, k.dw_slab, p.dw_shares, dw + v0 * dim, width * dim, stream);
         } else {
             rc = product<T, T, true, false>(hd, zv, p.big_dw, p.rows_p, p.dw_share, 1, dim, width, false, dw + v0 * dim, dim, 0, stream);
         }
     }
-    if (!rc && k.dh) rc = launch(slab_sum_kernel<T>, dim3((unsigned)ceil_div(rows * dim, 1024)), dim3(256), stream, k.dh, k.dh_slab, (int)p.dh_shares, dh, rows * dim);
+    if (!rc && k.dh) rc = slab_sum<T>(k.dh, k.dh_slab, p.dh_shares, dh, rows * dim, stream);
     return rc;
 }
 
