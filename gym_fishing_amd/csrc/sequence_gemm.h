@@ -36,7 +36,8 @@ struct Stage {
     static constexpr int RB = BM * (int)sizeof(T), CPR = RB / 16;    // k-major: bytes, chunks of a row
     static_assert(CHUNKS % THREADS == 0, "whole waves of loads");
 
-    static __device__ __forceinline__ int unit_swizzle(int k) { return sizeof(T) == 2 ? (k & 3) | ((k >> 3 & 1) << 2) : (k >> 2) & 3; }
+    static constexpr int UNITS = RB / (sizeof(T) == 2 ? 32 : 64);    // k-major: swizzled units of a row
+    static __device__ __forceinline__ int unit_swizzle(int k) { return (sizeof(T) == 2 ? (k & 3) | ((k >> 3 & 1) << 2) : (k >> 2) & 3) & (UNITS - 1); }
 
     // The tile's corner is uniform (scalar registers); a lane's offset from it fits 32 bits
     static __device__ __forceinline__ void load(char* lds, const Operand<T>& o, int64_t m0, int64_t k0) {
@@ -76,30 +77,45 @@ struct Stage {
             }
         } else if constexpr (sizeof(T) == 2) {
             // In assembly because the compiler takes the builtin for a reader of the buffer that is being filled and waits for the
-            // loads in flight.  Four tiles a block, the wait inside it.
-            static_assert(N % 4 == 0, "blocks of four tiles");
+            // loads in flight.  Four (two) tiles a block, the wait inside it.
+            static_assert(N % 2 == 0, "blocks of two tiles");
             const int k = 8 * g + (i >> 2);
             const uint32_t row = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)lds + k * RB + ((i & 3) << 3);
+            union Two {
+                uint64_t h[2];
+                bf16x8 f;
+            };
+            auto at = [&](int n) { return row + ((((m0 >> 4) + n) ^ unit_swizzle(k)) << 5); };
+            if constexpr (N % 4 == 0) {
 #pragma unroll
-            for (int n = 0; n < N; n += 4) {
-                uint32_t at[4];
+                for (int n = 0; n < N; n += 4) {
+                    Two r[4];
+                    asm volatile(
+                        "ds_read_b64_tr_b16 %0, %8 offset:%12\n\tds_read_b64_tr_b16 %1, %8 offset:%13\n\t"
+                        "ds_read_b64_tr_b16 %2, %9 offset:%12\n\tds_read_b64_tr_b16 %3, %9 offset:%13\n\t"
+                        "ds_read_b64_tr_b16 %4, %10 offset:%12\n\tds_read_b64_tr_b16 %5, %10 offset:%13\n\t"
+                        "ds_read_b64_tr_b16 %6, %11 offset:%12\n\tds_read_b64_tr_b16 %7, %11 offset:%13\n\t"
+                        "s_waitcnt lgkmcnt(0)"
+                        : "=&v"(r[0].h[0]), "=&v"(r[0].h[1]), "=&v"(r[1].h[0]), "=&v"(r[1].h[1]), "=&v"(r[2].h[0]), "=&v"(r[2].h[1]), "=&v"(r[3].h[0]), "=&v"(r[3].h[1])
+                        : "v"(at(n)), "v"(at(n + 1)), "v"(at(n + 2)), "v"(at(n + 3)), "n"(S * 32 * RB), "n"((S * 32 + 4) * RB)
+                        : "memory");
 #pragma unroll
-                for (int x = 0; x < 4; ++x) at[x] = row + ((((m0 >> 4) + n + x) ^ unit_swizzle(k)) << 5);
-                union Two {
-                    uint64_t h[2];
-                    bf16x8 f;
-                } r[4];
-                asm volatile(
-                    "ds_read_b64_tr_b16 %0, %8 offset:%12\n\tds_read_b64_tr_b16 %1, %8 offset:%13\n\t"
-                    "ds_read_b64_tr_b16 %2, %9 offset:%12\n\tds_read_b64_tr_b16 %3, %9 offset:%13\n\t"
-                    "ds_read_b64_tr_b16 %4, %10 offset:%12\n\tds_read_b64_tr_b16 %5, %10 offset:%13\n\t"
-                    "ds_read_b64_tr_b16 %6, %11 offset:%12\n\tds_read_b64_tr_b16 %7, %11 offset:%13\n\t"
-                    "s_waitcnt lgkmcnt(0)"
-                    : "=&v"(r[0].h[0]), "=&v"(r[0].h[1]), "=&v"(r[1].h[0]), "=&v"(r[1].h[1]), "=&v"(r[2].h[0]), "=&v"(r[2].h[1]), "=&v"(r[3].h[0]), "=&v"(r[3].h[1])
-                    : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "n"(S * 32 * RB), "n"((S * 32 + 4) * RB)
-                    : "memory");
+                    for (int x = 0; x < 4; ++x) f[n + x] = r[x].f;
+                }
+            } else {
 #pragma unroll
-                for (int x = 0; x < 4; ++x) f[n + x] = r[x].f;
+                for (int n = 0; n < N; n += 2) {
+                    Two r[2];
+                    asm volatile(
+                        "ds_read_b64_tr_b16 %0, %4 offset:%6\n\tds_read_b64_tr_b16 %1, %4 offset:%7\n\t"
+                        "ds_read_b64_tr_b16 %2, %5 offset:%6\n\tds_read_b64_tr_b16 %3, %5 offset:%7\n\t"
+                        "s_waitcnt lgkmcnt(0)"
+                        : "=&v"(r[0].h[0]), "=&v"(r[0].h[1]), "=&v"(r[1].h[0]), "=&v"(r[1].h[1])
+                        : "v"(at(n)), "v"(at(n + 1)), "n"(S * 32 * RB), "n"((S * 32 + 4) * RB)
+                        : "memory");
+                    f[n] = r[0].f;
+                    f[n + 1] = r[1].f;
+                }
             }
         } else {
 #pragma unroll

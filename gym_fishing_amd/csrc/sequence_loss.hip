@@ -278,25 +278,61 @@ __global__ void __launch_bounds__(256) zero_kernel(T* p, int64_t n) {
 // ---- the plan: tile sizes, pieces, shares ----
 constexpr int64_t kCUs = 256;
 
-// 256 x 256 tiles read the operands half as often as 128 x 128 ones, but there must be enough of them to fill the chip
-static bool big_tiles(int64_t m, int64_t n) { return m > 128 && n > 128 && ceil_div(m, 256) * ceil_div(n, 256) >= kCUs; }
-
-// how often to split k so that the tiles fill the chip
-static int64_t shares_of(int64_t m, int64_t n, bool big, int64_t k_steps) {
-    const int64_t b = big ? 256 : 128, tiles = ceil_div(m, b) * ceil_div(n, b), slots = big ? kCUs : 2 * kCUs;
-    int64_t s = slots / tiles;
-    if (s < 1) s = 1;
-    const int64_t most = k_steps / 4 > 0 ? k_steps / 4 : 1;
-    return s < most ? s : most;
+// What a workgroup's tile of b x b outputs costs, us: a staged 128 bytes of k, and what surrounds the product (first load, epilogue).
+// Measured on 8192 x 32771 x 1024 (b = 256: 16 steps, 42 us a tile in all), 103424 x 100 x 128 (128) and 5001 x 1009 x 200 (64, f32)
+template <typename T>
+static double step_us(int64_t b) {
+    if (sizeof(T) == 2) return b == 256 ? 2.0 : b == 128 ? 0.7 : 0.25;
+    return b == 256 ? 7.6 : b == 128 ? 1.9 : 0.5;
 }
+static double tile_us(int64_t b) { return b == 256 ? 10.0 : b == 128 ? 4.0 : 2.0; }
+
+struct Tiling {
+    int64_t b, shares, share;       // tile edge; how often k is split, and the split's elements of k
+};
+
+// the tile and the split of k that fill the chip's rounds of workgroups best; every split costs a float32 slab written and read
+template <typename T>
+static Tiling tiling(int64_t m, int64_t n, int64_t k, bool split) {
+    const int64_t bk = 128 / (int64_t)sizeof(T), steps = ceil_div(k, bk);
+    Tiling best{64, 1, steps * bk};
+    double least = -1.0;
+    for (int64_t b = 256; b >= 64; b >>= 1) {
+        const int64_t tiles = ceil_div(m, b) * ceil_div(n, b);
+        for (int64_t s = 1; s <= (split ? 1024 : 1) && s <= steps; s <<= 1) {
+            const double each = tile_us(b) + step_us<T>(b) * (double)ceil_div(steps, s);
+            const double us = (double)ceil_div(tiles * s, kCUs) * each + (s > 1 ? 4.0 + (double)(s * m * n) * 8e-6 / 4.0 : 0.0);
+            if (least < 0.0 || us < least) {
+                least = us;
+                best = Tiling{b, s, ceil_div(steps, s) * bk};
+            }
+        }
+    }
+    best.shares = ceil_div(steps * bk, best.share);
+    return best;
+}
+
+// f(an object of the tile's product type, its edge): the run-time edge made a type
+template <typename T, int B, bool A_MAJOR, bool B_MAJOR>
+struct TileType {
+    typedef Gemm<T, B, B, 2, B == 256 ? 4 : 2, A_MAJOR, B_MAJOR> G;
+    static constexpr int EDGE = B;
+};
+template <typename T, bool A_MAJOR, bool B_MAJOR, typename F>
+static int with_tile(int64_t b, F&& f) {
+    return b == 256 ? f(TileType<T, 256, A_MAJOR, B_MAJOR>{}) : b == 128 ? f(TileType<T, 128, A_MAJOR, B_MAJOR>{}) : f(TileType<T, 64, A_MAJOR, B_MAJOR>{});
+}
+static int64_t part_levels(int64_t b) { return b == 256 ? 64 : b / 2; }      // levels of a wave's columns
 
 struct LossPlan {
     int64_t bk, dim_p, rows_p, piece;       // elements of a staged k step; padded depth and row count; levels of a piece
-    bool big_z;
+    int64_t z;                              // forward: tile edge
     int parts;
-    int64_t dh_share, dh_shares, dw_share, dw_shares;
-    bool big_dh, big_dw;
+    Tiling dh;                              // of a whole piece; the last one's is made for its width
 };
+
+template <typename T>
+static Tiling dw_tiling(const LossPlan& p, int64_t width, int64_t dim) { return tiling<T>(dim, width, p.rows_p, true); }
 
 template <typename T>
 static LossPlan loss_plan(int64_t rows, int64_t levels, int64_t dim) {
@@ -305,19 +341,25 @@ static LossPlan loss_plan(int64_t rows, int64_t levels, int64_t dim) {
     p.bk = 128 / (int64_t)sizeof(T);
     p.dim_p = round_up(dim, p.bk);
     p.rows_p = round_up(rows, p.bk);
-    const int64_t pieces = ceil_div(levels, 16384);
-    p.piece = pieces == 1 ? levels : round_up(ceil_div(levels, pieces), 256);
-    p.big_z = big_tiles(rows, p.piece);
-    p.parts = (int)(p.big_z ? ceil_div(levels, 256) * 4 : ceil_div(levels, 128) * 2);
-    const int64_t dh_k = round_up(p.piece, p.bk);
-    p.big_dh = ceil_div(dim, 256) * ceil_div(rows, 256) * (dh_k / p.bk / 8) >= kCUs && dim > 128;
-    p.dh_shares = shares_of(dim, rows, p.big_dh, dh_k / p.bk);
-    p.dh_share = round_up(ceil_div(dh_k, p.dh_shares), p.bk);
-    p.dh_shares = ceil_div(dh_k, p.dh_share);
-    p.big_dw = ceil_div(dim, 256) * ceil_div(p.piece, 256) * (p.rows_p / p.bk / 8) >= kCUs && dim > 128;
-    p.dw_shares = shares_of(dim, p.piece, p.big_dw, p.rows_p / p.bk);
-    p.dw_share = round_up(ceil_div(p.rows_p, p.dw_shares), p.bk);
-    p.dw_shares = ceil_div(p.rows_p, p.dw_share);
+    p.z = tiling<T>(rows, levels, dim, false).b;
+    p.parts = (int)(ceil_div(levels, p.z) * (p.z / part_levels(p.z)));
+    // A piece keeps dz^T for the two products: at most 24576 levels, at least 8192, and of those the width whose product for dW
+    // fills its rounds of workgroups best (32771 levels, dim 1024: three pieces of 43 tiles left a third of the chip idle)
+    p.piece = levels;
+    if (levels > 16384) {
+        double best = 0.0;
+        const int64_t across = ceil_div(dim, 256);
+        for (int64_t t = 96; t >= 32; --t) {
+            const int64_t tiles = t * across, s = tiles < kCUs ? kCUs / tiles : 1;
+            const double full = (double)(tiles * s) / (double)round_up(tiles * s, kCUs);
+            if (full > best + 1e-9) {
+                best = full;
+                p.piece = t * 256;
+            }
+        }
+        if (p.piece > levels) p.piece = levels;
+    }
+    p.dh = tiling<T>(dim, rows, p.piece, true);
     return p;
 }
 
@@ -325,7 +367,7 @@ template <typename T>
 struct LossWork {
     float *top = nullptr, *sum = nullptr, *taken = nullptr, *dh = nullptr, *dw = nullptr;
     T *h = nullptr, *w = nullptr, *dzt = nullptr;
-    int64_t dh_slab = 0, dw_slab = 0, bytes = 0;
+    int64_t dh_slab = 0, bytes = 0;
 };
 
 // the padded copies are counted whether the operands need them or not: the caller asks before the pointers are known
@@ -338,9 +380,10 @@ static LossWork<T> loss_work(const LossPlan& p, int64_t rows, int64_t levels, in
     if (backward) {
         w.dzt = c.take<T>(round_up(p.piece, 256) * p.rows_p);
         w.dh_slab = round_up(rows * dim, 4);
-        w.dw_slab = round_up(p.piece * dim, 4);
-        if (p.dh_shares > 1 || p.piece < levels) w.dh = c.take<float>(p.dh_shares * w.dh_slab);
-        if (p.dw_shares > 1) w.dw = c.take<float>(p.dw_shares * w.dw_slab);
+        if (p.dh.shares > 1 || p.piece < levels) w.dh = c.take<float>(p.dh.shares * w.dh_slab);
+        const int64_t last = levels % p.piece, a = dw_tiling<T>(p, p.piece, dim).shares, b = last ? dw_tiling<T>(p, last, dim).shares : 1;
+        const int64_t slabs_a = a > 1 ? a * round_up(p.piece * dim, 4) : 0, slabs_b = b > 1 ? b * round_up(last * dim, 4) : 0;
+        w.dw = c.take<float>(slabs_a > slabs_b ? slabs_a : slabs_b);
     } else {
         w.top = c.take<float>(rows * p.parts);
         w.sum = c.take<float>(rows * p.parts);
@@ -353,14 +396,9 @@ static LossWork<T> loss_work(const LossPlan& p, int64_t rows, int64_t levels, in
 static int loss_check(int32_t dtype, int64_t rows, int64_t levels, int64_t dim) {
     if (dtype != FISHING_DTYPE_F32 && dtype != FISHING_DTYPE_BF16) return FISHING_ERR_UNSUPPORTED;
     if (rows < 0 || rows > 0x7fffffff || levels < 1 || levels > 0x7ffffff || dim < 1 || dim > 65536) return FISHING_ERR_SIZE;
-    if (ceil_div(rows, 128) * ceil_div(levels, 128) > 0x7fffffff || ceil_div(rows, 128) * ceil_div(dim, 128) > 0x7fffffff) return FISHING_ERR_SIZE;    // workgroups of a launch
+    if (ceil_div(rows, 64) * ceil_div(levels, 64) > 0x7fffffff || ceil_div(rows, 64) * ceil_div(dim, 64) > 0x7fffffff) return FISHING_ERR_SIZE;    // workgroups of a launch
     return FISHING_OK;
 }
-
-template <typename T>
-using Big = Gemm<T, 256, 256, 2, 4, false, false>;
-template <typename T>
-using Small = Gemm<T, 128, 128, 2, 2, false, false>;
 
 template <typename T>
 static int pad(const T* src, int64_t ld, int64_t rows, int64_t width, T* dst, int64_t padded, const void* target, int target_bytes, int64_t levels, hipStream_t stream) {
@@ -388,9 +426,12 @@ static int loss_forward(int64_t rows, int64_t levels, int64_t dim, const T* h, i
     int rc = padded_operand<T>(p, h, h_ld, rows, dim, k.h, a, stream);
     if (!rc) rc = padded_operand<T>(p, w, w_ld, levels, dim, k.w, b, stream);
     if (rc) return rc;
-    const int64_t t = p.big_z ? 256 : 128, tm = ceil_div(rows, t), tn = ceil_div(levels, t);
-    rc = p.big_z ? launch(loss_part_kernel<T, Big<T>, 256, 256>, dim3((unsigned)(tm * tn)), dim3(512), stream, a, b, p.dim_p, target, target_bytes, tm, tn, k.top, k.sum, k.taken)
-                 : launch(loss_part_kernel<T, Small<T>, 128, 128>, dim3((unsigned)(tm * tn)), dim3(256), stream, a, b, p.dim_p, target, target_bytes, tm, tn, k.top, k.sum, k.taken);
+    rc = with_tile<T, false, false>(p.z, [&](auto t) {
+        typedef decltype(t) Tile;
+        const int64_t tm = ceil_div(rows, Tile::EDGE), tn = ceil_div(levels, Tile::EDGE);
+        return launch(loss_part_kernel<T, typename Tile::G, Tile::EDGE, Tile::EDGE>, dim3((unsigned)(tm * tn)), dim3(Tile::G::THREADS), stream, a, b, p.dim_p, target, target_bytes,
+                      tm, tn, k.top, k.sum, k.taken);
+    });
     if (rc) return rc;
     auto join_parts = [&](auto kernel, int r, int l) {
         return launch(kernel, dim3((unsigned)ceil_div(rows, r)), dim3(r * l), stream, k.top, k.sum, k.taken, target, target_bytes, rows, levels, p.parts, loss, lse);
@@ -399,13 +440,13 @@ static int loss_forward(int64_t rows, int64_t levels, int64_t dim, const T* h, i
 }
 
 template <typename T, typename O, bool A_MAJOR, bool B_MAJOR>
-static int product(const Operand<T>& a, const Operand<T>& b, bool big, int64_t k, int64_t share, int64_t shares, int64_t m, int64_t n, bool add, O* out, int64_t ld, int64_t slab,
-                   hipStream_t stream) {
-    const int64_t t = big ? 256 : 128, tm = ceil_div(m, t), tn = ceil_div(n, t);
-    const dim3 grid((unsigned)(tm * tn), (unsigned)shares);
-    if (big)
-        return launch(product_kernel<T, O, Gemm<T, 256, 256, 2, 4, A_MAJOR, B_MAJOR>, 256, 256>, grid, dim3(512), stream, a, b, k, share, m, n, tm, tn, add, out, ld, slab);
-    return launch(product_kernel<T, O, Gemm<T, 128, 128, 2, 2, A_MAJOR, B_MAJOR>, 128, 128>, grid, dim3(256), stream, a, b, k, share, m, n, tm, tn, add, out, ld, slab);
+static int product(const Operand<T>& a, const Operand<T>& b, const Tiling& t, int64_t k, int64_t m, int64_t n, bool add, O* out, int64_t ld, int64_t slab, hipStream_t stream) {
+    return with_tile<T, A_MAJOR, B_MAJOR>(t.b, [&](auto tile) {
+        typedef decltype(tile) Tile;
+        const int64_t tm = ceil_div(m, Tile::EDGE), tn = ceil_div(n, Tile::EDGE);
+        return launch(product_kernel<T, O, typename Tile::G, Tile::EDGE, Tile::EDGE>, dim3((unsigned)(tm * tn), (unsigned)t.shares), dim3(Tile::G::THREADS), stream, a, b, k, t.share,
+                      m, n, tm, tn, add, out, ld, slab);
+    });
 }
 
 template <typename T>
@@ -418,30 +459,35 @@ static int loss_backward(int64_t rows, int64_t levels, int64_t dim, const T* h, 
     if (!rc) rc = padded_operand<T>(p, w, w_ld, levels, dim, k.w, b, stream);
     for (int64_t v0 = 0; v0 < levels && !rc; v0 += p.piece) {
         const int64_t width = levels - v0 < p.piece ? levels - v0 : p.piece, width_p = round_up(width, p.bk);
-        const int64_t t = p.big_z ? 256 : 128, tm = ceil_div(rows, t), tn = ceil_div(width, t);
-        rc = p.big_z ? launch(loss_dz_kernel<T, Big<T>, 256, 256>, dim3((unsigned)(tm * tn)), dim3(512), stream, a, b, p.dim_p, target, target_bytes, levels, v0, tm, tn, lse, g,
-                              k.dzt, p.rows_p)
-                     : launch(loss_dz_kernel<T, Small<T>, 128, 128>, dim3((unsigned)(tm * tn)), dim3(256), stream, a, b, p.dim_p, target, target_bytes, levels, v0, tm, tn, lse, g,
-                              k.dzt, p.rows_p);
+        rc = with_tile<T, false, false>(tiling<T>(rows, width, dim, false).b, [&](auto t) {
+            typedef decltype(t) Tile;
+            const int64_t tm = ceil_div(rows, Tile::EDGE), tn = ceil_div(width, Tile::EDGE);
+            return launch(loss_dz_kernel<T, typename Tile::G, Tile::EDGE, Tile::EDGE>, dim3((unsigned)(tm * tn)), dim3(Tile::G::THREADS), stream, a, b, p.dim_p, target, target_bytes,
+                          levels, v0, tm, tn, lse, g, k.dzt, p.rows_p);
+        });
         if (rc) break;
         // dh[r][d]: m = d, n = r, k = the piece's levels, both operands k-major; W's rows beyond the last meet zeros of dz
         const Operand<T> wd{b.p + v0 * b.ld, b.ld, p.dim_p, width}, zr{k.dzt, p.rows_p, p.rows_p, width_p};
-        if (k.dh)
-            rc = product<T, float, true, true>(wd, zr, p.big_dh, width_p, p.dh_share, p.dh_shares, dim, rows, v0 > 0, k.dh, dim, k.dh_slab, stream);
-        else
-            rc = product<T, T, true, true>(wd, zr, p.big_dh, width_p, p.dh_share, 1, dim, rows, false, dh, dim, 0, stream);
+        Tiling t = width == p.piece ? p.dh : tiling<T>(dim, rows, width, true);
+        if (t.shares > p.dh.shares) {                       // (the first piece's slabs are all there are)
+            t.share = round_up(ceil_div(width_p, p.dh.shares), p.bk);
+            t.shares = ceil_div(width_p, t.share);
+        }
+        rc = k.dh ? product<T, float, true, true>(wd, zr, t, width_p, dim, rows, v0 > 0, k.dh, dim, k.dh_slab, stream)
+                  : product<T, T, true, true>(wd, zr, t, width_p, dim, rows, false, dh, dim, 0, stream);
         if (rc) break;
         // dW[v][d]: m = d, n = v, k = rows; h's rows beyond the last meet zeros of dz
         const Operand<T> hd{k.h, p.dim_p, p.dim_p, rows}, zv{k.dzt, p.rows_p, width, width};
-        if (k.dw) {
-            rc = product<T, float, true, false>(hd, zv, p.big_dw, p.rows_p, p.dw_share, p.dw_shares, dim, width, false, k.dw, dim, k.dw_slab, stream);
-            if (!rc)
-                rc = slab_sum<T>(k.dw, k.dw_slab, p.dw_shares, dw + v0 * dim, width * dim, stream);
+        t = dw_tiling<T>(p, width, dim);
+        if (t.shares > 1) {
+            const int64_t slab = round_up(width * dim, 4);
+            rc = product<T, float, true, false>(hd, zv, t, p.rows_p, dim, width, false, k.dw, dim, slab, stream);
+            if (!rc) rc = slab_sum<T>(k.dw, slab, t.shares, dw + v0 * dim, width * dim, stream);
         } else {
-            rc = product<T, T, true, false>(hd, zv, p.big_dw, p.rows_p, p.dw_share, 1, dim, width, false, dw + v0 * dim, dim, 0, stream);
+            rc = product<T, T, true, false>(hd, zv, t, p.rows_p, dim, width, false, dw + v0 * dim, dim, 0, stream);
         }
     }
-    if (!rc && k.dh) rc = slab_sum<T>(k.dh, k.dh_slab, p.dh_shares, dh, rows * dim, stream);
+    if (!rc && k.dh) rc = slab_sum<T>(k.dh, k.dh_slab, p.dh.shares, dh, rows * dim, stream);
     return rc;
 }
 
