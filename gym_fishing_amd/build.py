@@ -45,6 +45,7 @@ TU_FLAGS = {"fishing_step.hip": ["-fno-slp-vectorize", "-mllvm", "-amdgpu-kernar
             "fishing_rollout.hip": ["-fno-slp-vectorize"],
             # the sequence operators accumulate in float32 with fused multiply-adds: no NumPy rounding to reproduce there
             "sequence_embedding.hip": ["-ffp-contract=fast"], "sequence_attention.hip": ["-ffp-contract=fast"],
+            "sequence_attention_back.hip": ["-ffp-contract=fast"],
             "sequence_loss.hip": ["-ffp-contract=fast"]}
 
 

@@ -7,20 +7,10 @@
 // and with R the gradient of the state behind step t, R_t = scale * q_t do_t^T + a_{t+1} R_{t+1} (R_{T-1} also takes the final state's):
 //   dq_t = scale * S_t do_t      dk_t = R_t v_t      dv_t = R_t^T k_t      dS_{-1} = a_0 R_0
 // so every gradient is the same recurrence with the roles of its operands exchanged, dk and dv backwards in time.
-#include "sequence_common.h"
+#include "sequence_walk.h"
 
 namespace fishing {
 namespace seq {
-
-constexpr int kMaxHeadDim = 128;
-
-struct Strided {
-    const void* p;
-    int64_t batch, step, head;
-};
-
-// exp(-inf * 0) would be NaN: a decay of zero is carried as a logarithm far below float32's range
-__device__ __forceinline__ float log_decay_of(const float* log_decay, int h) { return fmaxf(log_decay[h], -1.0e4f); }
 
 // ---- the single step: a wave owns one (env, head); its state goes through registers once.  Bound by the state's two trips. ----
 template <typename T, int V>
@@ -100,71 +90,6 @@ __global__ void __launch_bounds__(256) step_kernel_recurrent(Strided q, Strided 
     }
 }
 
-// ---- whole episodes, one step after the other: a workgroup owns (batch, head) and 32 columns of the state; thread (column c,
-// part g of eight) keeps 16 of its rows in registers.  BACK walks the steps backwards: a_{t+1} stands in front of step t, none in
-// front of the last, a_0 behind the first.  The operands'
-// roles: o = read_scale q S, S += write_scale k v^T. ----
-template <typename T, bool BACK>
-__global__ void __launch_bounds__(256) recurrent_kernel(Strided q, Strided k, Strided v, const float* log_decay, const uint8_t* starts, int64_t starts_batch,
-                                                        int64_t starts_step, const float* state, float* state_out, Strided out, int64_t steps, int32_t heads,
-                                                        int32_t dk, int32_t dv, bool state_t, float read_scale, float write_scale) {
-    __shared__ float row[2][kMaxHeadDim];
-    const int64_t n = blockIdx.x / heads;
-    const int h = (int)(blockIdx.x - n * heads);
-    const int g = threadIdx.x & 7, c = blockIdx.y * 32 + (threadIdx.x >> 3);
-    const float a = expf(log_decay_of(log_decay, h));
-    const float* s0 = state ? state + (int64_t)blockIdx.x * dk * dv : nullptr;
-    // element (i, c) of the state, or of its transpose where the operands' roles are exchanged
-    auto at = [&](int i) { return state_t ? (int64_t)c * dk + i : (int64_t)i * dv + c; };
-    float s[16];
-#pragma unroll
-    for (int x = 0; x < 16; ++x) {
-        const int i = x * 8 + g;
-        s[x] = s0 && i < dk && c < dv ? s0[at(i)] : 0.0f;
-    }
-    auto cut = [&](int64_t t) { return starts && starts[n * starts_batch + t * starts_step]; };
-    for (int64_t u = 0; u < steps; ++u) {
-        const int64_t t = BACK ? steps - 1 - u : u;
-        const T* qp = (const T*)q.p + n * q.batch + t * q.step + h * q.head;
-        const T* kp = (const T*)k.p + n * k.batch + t * k.step + h * k.head;
-        const T* vp = (const T*)v.p + n * v.batch + t * v.step + h * v.head;
-        __syncthreads();
-        for (int i = threadIdx.x; i < dk; i += 256) {
-            row[0][i] = to_f32(qp[i]) * read_scale;
-            row[1][i] = to_f32(kp[i]) * write_scale;
-        }
-        __syncthreads();
-        float keep = a;
-        if (BACK)
-            keep = u == 0 ? 1.0f : cut(t + 1) ? 0.0f : a;
-        else if (cut(t))
-            keep = 0.0f;
-        const float vc = c < dv ? to_f32(vp[c]) : 0.0f;
-        float o = 0.0f;
-#pragma unroll
-        for (int x = 0; x < 16; ++x) {
-            const int i = x * 8 + g;
-            if (i < dk) {
-                s[x] = (keep == 0.0f ? 0.0f : keep * s[x]) + row[1][i] * vc;
-                o += row[0][i] * s[x];
-            }
-        }
-        o += __shfl_xor(o, 1);
-        o += __shfl_xor(o, 2);
-        o += __shfl_xor(o, 4);
-        if (g == 0 && c < dv) ((T*)out.p)[n * out.batch + t * out.step + h * out.head + c] = from_f32<T>(o);
-    }
-    if (state_out && c < dv) {
-        float* s1 = state_out + (int64_t)blockIdx.x * dk * dv;
-        const float last = BACK && steps > 0 ? (cut(0) ? 0.0f : a) : 1.0f;
-#pragma unroll
-        for (int x = 0; x < 16; ++x) {
-            const int i = x * 8 + g;
-            if (i < dk) s1[at(i)] = last == 0.0f ? 0.0f : last * s[x];
-        }
-    }
-}
-
 static int attention_check(const FishingDecayAttention* a, bool one_step) {
     if (!a) return FISHING_ERR_NULL;
     if (a->dtype != FISHING_DTYPE_F32 && a->dtype != FISHING_DTYPE_BF16) return FISHING_ERR_UNSUPPORTED;
@@ -190,26 +115,22 @@ static int attention_step(const FishingDecayAttention* a, hipStream_t stream) {
     return go(step_kernel_recurrent<T, 1>);
 }
 
-template <typename T, bool BACK>
-static int recurrent(const FishingDecayAttention* a, Strided q, Strided k, Strided v, const float* state, float* state_out, Strided out, int dk, int dv, bool state_t,
-                     double read_scale, double write_scale, hipStream_t stream) {
-    return launch(recurrent_kernel<T, BACK>, dim3((unsigned)(a->batch * a->heads), (unsigned)ceil_div(dv, 32)), dim3(256), stream, q, k, v, a->log_decay, a->starts,
-                  a->starts_stride[0], a->starts_stride[1], state, state_out, out, a->steps, a->heads, dk, dv, state_t, (float)read_scale, (float)write_scale);
+extern template int walk<float, true>(const FishingDecayAttention*, Strided, Strided, Strided, const float*, float*, Strided, int, int, bool, double, double, void*, hipStream_t);
+extern template int walk<bf16, true>(const FishingDecayAttention*, Strided, Strided, Strided, const float*, float*, Strided, int, int, bool, double, double, void*, hipStream_t);
+
+template <typename T>
+static int attention_forward(const FishingDecayAttention* a, void* work, hipStream_t stream) {
+    return walk<T, false>(a, strided(a->q, a->q_stride), strided(a->k, a->k_stride), strided(a->v, a->v_stride), a->state, a->state_out,
+                               strided((const void*)a->out, a->out_stride), a->dk, a->dv, false, a->scale, 1.0, work, stream);
 }
 
 template <typename T>
-static int attention_forward(const FishingDecayAttention* a, hipStream_t stream) {
-    return recurrent<T, false>(a, strided(a->q, a->q_stride), strided(a->k, a->k_stride), strided(a->v, a->v_stride), a->state, a->state_out,
-                               strided((const void*)a->out, a->out_stride), a->dk, a->dv, false, a->scale, 1.0, stream);
-}
-
-template <typename T>
-static int attention_backward(const FishingDecayAttention* a, hipStream_t stream) {
+static int attention_backward(const FishingDecayAttention* a, void* work, hipStream_t stream) {
     const Strided q = strided(a->q, a->q_stride), k = strided(a->k, a->k_stride), v = strided(a->v, a->v_stride), g = strided(a->dout, a->dout_stride);
     // dq: read with do the state that (v, k) build;  dk, dv: read with v, k the state's gradient that (do, q), (q, do) build backwards
-    int rc = recurrent<T, false>(a, g, v, k, a->state, nullptr, strided((const void*)a->dq, a->dq_stride), a->dv, a->dk, true, a->scale, 1.0, stream);
-    if (!rc) rc = recurrent<T, true>(a, v, g, q, a->dstate_out, nullptr, strided((const void*)a->dk_out, a->dk_stride), a->dv, a->dk, true, 1.0, a->scale, stream);
-    if (!rc) rc = recurrent<T, true>(a, k, q, g, a->dstate_out, a->dstate, strided((const void*)a->dv_out, a->dv_stride), a->dk, a->dv, false, 1.0, a->scale, stream);
+    int rc = walk<T, false>(a, g, v, k, a->state, nullptr, strided((const void*)a->dq, a->dq_stride), a->dv, a->dk, true, a->scale, 1.0, work, stream);
+    if (!rc) rc = walk<T, true>(a, v, g, q, a->dstate_out, nullptr, strided((const void*)a->dk_out, a->dk_stride), a->dv, a->dk, true, 1.0, a->scale, work, stream);
+    if (!rc) rc = walk<T, true>(a, k, q, g, a->dstate_out, a->dstate, strided((const void*)a->dv_out, a->dv_stride), a->dk, a->dv, false, 1.0, a->scale, work, stream);
     return rc;
 }
 
@@ -229,24 +150,28 @@ int fishing_decay_attention_step(const FishingDecayAttention* a, fishing_stream_
 
 int64_t fishing_decay_attention_workspace(const FishingDecayAttention* a, int32_t backward) {
     if (int rc = attention_check(a, false)) return rc;
-    (void)backward;
-    return 256;
+    const int64_t pairs = a->batch * a->heads, one = walk_work(walk_plan(pairs, a->steps, a->dk, a->dv), pairs, nullptr).bytes;
+    if (!backward) return one;
+    const int64_t other = walk_work(walk_plan(pairs, a->steps, a->dv, a->dk), pairs, nullptr).bytes;      // the walks run one after the other
+    return one > other ? one : other;
 }
 
 int fishing_decay_attention_forward(const FishingDecayAttention* a, void* workspace, int64_t workspace_bytes, fishing_stream_t stream) {
     if (int rc = attention_check(a, false)) return rc;
     if (a->batch == 0) return FISHING_OK;
     if ((a->steps > 0 && !a->out) || !workspace) return FISHING_ERR_NULL;
+    if (!aligned16(workspace)) return FISHING_ERR_ALIGN;
     if (workspace_bytes < fishing_decay_attention_workspace(a, 0)) return FISHING_ERR_SIZE;
-    return a->dtype == FISHING_DTYPE_F32 ? attention_forward<float>(a, (hipStream_t)stream) : attention_forward<bf16>(a, (hipStream_t)stream);
+    return a->dtype == FISHING_DTYPE_F32 ? attention_forward<float>(a, workspace, (hipStream_t)stream) : attention_forward<bf16>(a, workspace, (hipStream_t)stream);
 }
 
 int fishing_decay_attention_backward(const FishingDecayAttention* a, void* workspace, int64_t workspace_bytes, fishing_stream_t stream) {
     if (int rc = attention_check(a, false)) return rc;
     if (a->batch == 0) return FISHING_OK;
     if ((a->steps > 0 && (!a->dout || !a->dq || !a->dk_out || !a->dv_out)) || !workspace) return FISHING_ERR_NULL;
+    if (!aligned16(workspace)) return FISHING_ERR_ALIGN;
     if (workspace_bytes < fishing_decay_attention_workspace(a, 1)) return FISHING_ERR_SIZE;
-    return a->dtype == FISHING_DTYPE_F32 ? attention_backward<float>(a, (hipStream_t)stream) : attention_backward<bf16>(a, (hipStream_t)stream);
+    return a->dtype == FISHING_DTYPE_F32 ? attention_backward<float>(a, workspace, (hipStream_t)stream) : attention_backward<bf16>(a, workspace, (hipStream_t)stream);
 }
 
 }  // extern "C"

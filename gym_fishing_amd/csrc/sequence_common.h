@@ -38,7 +38,7 @@ template <typename T>
 __host__ __device__ constexpr int vec_of() { return 16 / (int)sizeof(T); }
 
 static inline bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
-static inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+__host__ __device__ inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 static inline int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
 
 // This launch's own status, as hipLaunchKernel returns it

@@ -1,0 +1,564 @@
+// sequence_walk.h -- linear attention's walk over whole episodes: the chunk kernels, what repairs values that are not numbers, and the
+// walk's plan and launches.  Instantiated forwards in sequence_attention.hip and backwards in sequence_attention_back.hip.
+#pragma once
+#include "sequence_common.h"
+
+namespace fishing {
+namespace seq {
+
+constexpr int kMaxHeadDim = 128;
+
+struct Strided {
+    const void* p;
+    int64_t batch, step, head;
+};
+
+// exp(-inf * 0) would be NaN: a decay of zero is carried as a logarithm far below float32's range
+__device__ __forceinline__ float log_decay_of(const float* log_decay, int h) { return fmaxf(log_decay[h], -1.0e4f); }
+
+// ---- whole episodes, 32 steps at a time: one wave owns a (batch, head), up to 64 columns of its state, and a run of steps ----
+//
+// With g = exp(log_decay) and the steps x of a chunk of n, "open" meaning that no start lies between:
+//   forwards   o_x = sum_{y <= x, open} g^(x-y) (q_x . k_y) v_y + [open to the chunk's front] g^(x+1) q_x S
+//              S' = [no start] g^n S + sum_{y, open to the end} g^(n-1-y) k_y v_y^T
+//   backwards  o_x = sum_{y >= x, open} g^(y-x) (q_x . k_y) v_y + [open to the chunk's end] g^(n-1-x) q_x S
+//              S' = [no start] g^n S + sum_{y, no start in 0 .. y} g^(y+1) k_y v_y^T
+// so a chunk is four small products on the matrix cores.  The layouts chain without a shuffle: the tile k q^T has its columns in
+// lanes and four rows y in registers, which is the second operand of v^T (k q^T); a state tile k^T v likewise is the first of S^T q^T;
+// the outputs come as four neighbouring columns of one step per lane.  k and v are read by columns through the transposing LDS read
+// (bf16) or element reads (f32).  bf16: scores, the state's copy and the decayed v, which the products need in bf16, are carried as
+// two bf16 terms (16 bits; the decayed v as three: the state is an answer in float32): one term would lose 1.7x the output's own
+// rounding, and the matrix cores have the time.
+// A wave alone needs no barriers; the next chunk's rows are loaded into registers while this one is computed.  Bound by HBM: q, k, v
+// read, out written once.
+
+template <typename T>
+struct Lanes;
+template <>
+struct Lanes<bf16> {
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    typedef s16x4 Quad;
+    static constexpr bool SPLIT = true;
+    // four steps y of one column; each lane names the 8 bytes (4 columns of one step) that it contributes
+    static __device__ __forceinline__ Quad column(const char* rows, int pitch, int y0, int col, int spread) {
+        const int i = threadIdx.x & 15, g = threadIdx.x >> 4 & 3;
+        const char* at = rows + (y0 + 4 * g + (i >> 2)) * pitch + (col + spread * (i & 3)) * 2;
+        return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at);
+    }
+    static __device__ __forceinline__ Quad state_column(const char* rows, int pitch, int y0, int c) { return column(rows, pitch, y0, 32 * (c >> 1) + 4 * (c & 1), 8); }
+    static __device__ __forceinline__ Quad value_column(const char* rows, int pitch, int y0, int n) { return column(rows, pitch, y0, 16 * n, 4); }
+    // eight neighbouring elements of one row, as the quads of tiles 2c and 2c + 1
+    static __device__ __forceinline__ void row_quads(const char* rows, int pitch, int y, int c, Quad& a, Quad& b) {
+        const int g = threadIdx.x >> 4 & 3;
+        typedef short s16x8 __attribute__((ext_vector_type(8)));
+        const s16x8 x = *(const s16x8*)(rows + y * pitch + (32 * c + 8 * g) * 2);
+        a = __builtin_shufflevector(x, x, 0, 1, 2, 3);
+        b = __builtin_shufflevector(x, x, 4, 5, 6, 7);
+    }
+    // the state tile c's row 4 g + r
+    static __device__ __forceinline__ int state_row(int c, int g) { return 32 * (c >> 1) + 8 * g + 4 * (c & 1); }
+    static __device__ __forceinline__ f32x4 mma(Quad a0, Quad a1, Quad b0, Quad b1, f32x4 acc) {
+        union {
+            Quad q[2];
+            bf16x8 f;
+        } a{{a0, a1}}, b{{b0, b1}};
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.f, b.f, acc, 0, 0, 0);
+    }
+    static __device__ __forceinline__ Quad round(f32x4 x) {
+        union {
+            bf16x4 h;
+            Quad q;
+        } y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y.h[e] = (bf16)x[e];
+        return y.q;
+    }
+    static __device__ __forceinline__ f32x4 wide(Quad x) {
+        f32x4 y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = __uint_as_float((uint32_t)(uint16_t)x[e] << 16);
+        return y;
+    }
+};
+template <>
+struct Lanes<float> {
+    typedef f32x4 Quad;
+    static constexpr bool SPLIT = false;
+    static __device__ __forceinline__ Quad column(const char* rows, int pitch, int y0, int col) {
+        const int i = threadIdx.x & 15, g = threadIdx.x >> 4 & 3;
+        Quad x;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = *(const float*)(rows + (y0 + 4 * g + e) * pitch + (col + i) * 4);
+        return x;
+    }
+    static __device__ __forceinline__ Quad state_column(const char* rows, int pitch, int y0, int c) { return column(rows, pitch, y0, 16 * c); }
+    static __device__ __forceinline__ Quad value_column(const char* rows, int pitch, int y0, int n) { return column(rows, pitch, y0, 16 * n); }
+    static __device__ __forceinline__ void row_quads(const char* rows, int pitch, int y, int c, Quad& a, Quad& b) {
+        const int g = threadIdx.x >> 4 & 3;
+        a = *(const Quad*)(rows + y * pitch + (32 * c + 4 * g) * 4);
+        b = *(const Quad*)(rows + y * pitch + (32 * c + 16 + 4 * g) * 4);
+    }
+    static __device__ __forceinline__ int state_row(int c, int g) { return 16 * c + 4 * g; }
+    static __device__ __forceinline__ f32x4 mma(Quad a0, Quad a1, Quad b0, Quad b1, f32x4 acc) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a0[e], b0[e], acc, 0, 0, 0);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a1[e], b1[e], acc, 0, 0, 0);
+        return acc;
+    }
+    static __device__ __forceinline__ Quad round(f32x4 x) { return x; }
+    static __device__ __forceinline__ f32x4 wide(Quad x) { return x; }
+};
+
+constexpr int kChunk = 32;
+
+// a chunk's rows of one operand on their way from memory: 16 bytes a lane and load, rows behind the last and columns behind d zero
+template <typename T, int TILES>
+struct Rows {
+    static constexpr int EPC = 16 / (int)sizeof(T), CHUNKS = TILES * 16 / EPC, LOADS = kChunk * CHUNKS / 64, PITCH = TILES * 16 * (int)sizeof(T) + 16;
+    u32x4 x[LOADS];
+
+    template <bool VEC>
+    __device__ __forceinline__ void load(const Strided& o, int64_t n, int64_t h, int64_t t0, int rows, int d) {
+        const T* p = (const T*)o.p + n * o.batch + h * o.head + t0 * o.step;
+#pragma unroll
+        for (int s = 0; s < LOADS; ++s) {
+            const int at = s * 64 + threadIdx.x, row = at / CHUNKS, c = at % CHUNKS * EPC;
+            x[s] = u32x4{0, 0, 0, 0};
+            if (row < rows && c < d) {
+                const T* from = p + row * o.step + c;
+                if (VEC) {
+                    x[s] = *(const u32x4*)from;
+                } else {
+                    Pack<T, EPC> y;
+#pragma unroll
+                    for (int e = 0; e < EPC; ++e) y.e[e] = c + e < d ? from[e] : from_f32<T>(0.0f);
+                    x[s] = *(const u32x4*)&y;
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ void put(char* lds) const {
+#pragma unroll
+        for (int s = 0; s < LOADS; ++s) {
+            const int at = s * 64 + threadIdx.x;
+            *(u32x4*)(lds + at / CHUNKS * PITCH + at % CHUNKS * 16) = x[s];
+        }
+    }
+};
+
+struct ChunkArgs {
+    Strided q, k, v, out;
+    const float* log_decay;
+    const uint8_t* starts;
+    int64_t starts_batch, starts_step;
+    const float* state;        // [batch, heads, dk, dv], or transposed: [batch, heads, dv, dk]
+    float* state_out;
+    int64_t steps;
+    int32_t heads, dk, dv;
+    bool state_t;
+    float read_scale, write_scale;
+    int32_t slices, segs;
+    int64_t seg_steps;
+    float *carry, *through;    // per (pair, slice, segment): the state behind it in lane order, and what it lets through
+    uint32_t* odd;             // per (pair, slice, segment): some result is infinite or NaN
+};
+
+// LOCAL: only the state that a segment adds (from zero; the first from the state carried in), for the segments to be chained.
+template <typename T, int NK, int NV, bool BACK, bool VEC>
+__global__ void __launch_bounds__(64, (NK * NV * (int)sizeof(T) >= 64 ? 1 : 2)) chunk_kernel(ChunkArgs a, bool local) {
+    typedef Lanes<T> L;
+    typedef typename L::Quad Quad;
+    typedef Rows<T, NK> RK;
+    typedef Rows<T, NV> RV;
+    __shared__ __attribute__((aligned(16))) char qs[kChunk * RK::PITCH];
+    __shared__ __attribute__((aligned(16))) char ks[kChunk * RK::PITCH];
+    __shared__ __attribute__((aligned(16))) char vs[kChunk * RV::PITCH];
+    const int lane = threadIdx.x, i = lane & 15, g = lane >> 4;
+    const int64_t id = blockIdx.x, pair = id / (a.slices * a.segs);
+    const int rest = (int)(id - pair * (a.slices * a.segs)), slice = rest / a.segs, seg = rest - slice * a.segs;
+    if (local && seg == a.segs - 1) return;                  // nothing follows it
+    const int64_t n = pair / a.heads, h = pair - n * a.heads;
+    const int col0 = slice * NV * 16, cols = a.dv - col0;
+    Strided v = a.v, out = a.out;
+    v.p = (const T*)v.p + col0;
+    // segments are counted in the direction of the walk
+    const int64_t at = BACK ? a.segs - 1 - seg : seg, t_lo = at * a.seg_steps, t_hi = t_lo + a.seg_steps < a.steps ? t_lo + a.seg_steps : a.steps;
+    const int chunks = (int)ceil_div(t_hi - t_lo, kChunk);
+    const float ld = log_decay_of(a.log_decay, (int)h), l2 = ld * 1.4426950408889634f;
+    const float whole = (float)exp((double)ld * kChunk);     // the factor that compounds: rounded once
+
+    f32x4 S[NK][NV];
+    {
+        float* from = a.carry + (id - 1) * (NK * NV * 256);
+        const float* s0 = a.state ? a.state + pair * (int64_t)a.dk * a.dv : nullptr;
+#pragma unroll
+        for (int c = 0; c < NK; ++c)
+#pragma unroll
+            for (int m = 0; m < NV; ++m) {
+                S[c][m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                if (seg > 0) {
+                    if (!local) S[c][m] = *(const f32x4*)(from + (c * NV + m) * 256 + lane * 4);
+                } else if (s0) {
+                    const int col = m * 16 + i, row = L::state_row(c, g);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (col < cols && row + r < a.dk) S[c][m][r] = a.state_t ? s0[(int64_t)(col0 + col) * a.dk + row + r] : s0[(int64_t)(row + r) * a.dv + col0 + col];
+                }
+            }
+    }
+
+    RK rq, rk;
+    RV rv;
+    bool started = false;
+    auto fetch = [&](int x) {
+        const int64_t t0 = t_lo + (int64_t)(BACK ? chunks - 1 - x : x) * kChunk;
+        const int rows = t_hi - t0 < kChunk ? (int)(t_hi - t0) : kChunk;
+        if (!local) rq.template load<VEC>(a.q, n, h, t0, rows, a.dk);
+        rk.template load<VEC>(a.k, n, h, t0, rows, a.dk);
+        rv.template load<VEC>(v, n, h, t0, rows, cols);
+        started = a.starts && lane < rows && a.starts[n * a.starts_batch + (t0 + lane) * a.starts_step];
+    };
+    float odd = 0.0f, through = 1.0f;
+    if (chunks > 0) fetch(0);
+    for (int x = 0; x < chunks; ++x) {
+        const int64_t t0 = t_lo + (int64_t)(BACK ? chunks - 1 - x : x) * kChunk;
+        const int rows = t_hi - t0 < kChunk ? (int)(t_hi - t0) : kChunk;
+        __syncthreads();
+        if (!local) rq.put(qs);
+        rk.put(ks);
+        rv.put(vs);
+        const uint32_t st = (uint32_t)__ballot(started);
+        __syncthreads();
+        if (x + 1 < chunks) fetch(x + 1);
+
+        // what a chunk of `rows` steps lets of the state through, and of each step's k v^T into it
+        const float pass = st ? 0.0f : rows == kChunk ? whole : exp2f(rows * l2);
+        f32x4 w[2];
+        {
+            const int from = BACK ? 0 : st ? 31 - __clz(st) : 0, to = BACK ? (st ? __ffs(st) - 1 : kChunk) : kChunk;
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int y = 16 * t + 4 * g + r;
+                    w[t][r] = y >= from && y < to && y < rows ? a.write_scale * __builtin_amdgcn_exp2f((BACK ? y + 1 : rows - 1 - y) * l2) : 0.0f;
+                }
+        }
+
+        Quad q[2][NK], p[2][2], p_rest[2][2];     // [step tile][...]; scores: four y in registers, x in lanes
+        float into[2];                            // what a step sees of the state in front of the chunk
+        if (!local) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int c = 0; c < NK / 2; ++c) L::row_quads(qs, RK::PITCH, 16 * t + i, c, q[t][2 * c], q[t][2 * c + 1]);
+#pragma unroll
+            for (int ky = 0; ky < 2; ++ky) {
+                Quad k[NK];
+#pragma unroll
+                for (int c = 0; c < NK / 2; ++c) L::row_quads(ks, RK::PITCH, 16 * ky + i, c, k[2 * c], k[2 * c + 1]);
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    f32x4 z = {0.0f, 0.0f, 0.0f, 0.0f};
+                    if (BACK ? t <= ky : t >= ky) {        // (else no pair of these tiles is in order)
+#pragma unroll
+                        for (int c = 0; c < NK; c += 2) z = L::mma(k[c], k[c + 1], q[t][c], q[t][c + 1], z);
+                        const int step = 16 * t + i;
+                        const uint32_t upto = (2u << step) - 1u, near = BACK ? st & ~upto : st & upto;
+                        const int lo = BACK ? step : near ? 31 - __clz(near) : 0, hi = BACK ? (near ? __ffs(near) - 1 : kChunk) : step + 1;
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const int y = 16 * ky + 4 * g + r;
+                            const float d = __builtin_amdgcn_exp2f((BACK ? y - step : step - y) * l2) * (a.read_scale * a.write_scale);
+                            z[r] = y >= lo && y < hi ? z[r] * d : 0.0f;
+                        }
+                    }
+                    p[t][ky] = L::round(z);
+                    if (L::SPLIT) p_rest[t][ky] = L::round(z - L::wide(p[t][ky]));
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const int step = 16 * t + i;
+                const uint32_t upto = (2u << step) - 1u, near = BACK ? st & ~upto : st & upto;
+                into[t] = near ? 0.0f : a.read_scale * __builtin_amdgcn_exp2f((BACK ? rows - 1 - step : step + 1) * l2);
+            }
+        }
+        through = st ? 0.0f : through * pass;
+
+        Quad kc[2][NK];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int c = 0; c < NK; ++c) kc[t][c] = L::state_column(ks, RK::PITCH, 16 * t, c);
+#pragma unroll
+        for (int m = 0; m < NV; ++m) {
+            __builtin_amdgcn_sched_barrier(0);    // (16 columns at a time: their intermediates are a quarter of the registers)
+            const Quad v0 = L::value_column(vs, RV::PITCH, 0, m), v1 = L::value_column(vs, RV::PITCH, 16, m);
+            if (!local) {
+                f32x4 o[2];
+#pragma unroll
+                for (int t = 0; t < 2; ++t) o[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int c = 0; c < NK; c += 2) {
+                    const Quad s0 = L::round(S[c][m]), s1 = L::round(S[c + 1][m]);
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) o[t] = L::mma(s0, s1, q[t][c], q[t][c + 1], o[t]);
+                    if (L::SPLIT) {
+                        const Quad r0 = L::round(S[c][m] - L::wide(s0)), r1 = L::round(S[c + 1][m] - L::wide(s1));
+#pragma unroll
+                        for (int t = 0; t < 2; ++t) o[t] = L::mma(r0, r1, q[t][c], q[t][c + 1], o[t]);
+                    }
+                }
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[t][r] = into[t] == 0.0f ? 0.0f : o[t][r] * into[t];
+                    o[t] = L::mma(v0, v1, p[t][0], p[t][1], o[t]);
+                    if (L::SPLIT) o[t] = L::mma(v0, v1, p_rest[t][0], p_rest[t][1], o[t]);
+                    const int step = 16 * t + i, col = m * 16 + 4 * g;
+                    if (step < rows) {
+                        T* to = (T*)out.p + n * out.batch + h * out.head + (t0 + step) * out.step + col0 + col;
+                        Pack<T, 4> y;
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            y.e[r] = from_f32<T>(o[t][r]);
+                            if (col + r < cols) odd += o[t][r] * 0.0f;         // NaN from anything that is not a finite number
+                        }
+                        if (VEC) {
+                            if (col < cols) *(Pack<T, 4>*)to = y;
+                        } else {
+#pragma unroll
+                            for (int r = 0; r < 4; ++r)
+                                if (col + r < cols) to[r] = y.e[r];
+                        }
+                    }
+                }
+            }
+            f32x4 x0 = L::wide(v0) * w[0], x1 = L::wide(v1) * w[1];
+            Quad y0 = L::round(x0), y1 = L::round(x1);
+#pragma unroll
+            for (int c = 0; c < NK; ++c) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) S[c][m][r] = st ? 0.0f : S[c][m][r] * pass;
+                S[c][m] = L::mma(kc[0][c], kc[1][c], y0, y1, S[c][m]);
+            }
+            if (L::SPLIT) {
+                x0 -= L::wide(y0);
+                x1 -= L::wide(y1);
+                y0 = L::round(x0);
+                y1 = L::round(x1);
+#pragma unroll
+                for (int c = 0; c < NK; ++c) S[c][m] = L::mma(kc[0][c], kc[1][c], y0, y1, S[c][m]);
+                y0 = L::round(x0 - L::wide(y0));
+                y1 = L::round(x1 - L::wide(y1));
+#pragma unroll
+                for (int c = 0; c < NK; ++c) S[c][m] = L::mma(kc[0][c], kc[1][c], y0, y1, S[c][m]);
+            }
+        }
+    }
+
+    if (local) {
+        float* to = a.carry + id * (NK * NV * 256);
+#pragma unroll
+        for (int c = 0; c < NK; ++c)
+#pragma unroll
+            for (int m = 0; m < NV; ++m) *(f32x4*)(to + (c * NV + m) * 256 + lane * 4) = S[c][m];
+        if (lane == 0) a.through[id] = through;
+        return;
+    }
+    if (a.state_out && seg == a.segs - 1) {
+        float* s1 = a.state_out + pair * (int64_t)a.dk * a.dv;
+#pragma unroll
+        for (int c = 0; c < NK; ++c)
+#pragma unroll
+            for (int m = 0; m < NV; ++m) {
+                const int col = m * 16 + i, row = L::state_row(c, g);
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (col < cols && row + r < a.dk) {
+                        odd += S[c][m][r] * 0.0f;
+                        if (a.state_t)
+                            s1[(int64_t)(col0 + col) * a.dk + row + r] = S[c][m][r];
+                        else
+                            s1[(int64_t)(row + r) * a.dv + col0 + col] = S[c][m][r];
+                    }
+            }
+    }
+    const bool any = __ballot(odd != 0.0f) != 0;       // (NaN is not 0 either)
+    if (lane == 0) a.odd[id] = any ? 1u : 0u;
+}
+
+// the states behind a pair's segments, chained: carry[s] = through[s] carry[s - 1] + carry[s]
+static __global__ void __launch_bounds__(256) chain_kernel(float* carry, const float* through, int32_t segs, int32_t per) {
+    const int64_t group = blockIdx.y;
+    const int at = blockIdx.x * 256 + threadIdx.x;
+    if (at >= per) return;
+    float* c = carry + group * segs * per + at;
+    const float* p = through + group * segs;
+    float s = c[0];
+#pragma unroll 8
+    for (int x = 1; x < segs - 1; ++x) {
+        const float f = p[x];
+        s = (f == 0.0f ? 0.0f : f * s) + c[(int64_t)x * per];
+        c[(int64_t)x * per] = s;
+    }
+}
+
+// ---- the recurrence itself, one step after the other, for pairs whose results are not all finite numbers: a product's masked terms
+// are zeros, and zero times NaN or infinity is NaN, so in such a pair values may have leaked into steps that do not see them.
+// Thread (column c, part p of eight) keeps 16 of the state's rows in registers. ----
+template <typename T, bool BACK>
+__device__ __forceinline__ void recurrent(const ChunkArgs& a, int64_t pair, int col0, float (&row)[2][kMaxHeadDim]) {
+    const int64_t n = pair / a.heads;
+    const int h = (int)(pair - n * a.heads);
+    const int g = threadIdx.x & 7, c = col0 + (threadIdx.x >> 3);
+    const float decay = expf(log_decay_of(a.log_decay, h));
+    const float* s0 = a.state ? a.state + pair * (int64_t)a.dk * a.dv : nullptr;
+    auto at = [&](int i) { return a.state_t ? (int64_t)c * a.dk + i : (int64_t)i * a.dv + c; };
+    float s[16];
+#pragma unroll
+    for (int x = 0; x < 16; ++x) {
+        const int i = x * 8 + g;
+        s[x] = s0 && i < a.dk && c < a.dv ? s0[at(i)] : 0.0f;
+    }
+    auto cut = [&](int64_t t) { return a.starts && a.starts[n * a.starts_batch + t * a.starts_step]; };
+    for (int64_t u = 0; u < a.steps; ++u) {
+        const int64_t t = BACK ? a.steps - 1 - u : u;
+        const T* qp = (const T*)a.q.p + n * a.q.batch + t * a.q.step + h * a.q.head;
+        const T* kp = (const T*)a.k.p + n * a.k.batch + t * a.k.step + h * a.k.head;
+        const T* vp = (const T*)a.v.p + n * a.v.batch + t * a.v.step + h * a.v.head;
+        __syncthreads();
+        for (int i = threadIdx.x; i < a.dk; i += 256) {
+            row[0][i] = to_f32(qp[i]) * a.read_scale;
+            row[1][i] = to_f32(kp[i]) * a.write_scale;
+        }
+        __syncthreads();
+        float keep = decay;
+        if (BACK)
+            keep = u == 0 ? 1.0f : cut(t + 1) ? 0.0f : decay;
+        else if (cut(t))
+            keep = 0.0f;
+        const float vc = c < a.dv ? to_f32(vp[c]) : 0.0f;
+        float o = 0.0f;
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+            const int i = x * 8 + g;
+            if (i < a.dk) {
+                s[x] = (keep == 0.0f ? 0.0f : keep * s[x]) + row[1][i] * vc;
+                o += row[0][i] * s[x];
+            }
+        }
+        o += __shfl_xor(o, 1);
+        o += __shfl_xor(o, 2);
+        o += __shfl_xor(o, 4);
+        if (g == 0 && c < a.dv) ((T*)a.out.p)[n * a.out.batch + t * a.out.step + h * a.out.head + c] = from_f32<T>(o);
+    }
+    if (a.state_out && c < a.dv) {
+        float* s1 = a.state_out + pair * (int64_t)a.dk * a.dv;
+        const float last = BACK && a.steps > 0 ? (cut(0) ? 0.0f : decay) : 1.0f;
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+            const int i = x * 8 + g;
+            if (i < a.dk) s1[at(i)] = last == 0.0f ? 0.0f : last * s[x];
+        }
+    }
+}
+
+constexpr int kOddGroup = 64;
+
+template <typename T, bool BACK>
+__global__ void __launch_bounds__(256) odd_kernel(ChunkArgs a, int64_t pairs) {
+    __shared__ float row[2][kMaxHeadDim];
+    __shared__ uint32_t odd[kOddGroup];
+    const int per = a.slices * a.segs;
+    for (int64_t p0 = (int64_t)blockIdx.x * kOddGroup; p0 < pairs; p0 += (int64_t)gridDim.x * kOddGroup) {
+        const int here = pairs - p0 < kOddGroup ? (int)(pairs - p0) : kOddGroup;
+        if (threadIdx.x < kOddGroup) odd[threadIdx.x] = 0;
+        __syncthreads();
+        for (int x = threadIdx.x; x < here * per; x += 256)
+            if (a.odd[p0 * per + x]) odd[x / per] = 1;
+        __syncthreads();
+        for (int x = 0; x < here; ++x) {
+            if (!odd[x]) continue;
+            for (int col = 0; col < a.dv; col += 32) recurrent<T, BACK>(a, p0 + x, col, row);
+        }
+        __syncthreads();
+    }
+}
+
+// How a walk over (batch, heads) pairs is cut: column slices of the state, and, where there are few waves and many steps, segments of
+// the steps, whose states are computed first (from k and v alone) and chained.
+struct WalkPlan {
+    int nk, nv, slices, segs;
+    int64_t seg_steps;
+};
+
+static WalkPlan walk_plan(int64_t pairs, int64_t steps, int dk, int dv) {
+    WalkPlan p;
+    p.nk = dk <= 32 ? 2 : dk <= 64 ? 4 : 8;
+    p.nv = dv <= 32 ? 2 : 4;
+    p.slices = (int)ceil_div(dv, p.nv * 16);
+    // 1024 SIMDs, two waves each; a segment costs a state written, read, chained and read, so it is at least eight chunks long
+    const int64_t waves = pairs * p.slices, want = waves > 0 ? 2048 / waves : 1, most = steps / (8 * kChunk);
+    int64_t segs = want < most ? want : most;
+    if (segs < 2) segs = 1;
+    p.seg_steps = segs > 1 ? round_up(ceil_div(steps, segs), kChunk) : (steps > 0 ? steps : 1);
+    p.segs = steps > 0 ? (int)ceil_div(steps, p.seg_steps) : 1;
+    return p;
+}
+
+struct WalkWork {
+    float *carry, *through;
+    uint32_t* odd;
+    int64_t bytes;
+};
+
+static WalkWork walk_work(const WalkPlan& p, int64_t pairs, void* at) {
+    Carve c(at);
+    WalkWork w{};
+    const int64_t units = pairs * p.slices * p.segs;
+    w.odd = c.take<uint32_t>(units);
+    if (p.segs > 1) {
+        w.through = c.take<float>(units);
+        w.carry = c.take<float>(units * p.nk * p.nv * 256);
+    }
+    w.bytes = c.used + 256;
+    return w;
+}
+
+template <typename T, bool BACK>
+int walk(const FishingDecayAttention* f, Strided q, Strided k, Strided v, const float* state, float* state_out, Strided out, int dk, int dv, bool state_t,
+                double read_scale, double write_scale, void* workspace, hipStream_t stream) {
+    const int64_t pairs = f->batch * f->heads;
+    const WalkPlan p = walk_plan(pairs, f->steps, dk, dv);
+    const WalkWork w = walk_work(p, pairs, workspace);
+    constexpr int V = vec_of<T>();
+    auto wide = [&](const Strided& s, int d) { return d % V == 0 && aligned16(s.p) && s.batch % V == 0 && s.step % V == 0 && s.head % V == 0; };
+    const ChunkArgs a{q, k, v, out, f->log_decay, f->starts, f->starts_stride[0], f->starts_stride[1], state, state_out, f->steps, f->heads, dk, dv, state_t,
+                      (float)read_scale, (float)write_scale, p.slices, p.segs, p.seg_steps, w.carry, w.through, w.odd};
+    const bool vec = wide(q, dk) && wide(k, dk) && wide(v, dv) && wide(out, dv);
+    const dim3 grid((unsigned)(pairs * p.slices * p.segs));
+    auto run = [&](auto kernel) {
+        int rc = 0;
+        if (p.segs > 1) {
+            rc = launch(kernel, grid, dim3(64), stream, a, true);
+            const int per = p.nk * p.nv * 256;
+            if (!rc) rc = launch(chain_kernel, dim3((unsigned)ceil_div(per, 256), (unsigned)(pairs * p.slices)), dim3(256), stream, w.carry, w.through, p.segs, per);
+        }
+        return rc ? rc : launch(kernel, grid, dim3(64), stream, a, false);
+    };
+    auto tiles = [&](auto wide_rows) {
+        constexpr bool W = decltype(wide_rows)::value;
+        return p.nv == 2 ? (p.nk == 2 ? run(chunk_kernel<T, 2, 2, BACK, W>) : p.nk == 4 ? run(chunk_kernel<T, 4, 2, BACK, W>) : run(chunk_kernel<T, 8, 2, BACK, W>))
+                         : (p.nk == 2 ? run(chunk_kernel<T, 2, 4, BACK, W>) : p.nk == 4 ? run(chunk_kernel<T, 4, 4, BACK, W>) : run(chunk_kernel<T, 8, 4, BACK, W>));
+    };
+    const int rc = vec ? tiles(std::true_type{}) : tiles(std::false_type{});
+    if (rc) return rc;
+    const int64_t groups = ceil_div(pairs, kOddGroup);
+    return launch(odd_kernel<T, BACK>, dim3((unsigned)(groups < 1024 ? groups : 1024)), dim3(256), stream, a, pairs);
+}
+
+}  // namespace seq
+}  // namespace fishing
