@@ -66,27 +66,11 @@ struct Carve {
     }
 };
 
-// Matrix-core tiles.  16 x 16 outputs, lane l: the A operand's row / B operand's column is l % 16, its k indices are
-// (l / 16) * E .. + E - 1 (E = 8 for bf16 with k = 32, 1 for f32 with k = 4); the accumulator's column is l % 16, its four
-// rows (l / 16) * 4 .. + 3.
-template <typename T>
-struct Mma;
-template <>
-struct Mma<bf16> {
-    static constexpr int K = 32, E = 8;
-    typedef bf16x8 Frag;
-    static __device__ __forceinline__ f32x4 run(Frag a, Frag b, f32x4 c) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
-    }
-};
-template <>
-struct Mma<float> {
-    static constexpr int K = 4, E = 1;
-    typedef float Frag;
-    static __device__ __forceinline__ f32x4 run(Frag a, Frag b, f32x4 c) {
-        return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
-    }
-};
+// Workgroups are dealt round-robin over the 8 XCDs, each with its own L2: hand each XCD a contiguous run
+__device__ __forceinline__ int64_t xcd_run(int64_t id, int64_t count) {
+    const int64_t per = count / 8, rest = count % 8, x = id % 8, at = id / 8;
+    return x * per + (x < rest ? x : rest) + at;
+}
 
 }  // namespace seq
 }  // namespace fishing

@@ -211,11 +211,5 @@ struct Gemm {
     }
 };
 
-// Workgroups are dealt round-robin over the 8 XCDs, each with its own L2: hand each XCD a contiguous run of tiles
-__device__ __forceinline__ int64_t xcd_tile(int64_t id, int64_t count) {
-    const int64_t per = count / 8, rest = count % 8, x = id % 8, at = id / 8;
-    return x * per + (x < rest ? x : rest) + at;
-}
-
 }  // namespace seq
 }  // namespace fishing

@@ -16,7 +16,7 @@ struct Strided {
 // exp(-inf * 0) would be NaN: a decay of zero is carried as a logarithm far below float32's range
 __device__ __forceinline__ float log_decay_of(const float* log_decay, int h) { return fmaxf(log_decay[h], -1.0e4f); }
 
-// ---- whole episodes, 32 steps at a time: one wave owns a (batch, head), up to 64 columns of its state, and a run of steps ----
+// ---- whole episodes, a chunk of 32 (f32: 16) steps at a time: one wave owns a (batch, head), up to 64 columns of its state, and a run of steps ----
 //
 // With g = exp(log_decay) and the steps x of a chunk of n, "open" meaning that no start lies between:
 //   forwards   o_x = sum_{y <= x, open} g^(x-y) (q_x . k_y) v_y + [open to the chunk's front] g^(x+1) q_x S
@@ -39,6 +39,7 @@ struct Lanes<bf16> {
     typedef short s16x4 __attribute__((ext_vector_type(4)));
     typedef s16x4 Quad;
     static constexpr bool SPLIT = true;
+    static constexpr int TILES = 2;            // of 16 steps in a chunk: the products over steps take 32 at once
     // four steps y of one column; each lane names the 8 bytes (4 columns of one step) that it contributes
     static __device__ __forceinline__ Quad column(const char* rows, int pitch, int y0, int col, int spread) {
         const int i = threadIdx.x & 15, g = threadIdx.x >> 4 & 3;
@@ -64,6 +65,7 @@ struct Lanes<bf16> {
         } a{{a0, a1}}, b{{b0, b1}};
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.f, b.f, acc, 0, 0, 0);
     }
+    static __device__ __forceinline__ f32x4 over_steps(const Quad (&a)[2], const Quad (&b)[2], f32x4 acc) { return mma(a[0], a[1], b[0], b[1], acc); }
     static __device__ __forceinline__ Quad round(f32x4 x) {
         union {
             bf16x4 h;
@@ -84,6 +86,7 @@ template <>
 struct Lanes<float> {
     typedef f32x4 Quad;
     static constexpr bool SPLIT = false;
+    static constexpr int TILES = 1;            // the products over steps take 4 at once: longer chunks would only add masked scores
     static __device__ __forceinline__ Quad column(const char* rows, int pitch, int y0, int col) {
         const int i = threadIdx.x & 15, g = threadIdx.x >> 4 & 3;
         Quad x;
@@ -106,35 +109,54 @@ struct Lanes<float> {
         for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a1[e], b1[e], acc, 0, 0, 0);
         return acc;
     }
+    static __device__ __forceinline__ f32x4 over_steps(const Quad (&a)[1], const Quad (&b)[1], f32x4 acc) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[0][e], b[0][e], acc, 0, 0, 0);
+        return acc;
+    }
     static __device__ __forceinline__ Quad round(f32x4 x) { return x; }
     static __device__ __forceinline__ f32x4 wide(Quad x) { return x; }
 };
 
-constexpr int kChunk = 32;
-
-// a chunk's rows of one operand on their way from memory: 16 bytes a lane and load, rows behind the last and columns behind d zero
-template <typename T, int TILES>
+// A chunk's rows of one operand on their way from memory, 16 bytes a lane and load.  A load covers whole rows, so the loads of a
+// lane differ by a uniform step.  Rows behind the last and columns behind d are zeros.
+template <typename T, int TILES, int STEPS>
 struct Rows {
-    static constexpr int EPC = 16 / (int)sizeof(T), CHUNKS = TILES * 16 / EPC, LOADS = kChunk * CHUNKS / 64, PITCH = TILES * 16 * (int)sizeof(T) + 16;
+    static constexpr int EPC = 16 / (int)sizeof(T), CHUNKS = TILES * 16 / EPC, PER = 64 / CHUNKS > 0 ? 64 / CHUNKS : 1, ACROSS = CHUNKS > 64 ? CHUNKS / 64 : 1;
+    static constexpr bool EVEN = 64 % CHUNKS == 0;                    // (96 columns: 12 chunks a row do not divide 64 lanes)
+    static constexpr int LOADS = EVEN ? STEPS / PER : (STEPS * CHUNKS + 63) / 64, PITCH = TILES * 16 * (int)sizeof(T) + 16;
     u32x4 x[LOADS];
 
     template <bool VEC>
-    __device__ __forceinline__ void load(const Strided& o, int64_t n, int64_t h, int64_t t0, int rows, int d) {
-        const T* p = (const T*)o.p + n * o.batch + h * o.head + t0 * o.step;
+    static __device__ __forceinline__ u32x4 one(const T* from, int c, int d) {
+        if (VEC) return *(const u32x4*)from;
+        Pack<T, EPC> y;
 #pragma unroll
-        for (int s = 0; s < LOADS; ++s) {
-            const int at = s * 64 + threadIdx.x, row = at / CHUNKS, c = at % CHUNKS * EPC;
-            x[s] = u32x4{0, 0, 0, 0};
-            if (row < rows && c < d) {
-                const T* from = p + row * o.step + c;
-                if (VEC) {
-                    x[s] = *(const u32x4*)from;
-                } else {
-                    Pack<T, EPC> y;
+        for (int e = 0; e < EPC; ++e) y.e[e] = c + e < d ? from[e] : from_f32<T>(0.0f);
+        return *(const u32x4*)&y;
+    }
+    // p: the chunk's first row (uniform)
+    template <bool VEC>
+    __device__ __forceinline__ void load(const T* p, int64_t step, int rows, int d) {
 #pragma unroll
-                    for (int e = 0; e < EPC; ++e) y.e[e] = c + e < d ? from[e] : from_f32<T>(0.0f);
-                    x[s] = *(const u32x4*)&y;
-                }
+        for (int s = 0; s < LOADS; ++s) x[s] = u32x4{0, 0, 0, 0};
+        if (EVEN) {
+            const int row = threadIdx.x / CHUNKS, c = threadIdx.x % CHUNKS * EPC;
+            if (c >= d) return;
+            const int64_t at = row * step + c;
+            if (rows == STEPS) {
+#pragma unroll
+                for (int s = 0; s < LOADS; ++s) x[s] = one<VEC>(p + s * PER * step + at, c, d);
+            } else {
+#pragma unroll
+                for (int s = 0; s < LOADS; ++s)
+                    if (row + s * PER < rows) x[s] = one<VEC>(p + s * PER * step + at, c, d);
+            }
+        } else {
+#pragma unroll
+            for (int s = 0; s < LOADS; ++s) {
+                const int at = s * 64 + threadIdx.x, row = at / CHUNKS, c = at % CHUNKS * EPC;
+                if (row < rows && c < d) x[s] = one<VEC>(p + row * step + c, c, d);
             }
         }
     }
@@ -142,7 +164,7 @@ struct Rows {
 #pragma unroll
         for (int s = 0; s < LOADS; ++s) {
             const int at = s * 64 + threadIdx.x;
-            *(u32x4*)(lds + at / CHUNKS * PITCH + at % CHUNKS * 16) = x[s];
+            if (EVEN || at < STEPS * CHUNKS) *(u32x4*)(lds + at / CHUNKS * PITCH + at % CHUNKS * 16) = x[s];
         }
     }
 };
@@ -164,29 +186,48 @@ struct ChunkArgs {
     uint32_t* odd;             // per (pair, slice, segment): some result is infinite or NaN
 };
 
-// LOCAL: only the state that a segment adds (from zero; the first from the state carried in), for the segments to be chained.
+// local: only the state that a segment adds (from zero; the first from the state carried in), for the segments to be chained.
 template <typename T, int NK, int NV, bool BACK, bool VEC>
-__global__ void __launch_bounds__(64, (NK * NV * (int)sizeof(T) >= 64 ? 1 : 2)) chunk_kernel(ChunkArgs a, bool local) {
+__global__ void __launch_bounds__(64, (NK * NV >= 24 ? 1 : 2)) chunk_kernel(ChunkArgs a, bool local) {
     typedef Lanes<T> L;
     typedef typename L::Quad Quad;
-    typedef Rows<T, NK> RK;
-    typedef Rows<T, NV> RV;
-    __shared__ __attribute__((aligned(16))) char qs[kChunk * RK::PITCH];
-    __shared__ __attribute__((aligned(16))) char ks[kChunk * RK::PITCH];
-    __shared__ __attribute__((aligned(16))) char vs[kChunk * RV::PITCH];
+    constexpr int TS = L::TILES, CH = 16 * TS;
+    typedef Rows<T, NK, CH> RK;
+    typedef Rows<T, NV, CH> RV;
+    __shared__ __attribute__((aligned(16))) char qs[CH * RK::PITCH];
+    __shared__ __attribute__((aligned(16))) char ks[CH * RK::PITCH];
+    __shared__ __attribute__((aligned(16))) char vs[CH * RV::PITCH];
     const int lane = threadIdx.x, i = lane & 15, g = lane >> 4;
-    const int64_t id = blockIdx.x, pair = id / (a.slices * a.segs);
+    // (slices of a pair read the same q and k: neighbours on one XCD)
+    const int64_t id = xcd_run(blockIdx.x, gridDim.x), pair = id / (a.slices * a.segs);
     const int rest = (int)(id - pair * (a.slices * a.segs)), slice = rest / a.segs, seg = rest - slice * a.segs;
     if (local && seg == a.segs - 1) return;                  // nothing follows it
     const int64_t n = pair / a.heads, h = pair - n * a.heads;
     const int col0 = slice * NV * 16, cols = a.dv - col0;
-    Strided v = a.v, out = a.out;
-    v.p = (const T*)v.p + col0;
+    const T* qp = (const T*)a.q.p + n * a.q.batch + h * a.q.head;
+    const T* kp = (const T*)a.k.p + n * a.k.batch + h * a.k.head;
+    const T* vp = (const T*)a.v.p + n * a.v.batch + h * a.v.head + col0;
+    T* op = (T*)a.out.p + n * a.out.batch + h * a.out.head + col0;
     // segments are counted in the direction of the walk
     const int64_t at = BACK ? a.segs - 1 - seg : seg, t_lo = at * a.seg_steps, t_hi = t_lo + a.seg_steps < a.steps ? t_lo + a.seg_steps : a.steps;
-    const int chunks = (int)ceil_div(t_hi - t_lo, kChunk);
+    const int chunks = (int)ceil_div(t_hi - t_lo, CH);
     const float ld = log_decay_of(a.log_decay, (int)h), l2 = ld * 1.4426950408889634f;
-    const float whole = (float)exp((double)ld * kChunk);     // the factor that compounds: rounded once
+    const float whole = (float)exp((double)ld * CH);     // the factor that compounds: rounded once
+
+    // What a chunk without a start weighs its terms with: a score of steps d apart, in order; a step's k v^T behind the chunk; the
+    // state in front at a step
+    f32x4 near[TS], behind[TS];
+    float ahead[TS];
+#pragma unroll
+    for (int t = 0; t < TS; ++t) {
+        ahead[t] = a.read_scale * __builtin_amdgcn_exp2f((BACK ? CH - 1 - (16 * t + i) : 16 * t + i + 1) * l2);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int y = 4 * g + r, d = BACK ? y - i + 16 * t : i + 16 * t - y;      // (tiles t apart)
+            near[t][r] = d >= 0 ? __builtin_amdgcn_exp2f(d * l2) * (a.read_scale * a.write_scale) : 0.0f;
+            behind[t][r] = a.write_scale * __builtin_amdgcn_exp2f((BACK ? 16 * t + y + 1 : CH - 1 - (16 * t + y)) * l2);
+        }
+    }
 
     f32x4 S[NK][NV];
     {
@@ -211,19 +252,21 @@ __global__ void __launch_bounds__(64, (NK * NV * (int)sizeof(T) >= 64 ? 1 : 2)) 
     RK rq, rk;
     RV rv;
     bool started = false;
+    auto front = [&](int x) { return t_lo + (int64_t)(BACK ? chunks - 1 - x : x) * CH; };
+    auto count = [&](int64_t t0) { return t_hi - t0 < CH ? (int)(t_hi - t0) : CH; };
     auto fetch = [&](int x) {
-        const int64_t t0 = t_lo + (int64_t)(BACK ? chunks - 1 - x : x) * kChunk;
-        const int rows = t_hi - t0 < kChunk ? (int)(t_hi - t0) : kChunk;
-        if (!local) rq.template load<VEC>(a.q, n, h, t0, rows, a.dk);
-        rk.template load<VEC>(a.k, n, h, t0, rows, a.dk);
-        rv.template load<VEC>(v, n, h, t0, rows, cols);
+        const int64_t t0 = front(x);
+        const int rows = count(t0);
+        if (!local) rq.template load<VEC>(qp + t0 * a.q.step, a.q.step, rows, a.dk);
+        rk.template load<VEC>(kp + t0 * a.k.step, a.k.step, rows, a.dk);
+        rv.template load<VEC>(vp + t0 * a.v.step, a.v.step, rows, cols);
         started = a.starts && lane < rows && a.starts[n * a.starts_batch + (t0 + lane) * a.starts_step];
     };
     float odd = 0.0f, through = 1.0f;
     if (chunks > 0) fetch(0);
     for (int x = 0; x < chunks; ++x) {
-        const int64_t t0 = t_lo + (int64_t)(BACK ? chunks - 1 - x : x) * kChunk;
-        const int rows = t_hi - t0 < kChunk ? (int)(t_hi - t0) : kChunk;
+        const int64_t t0 = front(x);
+        const int rows = count(t0);
         __syncthreads();
         if (!local) rq.put(qs);
         rk.put(ks);
@@ -232,99 +275,110 @@ __global__ void __launch_bounds__(64, (NK * NV * (int)sizeof(T) >= 64 ? 1 : 2)) 
         __syncthreads();
         if (x + 1 < chunks) fetch(x + 1);
 
-        // what a chunk of `rows` steps lets of the state through, and of each step's k v^T into it
-        const float pass = st ? 0.0f : rows == kChunk ? whole : exp2f(rows * l2);
-        f32x4 w[2];
-        {
-            const int from = BACK ? 0 : st ? 31 - __clz(st) : 0, to = BACK ? (st ? __ffs(st) - 1 : kChunk) : kChunk;
+        f32x4 w[TS];
+        float into[TS], pass = whole;
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < TS; ++t) {
+            w[t] = behind[t];
+            into[t] = ahead[t];
+        }
+        if (st || rows != CH) {                   // uniform: few chunks
+            const int from = BACK ? 0 : st ? 31 - __clz(st) : 0, to = BACK && st ? __ffs(st) - 1 : rows;
+            pass = st ? 0.0f : exp2f(rows * l2);
+#pragma unroll
+            for (int t = 0; t < TS; ++t) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const int y = 16 * t + 4 * g + r;
-                    w[t][r] = y >= from && y < to && y < rows ? a.write_scale * __builtin_amdgcn_exp2f((BACK ? y + 1 : rows - 1 - y) * l2) : 0.0f;
+                    w[t][r] = y >= from && y < to ? a.write_scale * __builtin_amdgcn_exp2f((BACK ? y + 1 : rows - 1 - y) * l2) : 0.0f;
                 }
+                const int step = 16 * t + i;
+                const uint32_t upto = (2u << step) - 1u;
+                const bool shut = BACK ? (st & ~upto) != 0 || step >= rows : (st & upto) != 0;
+                into[t] = shut ? 0.0f : a.read_scale * __builtin_amdgcn_exp2f((BACK ? rows - 1 - step : step + 1) * l2);
+            }
         }
+        through = st ? 0.0f : through * pass;
 
-        Quad q[2][NK], p[2][2], p_rest[2][2];     // [step tile][...]; scores: four y in registers, x in lanes
-        float into[2];                            // what a step sees of the state in front of the chunk
+        Quad q[TS][NK], p[TS][TS], p_rest[TS][TS];     // [step tile][...]; scores: four y in registers, x in lanes
         if (!local) {
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+            for (int t = 0; t < TS; ++t)
 #pragma unroll
                 for (int c = 0; c < NK / 2; ++c) L::row_quads(qs, RK::PITCH, 16 * t + i, c, q[t][2 * c], q[t][2 * c + 1]);
 #pragma unroll
-            for (int ky = 0; ky < 2; ++ky) {
+            for (int ky = 0; ky < TS; ++ky) {
                 Quad k[NK];
 #pragma unroll
                 for (int c = 0; c < NK / 2; ++c) L::row_quads(ks, RK::PITCH, 16 * ky + i, c, k[2 * c], k[2 * c + 1]);
 #pragma unroll
-                for (int t = 0; t < 2; ++t) {
+                for (int t = 0; t < TS; ++t) {
                     f32x4 z = {0.0f, 0.0f, 0.0f, 0.0f};
                     if (BACK ? t <= ky : t >= ky) {        // (else no pair of these tiles is in order)
 #pragma unroll
                         for (int c = 0; c < NK; c += 2) z = L::mma(k[c], k[c + 1], q[t][c], q[t][c + 1], z);
-                        const int step = 16 * t + i;
-                        const uint32_t upto = (2u << step) - 1u, near = BACK ? st & ~upto : st & upto;
-                        const int lo = BACK ? step : near ? 31 - __clz(near) : 0, hi = BACK ? (near ? __ffs(near) - 1 : kChunk) : step + 1;
+                        z *= near[BACK ? ky - t : t - ky];
+                        if (st) {
+                            const int step = 16 * t + i;
+                            const uint32_t upto = (2u << step) - 1u, cuts = BACK ? st & ~upto : st & upto;
+                            const int lo = !BACK && cuts ? 31 - __clz(cuts) : 0, hi = BACK && cuts ? __ffs(cuts) - 1 : CH;
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            const int y = 16 * ky + 4 * g + r;
-                            const float d = __builtin_amdgcn_exp2f((BACK ? y - step : step - y) * l2) * (a.read_scale * a.write_scale);
-                            z[r] = y >= lo && y < hi ? z[r] * d : 0.0f;
+                            for (int r = 0; r < 4; ++r) {
+                                const int y = 16 * ky + 4 * g + r;
+                                z[r] = y >= lo && y < hi ? z[r] : 0.0f;
+                            }
                         }
                     }
                     p[t][ky] = L::round(z);
                     if (L::SPLIT) p_rest[t][ky] = L::round(z - L::wide(p[t][ky]));
                 }
             }
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const int step = 16 * t + i;
-                const uint32_t upto = (2u << step) - 1u, near = BACK ? st & ~upto : st & upto;
-                into[t] = near ? 0.0f : a.read_scale * __builtin_amdgcn_exp2f((BACK ? rows - 1 - step : step + 1) * l2);
-            }
         }
-        through = st ? 0.0f : through * pass;
 
-        Quad kc[2][NK];
+        Quad kc[NK][TS];
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < TS; ++t)
 #pragma unroll
-            for (int c = 0; c < NK; ++c) kc[t][c] = L::state_column(ks, RK::PITCH, 16 * t, c);
+            for (int c = 0; c < NK; ++c) kc[c][t] = L::state_column(ks, RK::PITCH, 16 * t, c);
 #pragma unroll
         for (int m = 0; m < NV; ++m) {
             __builtin_amdgcn_sched_barrier(0);    // (16 columns at a time: their intermediates are a quarter of the registers)
-            const Quad v0 = L::value_column(vs, RV::PITCH, 0, m), v1 = L::value_column(vs, RV::PITCH, 16, m);
-            if (!local) {
-                f32x4 o[2];
+            Quad v[TS];
 #pragma unroll
-                for (int t = 0; t < 2; ++t) o[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int t = 0; t < TS; ++t) v[t] = L::value_column(vs, RV::PITCH, 16 * t, m);
+            if (!local) {
+                f32x4 o[TS];
+#pragma unroll
+                for (int t = 0; t < TS; ++t) o[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int c = 0; c < NK; c += 2) {
                     const Quad s0 = L::round(S[c][m]), s1 = L::round(S[c + 1][m]);
 #pragma unroll
-                    for (int t = 0; t < 2; ++t) o[t] = L::mma(s0, s1, q[t][c], q[t][c + 1], o[t]);
+                    for (int t = 0; t < TS; ++t) o[t] = L::mma(s0, s1, q[t][c], q[t][c + 1], o[t]);
                     if (L::SPLIT) {
                         const Quad r0 = L::round(S[c][m] - L::wide(s0)), r1 = L::round(S[c + 1][m] - L::wide(s1));
 #pragma unroll
-                        for (int t = 0; t < 2; ++t) o[t] = L::mma(r0, r1, q[t][c], q[t][c + 1], o[t]);
+                        for (int t = 0; t < TS; ++t) o[t] = L::mma(r0, r1, q[t][c], q[t][c + 1], o[t]);
                     }
                 }
+                if (st) {                          // what is shut out may not be a number
 #pragma unroll
-                for (int t = 0; t < 2; ++t) {
+                    for (int t = 0; t < TS; ++t)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) o[t][r] = into[t] == 0.0f ? 0.0f : o[t][r] * into[t];
-                    o[t] = L::mma(v0, v1, p[t][0], p[t][1], o[t]);
-                    if (L::SPLIT) o[t] = L::mma(v0, v1, p_rest[t][0], p_rest[t][1], o[t]);
+                        for (int r = 0; r < 4; ++r) o[t][r] = into[t] == 0.0f ? 0.0f : o[t][r];
+                }
+#pragma unroll
+                for (int t = 0; t < TS; ++t) {
+                    o[t] = L::over_steps(v, p[t], o[t] * into[t]);
+                    if (L::SPLIT) o[t] = L::over_steps(v, p_rest[t], o[t]);
                     const int step = 16 * t + i, col = m * 16 + 4 * g;
                     if (step < rows) {
-                        T* to = (T*)out.p + n * out.batch + h * out.head + (t0 + step) * out.step + col0 + col;
+                        T* to = op + (t0 + step) * a.out.step + col;
                         Pack<T, 4> y;
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
                             y.e[r] = from_f32<T>(o[t][r]);
-                            if (col + r < cols) odd += o[t][r] * 0.0f;         // NaN from anything that is not a finite number
+                            odd += o[t][r] * 0.0f;         // NaN from anything that is not a finite number
                         }
                         if (VEC) {
                             if (col < cols) *(Pack<T, 4>*)to = y;
@@ -336,25 +390,30 @@ __global__ void __launch_bounds__(64, (NK * NV * (int)sizeof(T) >= 64 ? 1 : 2)) 
                     }
                 }
             }
-            f32x4 x0 = L::wide(v0) * w[0], x1 = L::wide(v1) * w[1];
-            Quad y0 = L::round(x0), y1 = L::round(x1);
+            f32x4 rest[TS];
+            Quad y[TS];
 #pragma unroll
-            for (int c = 0; c < NK; ++c) {
-#pragma unroll
-                for (int r = 0; r < 4; ++r) S[c][m][r] = st ? 0.0f : S[c][m][r] * pass;
-                S[c][m] = L::mma(kc[0][c], kc[1][c], y0, y1, S[c][m]);
+            for (int t = 0; t < TS; ++t) {
+                rest[t] = L::wide(v[t]) * w[t];
+                y[t] = L::round(rest[t]);
             }
+            if (st) {
+#pragma unroll
+                for (int c = 0; c < NK; ++c) S[c][m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            }
+#pragma unroll
+            for (int c = 0; c < NK; ++c) S[c][m] = L::over_steps(kc[c], y, S[c][m] * pass);
             if (L::SPLIT) {
-                x0 -= L::wide(y0);
-                x1 -= L::wide(y1);
-                y0 = L::round(x0);
-                y1 = L::round(x1);
 #pragma unroll
-                for (int c = 0; c < NK; ++c) S[c][m] = L::mma(kc[0][c], kc[1][c], y0, y1, S[c][m]);
-                y0 = L::round(x0 - L::wide(y0));
-                y1 = L::round(x1 - L::wide(y1));
+                for (int e = 0; e < 2; ++e) {
 #pragma unroll
-                for (int c = 0; c < NK; ++c) S[c][m] = L::mma(kc[0][c], kc[1][c], y0, y1, S[c][m]);
+                    for (int t = 0; t < TS; ++t) {
+                        rest[t] -= L::wide(y[t]);
+                        y[t] = L::round(rest[t]);
+                    }
+#pragma unroll
+                    for (int c = 0; c < NK; ++c) S[c][m] = L::over_steps(kc[c], y, S[c][m]);
+                }
             }
         }
     }
@@ -497,14 +556,14 @@ struct WalkPlan {
 
 static WalkPlan walk_plan(int64_t pairs, int64_t steps, int dk, int dv) {
     WalkPlan p;
-    p.nk = dk <= 32 ? 2 : dk <= 64 ? 4 : 8;
+    p.nk = dk <= 32 ? 2 : dk <= 64 ? 4 : dk <= 96 ? 6 : 8;
     p.nv = dv <= 32 ? 2 : 4;
     p.slices = (int)ceil_div(dv, p.nv * 16);
-    // 1024 SIMDs, two waves each; a segment costs a state written, read, chained and read, so it is at least eight chunks long
-    const int64_t waves = pairs * p.slices, want = waves > 0 ? 2048 / waves : 1, most = steps / (8 * kChunk);
+    // 1024 SIMDs, two waves each; a segment costs a state written, read, chained and read, so it is at least 256 steps long
+    const int64_t waves = pairs * p.slices, want = waves > 0 ? 2048 / waves : 1, most = steps / 256;
     int64_t segs = want < most ? want : most;
     if (segs < 2) segs = 1;
-    p.seg_steps = segs > 1 ? round_up(ceil_div(steps, segs), kChunk) : (steps > 0 ? steps : 1);
+    p.seg_steps = segs > 1 ? round_up(ceil_div(steps, segs), 32) : (steps > 0 ? steps : 1);
     p.segs = steps > 0 ? (int)ceil_div(steps, p.seg_steps) : 1;
     return p;
 }
@@ -551,8 +610,10 @@ int walk(const FishingDecayAttention* f, Strided q, Strided k, Strided v, const 
     };
     auto tiles = [&](auto wide_rows) {
         constexpr bool W = decltype(wide_rows)::value;
-        return p.nv == 2 ? (p.nk == 2 ? run(chunk_kernel<T, 2, 2, BACK, W>) : p.nk == 4 ? run(chunk_kernel<T, 4, 2, BACK, W>) : run(chunk_kernel<T, 8, 2, BACK, W>))
-                         : (p.nk == 2 ? run(chunk_kernel<T, 2, 4, BACK, W>) : p.nk == 4 ? run(chunk_kernel<T, 4, 4, BACK, W>) : run(chunk_kernel<T, 8, 4, BACK, W>));
+        return p.nv == 2 ? (p.nk == 2 ? run(chunk_kernel<T, 2, 2, BACK, W>) : p.nk == 4 ? run(chunk_kernel<T, 4, 2, BACK, W>)
+                            : p.nk == 6 ? run(chunk_kernel<T, 6, 2, BACK, W>) : run(chunk_kernel<T, 8, 2, BACK, W>))
+                         : (p.nk == 2 ? run(chunk_kernel<T, 2, 4, BACK, W>) : p.nk == 4 ? run(chunk_kernel<T, 4, 4, BACK, W>)
+                            : p.nk == 6 ? run(chunk_kernel<T, 6, 4, BACK, W>) : run(chunk_kernel<T, 8, 4, BACK, W>));
     };
     const int rc = vec ? tiles(std::true_type{}) : tiles(std::false_type{});
     if (rc) return rc;
