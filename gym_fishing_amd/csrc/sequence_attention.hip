@@ -150,10 +150,15 @@ int fishing_decay_attention_step(const FishingDecayAttention* a, fishing_stream_
 
 int64_t fishing_decay_attention_workspace(const FishingDecayAttention* a, int32_t backward) {
     if (int rc = attention_check(a, false)) return rc;
-    const int64_t pairs = a->batch * a->heads, one = walk_work(walk_plan(pairs, a->steps, a->dk, a->dv), pairs, nullptr).bytes;
-    if (!backward) return one;
-    const int64_t other = walk_work(walk_plan(pairs, a->steps, a->dv, a->dk), pairs, nullptr).bytes;      // the walks run one after the other
-    return one > other ? one : other;
+    // the largest of its walks, which run one after the other, whichever way their rows are read
+    const int64_t pairs = a->batch * a->heads;
+    int64_t most = 0;
+    for (int back = 0; back <= (backward ? 1 : 0); ++back)
+        for (int wide = 0; wide < 2; ++wide) {
+            const int64_t b = walk_work(walk_plan(pairs, a->steps, back ? a->dv : a->dk, back ? a->dk : a->dv, wide != 0), pairs, nullptr).bytes;
+            most = b > most ? b : most;
+        }
+    return most;
 }
 
 int fishing_decay_attention_forward(const FishingDecayAttention* a, void* workspace, int64_t workspace_bytes, fishing_stream_t stream) {

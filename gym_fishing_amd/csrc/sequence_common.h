@@ -66,6 +66,14 @@ struct Carve {
     }
 };
 
+// A value that is the same in every lane, into scalar registers: what a run-time division yields is in vector registers, and so
+// would be every address made of it
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ int64_t uniform(int64_t x) {
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)x), hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)((uint64_t)x >> 32));
+    return (int64_t)((uint64_t)hi << 32 | lo);
+}
+
 // Workgroups are dealt round-robin over the 8 XCDs, each with its own L2: hand each XCD a contiguous run
 __device__ __forceinline__ int64_t xcd_run(int64_t id, int64_t count) {
     const int64_t per = count / 8, rest = count % 8, x = id % 8, at = id / 8;

@@ -70,7 +70,7 @@ __global__ void __launch_bounds__(G::THREADS, 2)
     __shared__ __attribute__((aligned(16))) char lds0[G::BYTES];
     __shared__ __attribute__((aligned(16))) char lds1[G::BYTES];
     const int64_t tile = xcd_run(blockIdx.x, tiles_m * tiles_n);
-    const int64_t tm = tile % tiles_m, tn = tile / tiles_m;
+    const int64_t tn = uniform(tile / tiles_m), tm = tile - tn * tiles_m;
     // the target's column in this tile, or -1; read behind the product's barriers
     __shared__ int column[BM];
     if (threadIdx.x < BM) {
@@ -162,7 +162,7 @@ __global__ void __launch_bounds__(G::THREADS, 2)
     __shared__ __attribute__((aligned(16))) char lds0[G::BYTES];
     __shared__ __attribute__((aligned(16))) char lds1[G::BYTES];
     const int64_t tile = xcd_run(blockIdx.x, tiles_m * tiles_n);
-    const int64_t tm = tile % tiles_m, tn = tile / tiles_m;
+    const int64_t tn = uniform(tile / tiles_m), tm = tile - tn * tiles_m;
     // per row of the tile, read behind the product's barriers: lse (infinite for a padded target: a share of zero), the loss's
     // gradient, the target's column or -1
     __shared__ float row_lse[BM], row_g[BM];
@@ -208,7 +208,7 @@ __global__ void __launch_bounds__(G::THREADS, 2)
     __shared__ __attribute__((aligned(16))) char lds0[G::BYTES];
     __shared__ __attribute__((aligned(16))) char lds1[G::BYTES];
     const int64_t tile = xcd_run(blockIdx.x, tiles_m * tiles_n);
-    const int64_t tm = tile % tiles_m, tn = tile / tiles_m;
+    const int64_t tn = uniform(tile / tiles_m), tm = tile - tn * tiles_m;
     const int64_t lo = blockIdx.y * share, hi = lo + share < k ? lo + share : k;
     f32x4 acc[G::MT][G::NT];
     G::run(lds0, lds1, a, tm * BM, b, tn * BN, lo, hi, acc);

@@ -66,20 +66,21 @@ struct Lanes<bf16> {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.f, b.f, acc, 0, 0, 0);
     }
     static __device__ __forceinline__ f32x4 over_steps(const Quad (&a)[2], const Quad (&b)[2], f32x4 acc) { return mma(a[0], a[1], b[0], b[1], acc); }
+    // (two at a time, v_cvt_pk_bf16_f32; element by element the halves would live in registers of their own)
     static __device__ __forceinline__ Quad round(f32x4 x) {
         union {
             bf16x4 h;
             Quad q;
         } y;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) y.h[e] = (bf16)x[e];
+        y.h = __builtin_convertvector(x, bf16x4);
         return y.q;
     }
     static __device__ __forceinline__ f32x4 wide(Quad x) {
-        f32x4 y;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = __uint_as_float((uint32_t)(uint16_t)x[e] << 16);
-        return y;
+        union {
+            Quad q;
+            uint32_t u[2];
+        } y{x};
+        return f32x4{__uint_as_float(y.u[0] << 16), __uint_as_float(y.u[0] & 0xffff0000u), __uint_as_float(y.u[1] << 16), __uint_as_float(y.u[1] & 0xffff0000u)};
     }
 };
 template <>
@@ -118,53 +119,71 @@ struct Lanes<float> {
     static __device__ __forceinline__ f32x4 wide(Quad x) { return x; }
 };
 
-// A chunk's rows of one operand on their way from memory, 16 bytes a lane and load.  A load covers whole rows, so the loads of a
-// lane differ by a uniform step.  Rows behind the last and columns behind d are zeros.
-template <typename T, int TILES, int STEPS>
+// A chunk's rows of one operand on their way from memory, 16 bytes a lane and load.  Nothing is masked on the way in: columns behind
+// d and rows behind the last read ones that exist, and become zeros on the way to LDS, where a uniform test finds whole chunks.
+// VEC: the address is a uniform one and 32 bits of the lane's own.
+template <typename T, int TILES, int STEPS, bool VEC>
 struct Rows {
-    static constexpr int EPC = 16 / (int)sizeof(T), CHUNKS = TILES * 16 / EPC, PER = 64 / CHUNKS > 0 ? 64 / CHUNKS : 1, ACROSS = CHUNKS > 64 ? CHUNKS / 64 : 1;
-    static constexpr bool EVEN = 64 % CHUNKS == 0;                    // (96 columns: 12 chunks a row do not divide 64 lanes)
-    static constexpr int LOADS = EVEN ? STEPS / PER : (STEPS * CHUNKS + 63) / 64, PITCH = TILES * 16 * (int)sizeof(T) + 16;
+    static constexpr int EPC = 16 / (int)sizeof(T), CHUNKS = TILES * 16 / EPC, LOADS = STEPS * CHUNKS / 64, PITCH = TILES * 16 * (int)sizeof(T) + 16;
+    static constexpr bool EVEN = 64 % CHUNKS == 0;                    // (96 columns: 12 chunks a row do not divide the wave)
+    static constexpr int PER = EVEN ? 64 / CHUNKS : 0;                // rows of a load
+    static_assert(STEPS * CHUNKS % 64 == 0, "whole loads");
     u32x4 x[LOADS];
 
-    template <bool VEC>
-    static __device__ __forceinline__ u32x4 one(const T* from, int c, int d) {
-        if (VEC) return *(const u32x4*)from;
-        Pack<T, EPC> y;
-#pragma unroll
-        for (int e = 0; e < EPC; ++e) y.e[e] = c + e < d ? from[e] : from_f32<T>(0.0f);
-        return *(const u32x4*)&y;
+    static __device__ __forceinline__ int row_of(int s) { return EVEN ? threadIdx.x / CHUNKS + s * PER : (s * 64 + threadIdx.x) / CHUNKS; }
+    static __device__ __forceinline__ int chunk_of(int s) { return EVEN ? threadIdx.x % CHUNKS : (s * 64 + threadIdx.x) % CHUNKS; }
+
+    static __device__ __forceinline__ u32x4 at(const T* base, uint32_t bytes) {
+        asm("" : "+v"(bytes));                    // (kept next to the load: hoisted, it becomes a 64-bit pair of registers per load)
+        return *(const u32x4*)((const char*)base + bytes);
     }
     // p: the chunk's first row (uniform)
-    template <bool VEC>
     __device__ __forceinline__ void load(const T* p, int64_t step, int rows, int d) {
+        if constexpr (!VEC) {
 #pragma unroll
-        for (int s = 0; s < LOADS; ++s) x[s] = u32x4{0, 0, 0, 0};
-        if (EVEN) {
-            const int row = threadIdx.x / CHUNKS, c = threadIdx.x % CHUNKS * EPC;
-            if (c >= d) return;
-            const int64_t at = row * step + c;
-            if (rows == STEPS) {
+            for (int s = 0; s < LOADS; ++s) {
+                const int r = row_of(s), c = chunk_of(s) * EPC;
+                const T* from = p + (r < rows ? r : rows - 1) * step;
+                Pack<T, EPC> y;
 #pragma unroll
-                for (int s = 0; s < LOADS; ++s) x[s] = one<VEC>(p + s * PER * step + at, c, d);
-            } else {
-#pragma unroll
-                for (int s = 0; s < LOADS; ++s)
-                    if (row + s * PER < rows) x[s] = one<VEC>(p + s * PER * step + at, c, d);
+                for (int e = 0; e < EPC; ++e) y.e[e] = from[c + e < d ? c + e : 0];
+                x[s] = *(const u32x4*)&y;
             }
+        } else if (EVEN && rows == STEPS) {
+            const int c = chunk_of(0) * EPC;
+            const uint32_t mine = ((uint32_t)row_of(0) * (uint32_t)step + (c < d ? c : 0)) * (uint32_t)sizeof(T);
+#pragma unroll
+            for (int s = 0; s < LOADS; ++s) x[s] = at(p + (int64_t)(s * PER) * step, mine);
         } else {
 #pragma unroll
             for (int s = 0; s < LOADS; ++s) {
-                const int at = s * 64 + threadIdx.x, row = at / CHUNKS, c = at % CHUNKS * EPC;
-                if (row < rows && c < d) x[s] = one<VEC>(p + row * step + c, c, d);
+                const int r = row_of(s), c = chunk_of(s) * EPC;
+                x[s] = at(p, ((uint32_t)(r < rows ? r : rows - 1) * (uint32_t)step + (c < d ? c : 0)) * (uint32_t)sizeof(T));
             }
         }
     }
-    __device__ __forceinline__ void put(char* lds) const {
+    __device__ __forceinline__ void put(char* lds, int rows, int d) {
+        if (rows != STEPS || d < TILES * 16) {
+#pragma unroll
+            for (int s = 0; s < LOADS; ++s) {
+                const int r = row_of(s), c = chunk_of(s) * EPC;
+                if constexpr (VEC) {
+                    if (r >= rows || c >= d) x[s] = u32x4{0, 0, 0, 0};
+                } else {
+                    Pack<T, EPC> y = *(const Pack<T, EPC>*)&x[s];
+#pragma unroll
+                    for (int e = 0; e < EPC; ++e) y.e[e] = r < rows && c + e < d ? y.e[e] : from_f32<T>(0.0f);
+                    x[s] = *(const u32x4*)&y;
+                }
+            }
+        }
+        char* to = lds + threadIdx.x / CHUNKS * PITCH + threadIdx.x % CHUNKS * 16;
 #pragma unroll
         for (int s = 0; s < LOADS; ++s) {
-            const int at = s * 64 + threadIdx.x;
-            if (EVEN || at < STEPS * CHUNKS) *(u32x4*)(lds + at / CHUNKS * PITCH + at % CHUNKS * 16) = x[s];
+            if (EVEN)
+                *(u32x4*)(to + s * PER * PITCH) = x[s];
+            else
+                *(u32x4*)(lds + row_of(s) * PITCH + chunk_of(s) * 16) = x[s];
         }
     }
 };
@@ -186,23 +205,24 @@ struct ChunkArgs {
     uint32_t* odd;             // per (pair, slice, segment): some result is infinite or NaN
 };
 
-// local: only the state that a segment adds (from zero; the first from the state carried in), for the segments to be chained.
-template <typename T, int NK, int NV, bool BACK, bool VEC>
-__global__ void __launch_bounds__(64, (NK * NV >= 24 ? 1 : 2)) chunk_kernel(ChunkArgs a, bool local) {
+// LOCAL: only the state that a segment adds (from zero; the first from the state carried in), for the segments to be chained.
+template <typename T, int NK, int NV, bool BACK, bool VEC, bool LOCAL>
+__global__ void __launch_bounds__(64, (NK * NV >= 24 ? 1 : 2)) chunk_kernel(ChunkArgs a) {
     typedef Lanes<T> L;
     typedef typename L::Quad Quad;
     constexpr int TS = L::TILES, CH = 16 * TS;
-    typedef Rows<T, NK, CH> RK;
-    typedef Rows<T, NV, CH> RV;
+    typedef Rows<T, NK, CH, VEC> RK;
+    typedef Rows<T, NV, CH, VEC> RV;
     __shared__ __attribute__((aligned(16))) char qs[CH * RK::PITCH];
     __shared__ __attribute__((aligned(16))) char ks[CH * RK::PITCH];
     __shared__ __attribute__((aligned(16))) char vs[CH * RV::PITCH];
     const int lane = threadIdx.x, i = lane & 15, g = lane >> 4;
     // (slices of a pair read the same q and k: neighbours on one XCD)
-    const int64_t id = xcd_run(blockIdx.x, gridDim.x), pair = id / (a.slices * a.segs);
-    const int rest = (int)(id - pair * (a.slices * a.segs)), slice = rest / a.segs, seg = rest - slice * a.segs;
-    if (local && seg == a.segs - 1) return;                  // nothing follows it
-    const int64_t n = pair / a.heads, h = pair - n * a.heads;
+    const uint32_t units = (uint32_t)(a.slices * a.segs);
+    const int64_t id = xcd_run(blockIdx.x, gridDim.x), pair = uniform((int)((uint32_t)id / units));
+    const int rest = (int)id - (int)pair * (int)units, slice = uniform((int)((uint32_t)rest / (uint32_t)a.segs)), seg = rest - slice * a.segs;
+    if (LOCAL && seg == a.segs - 1) return;                  // nothing follows it
+    const int64_t n = uniform((int)((uint32_t)pair / (uint32_t)a.heads)), h = pair - n * a.heads;
     const int col0 = slice * NV * 16, cols = a.dv - col0;
     const T* qp = (const T*)a.q.p + n * a.q.batch + h * a.q.head;
     const T* kp = (const T*)a.k.p + n * a.k.batch + h * a.k.head;
@@ -211,23 +231,18 @@ __global__ void __launch_bounds__(64, (NK * NV >= 24 ? 1 : 2)) chunk_kernel(Chun
     // segments are counted in the direction of the walk
     const int64_t at = BACK ? a.segs - 1 - seg : seg, t_lo = at * a.seg_steps, t_hi = t_lo + a.seg_steps < a.steps ? t_lo + a.seg_steps : a.steps;
     const int chunks = (int)ceil_div(t_hi - t_lo, CH);
-    const float ld = log_decay_of(a.log_decay, (int)h), l2 = ld * 1.4426950408889634f;
-    const float whole = (float)exp((double)ld * CH);     // the factor that compounds: rounded once
+    const float ld = __int_as_float(uniform(__float_as_int(log_decay_of(a.log_decay, (int)h)))), l2 = ld * 1.4426950408889634f;
+    const float whole = __int_as_float(uniform(__float_as_int((float)exp((double)ld * CH))));     // the factor that compounds: rounded once
 
-    // What a chunk without a start weighs its terms with: a score of steps d apart, in order; a step's k v^T behind the chunk; the
-    // state in front at a step
-    f32x4 near[TS], behind[TS];
-    float ahead[TS];
+    // what a chunk without a start weighs a score of steps d apart with, in order, in tiles t apart
+    float near[TS][4];
 #pragma unroll
-    for (int t = 0; t < TS; ++t) {
-        ahead[t] = a.read_scale * __builtin_amdgcn_exp2f((BACK ? CH - 1 - (16 * t + i) : 16 * t + i + 1) * l2);
+    for (int t = 0; t < TS; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int y = 4 * g + r, d = BACK ? y - i + 16 * t : i + 16 * t - y;      // (tiles t apart)
+            const int y = 4 * g + r, d = BACK ? y - i + 16 * t : i + 16 * t - y;
             near[t][r] = d >= 0 ? __builtin_amdgcn_exp2f(d * l2) * (a.read_scale * a.write_scale) : 0.0f;
-            behind[t][r] = a.write_scale * __builtin_amdgcn_exp2f((BACK ? 16 * t + y + 1 : CH - 1 - (16 * t + y)) * l2);
         }
-    }
 
     f32x4 S[NK][NV];
     {
@@ -239,7 +254,7 @@ __global__ void __launch_bounds__(64, (NK * NV >= 24 ? 1 : 2)) chunk_kernel(Chun
             for (int m = 0; m < NV; ++m) {
                 S[c][m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
                 if (seg > 0) {
-                    if (!local) S[c][m] = *(const f32x4*)(from + (c * NV + m) * 256 + lane * 4);
+                    if (!LOCAL) S[c][m] = *(const f32x4*)(from + (c * NV + m) * 256 + lane * 4);
                 } else if (s0) {
                     const int col = m * 16 + i, row = L::state_row(c, g);
 #pragma unroll
@@ -251,16 +266,16 @@ __global__ void __launch_bounds__(64, (NK * NV >= 24 ? 1 : 2)) chunk_kernel(Chun
 
     RK rq, rk;
     RV rv;
-    bool started = false;
+    uint32_t started = 0;                         // the lane's step begins an episode (tested behind the wait for the rows)
     auto front = [&](int x) { return t_lo + (int64_t)(BACK ? chunks - 1 - x : x) * CH; };
     auto count = [&](int64_t t0) { return t_hi - t0 < CH ? (int)(t_hi - t0) : CH; };
     auto fetch = [&](int x) {
         const int64_t t0 = front(x);
         const int rows = count(t0);
-        if (!local) rq.template load<VEC>(qp + t0 * a.q.step, a.q.step, rows, a.dk);
-        rk.template load<VEC>(kp + t0 * a.k.step, a.k.step, rows, a.dk);
-        rv.template load<VEC>(vp + t0 * a.v.step, a.v.step, rows, cols);
-        started = a.starts && lane < rows && a.starts[n * a.starts_batch + (t0 + lane) * a.starts_step];
+        if (!LOCAL) rq.load(qp + t0 * a.q.step, a.q.step, rows, a.dk);
+        rk.load(kp + t0 * a.k.step, a.k.step, rows, a.dk);
+        rv.load(vp + t0 * a.v.step, a.v.step, rows, cols);
+        if (a.starts) started = a.starts[n * a.starts_batch + (t0 + (lane < rows ? lane : 0)) * a.starts_step];
     };
     float odd = 0.0f, through = 1.0f;
     if (chunks > 0) fetch(0);
@@ -268,46 +283,44 @@ __global__ void __launch_bounds__(64, (NK * NV >= 24 ? 1 : 2)) chunk_kernel(Chun
         const int64_t t0 = front(x);
         const int rows = count(t0);
         __syncthreads();
-        if (!local) rq.put(qs);
-        rk.put(ks);
-        rv.put(vs);
-        const uint32_t st = (uint32_t)__ballot(started);
+        if (!LOCAL) rq.put(qs, rows, a.dk);
+        rk.put(ks, rows, a.dk);
+        rv.put(vs, rows, cols);
+        const uint32_t st = (uint32_t)__ballot(started != 0 && lane < rows);
         __syncthreads();
-        if (x + 1 < chunks) fetch(x + 1);
-
-        f32x4 w[TS];
-        float into[TS], pass = whole;
+        // the weights of each step's k v^T behind the chunk, and of the state in front of it at each step (made anew: kept, they are
+        // registers that the rows in flight need)
+        float w[TS][4], into[TS], pass = whole;
+        int from = 0, to = rows;
+        uint32_t cuts[TS];
+        if (st || rows != CH) {                   // uniform: few chunks
+            pass = st ? 0.0f : exp2f(rows * l2);
+            if (!BACK && st) from = 31 - __clz(st);
+            if (BACK && st) to = __ffs(st) - 1;
+        }
 #pragma unroll
         for (int t = 0; t < TS; ++t) {
-            w[t] = behind[t];
-            into[t] = ahead[t];
-        }
-        if (st || rows != CH) {                   // uniform: few chunks
-            const int from = BACK ? 0 : st ? 31 - __clz(st) : 0, to = BACK && st ? __ffs(st) - 1 : rows;
-            pass = st ? 0.0f : exp2f(rows * l2);
 #pragma unroll
-            for (int t = 0; t < TS; ++t) {
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int y = 16 * t + 4 * g + r;
-                    w[t][r] = y >= from && y < to ? a.write_scale * __builtin_amdgcn_exp2f((BACK ? y + 1 : rows - 1 - y) * l2) : 0.0f;
-                }
-                const int step = 16 * t + i;
-                const uint32_t upto = (2u << step) - 1u;
-                const bool shut = BACK ? (st & ~upto) != 0 || step >= rows : (st & upto) != 0;
-                into[t] = shut ? 0.0f : a.read_scale * __builtin_amdgcn_exp2f((BACK ? rows - 1 - step : step + 1) * l2);
+            for (int r = 0; r < 4; ++r) {
+                const int y = 16 * t + 4 * g + r;
+                w[t][r] = y >= from && y < to ? a.write_scale * __builtin_amdgcn_exp2f((BACK ? y + 1 : rows - 1 - y) * l2) : 0.0f;
             }
+            const int step = 16 * t + i;
+            const uint32_t upto = (2u << step) - 1u;
+            cuts[t] = BACK ? st & ~upto : st & upto;
+            into[t] = cuts[t] || step >= rows ? 0.0f : a.read_scale * __builtin_amdgcn_exp2f((BACK ? rows - 1 - step : step + 1) * l2);
         }
         through = st ? 0.0f : through * pass;
 
         Quad q[TS][NK], p[TS][TS], p_rest[TS][TS];     // [step tile][...]; scores: four y in registers, x in lanes
-        if (!local) {
+        if (!LOCAL) {
 #pragma unroll
             for (int t = 0; t < TS; ++t)
 #pragma unroll
                 for (int c = 0; c < NK / 2; ++c) L::row_quads(qs, RK::PITCH, 16 * t + i, c, q[t][2 * c], q[t][2 * c + 1]);
 #pragma unroll
             for (int ky = 0; ky < TS; ++ky) {
+                __builtin_amdgcn_sched_barrier(0);
                 Quad k[NK];
 #pragma unroll
                 for (int c = 0; c < NK / 2; ++c) L::row_quads(ks, RK::PITCH, 16 * ky + i, c, k[2 * c], k[2 * c + 1]);
@@ -317,11 +330,10 @@ __global__ void __launch_bounds__(64, (NK * NV >= 24 ? 1 : 2)) chunk_kernel(Chun
                     if (BACK ? t <= ky : t >= ky) {        // (else no pair of these tiles is in order)
 #pragma unroll
                         for (int c = 0; c < NK; c += 2) z = L::mma(k[c], k[c + 1], q[t][c], q[t][c + 1], z);
-                        z *= near[BACK ? ky - t : t - ky];
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) z[r] *= near[BACK ? ky - t : t - ky][r];
                         if (st) {
-                            const int step = 16 * t + i;
-                            const uint32_t upto = (2u << step) - 1u, cuts = BACK ? st & ~upto : st & upto;
-                            const int lo = !BACK && cuts ? 31 - __clz(cuts) : 0, hi = BACK && cuts ? __ffs(cuts) - 1 : CH;
+                            const int lo = !BACK && cuts[t] ? 31 - __clz(cuts[t]) : 0, hi = BACK && cuts[t] ? __ffs(cuts[t]) - 1 : CH;
 #pragma unroll
                             for (int r = 0; r < 4; ++r) {
                                 const int y = 16 * ky + 4 * g + r;
@@ -335,18 +347,21 @@ __global__ void __launch_bounds__(64, (NK * NV >= 24 ? 1 : 2)) chunk_kernel(Chun
             }
         }
 
+        __builtin_amdgcn_sched_barrier(0);
         Quad kc[NK][TS];
 #pragma unroll
         for (int t = 0; t < TS; ++t)
 #pragma unroll
             for (int c = 0; c < NK; ++c) kc[c][t] = L::state_column(ks, RK::PITCH, 16 * t, c);
+        __builtin_amdgcn_sched_barrier(0);
+        if (x + 1 < chunks) fetch(x + 1);         // (behind the scores: their operands and the rows in flight do not fit together)
 #pragma unroll
         for (int m = 0; m < NV; ++m) {
             __builtin_amdgcn_sched_barrier(0);    // (16 columns at a time: their intermediates are a quarter of the registers)
             Quad v[TS];
 #pragma unroll
             for (int t = 0; t < TS; ++t) v[t] = L::value_column(vs, RV::PITCH, 16 * t, m);
-            if (!local) {
+            if (!LOCAL) {
                 f32x4 o[TS];
 #pragma unroll
                 for (int t = 0; t < TS; ++t) o[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -373,28 +388,29 @@ __global__ void __launch_bounds__(64, (NK * NV >= 24 ? 1 : 2)) chunk_kernel(Chun
                     if (L::SPLIT) o[t] = L::over_steps(v, p_rest[t], o[t]);
                     const int step = 16 * t + i, col = m * 16 + 4 * g;
                     if (step < rows) {
-                        T* to = op + (t0 + step) * a.out.step + col;
-                        Pack<T, 4> y;
+                        uint32_t mine = (i * (uint32_t)a.out.step + col) * (uint32_t)sizeof(T);
+                        asm("" : "+v"(mine));
+                        T* to = VEC ? (T*)((char*)(op + (t0 + 16 * t) * a.out.step) + mine) : op + (t0 + step) * a.out.step + col;
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            y.e[r] = from_f32<T>(o[t][r]);
-                            odd += o[t][r] * 0.0f;         // NaN from anything that is not a finite number
-                        }
+                        for (int r = 0; r < 4; ++r) odd += o[t][r] * 0.0f;         // NaN from anything that is not a finite number
                         if (VEC) {
-                            if (col < cols) *(Pack<T, 4>*)to = y;
+                            if (col < cols) *(Quad*)to = L::round(o[t]);
                         } else {
 #pragma unroll
                             for (int r = 0; r < 4; ++r)
-                                if (col + r < cols) to[r] = y.e[r];
+                                if (col + r < cols) to[r] = from_f32<T>(o[t][r]);
                         }
                     }
                 }
             }
+            __builtin_amdgcn_sched_barrier(0);
             f32x4 rest[TS];
             Quad y[TS];
 #pragma unroll
             for (int t = 0; t < TS; ++t) {
-                rest[t] = L::wide(v[t]) * w[t];
+                rest[t] = L::wide(v[t]);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) rest[t][r] *= w[t][r];
                 y[t] = L::round(rest[t]);
             }
             if (st) {
@@ -418,7 +434,7 @@ __global__ void __launch_bounds__(64, (NK * NV >= 24 ? 1 : 2)) chunk_kernel(Chun
         }
     }
 
-    if (local) {
+    if (LOCAL) {
         float* to = a.carry + id * (NK * NV * 256);
 #pragma unroll
         for (int c = 0; c < NK; ++c)
@@ -554,10 +570,10 @@ struct WalkPlan {
     int64_t seg_steps;
 };
 
-static WalkPlan walk_plan(int64_t pairs, int64_t steps, int dk, int dv) {
+static WalkPlan walk_plan(int64_t pairs, int64_t steps, int dk, int dv, bool wide) {
     WalkPlan p;
     p.nk = dk <= 32 ? 2 : dk <= 64 ? 4 : dk <= 96 ? 6 : 8;
-    p.nv = dv <= 32 ? 2 : 4;
+    p.nv = dv <= 32 || !wide ? 2 : 4;            // (rows that are not whole 16-byte accesses: one width is enough)
     p.slices = (int)ceil_div(dv, p.nv * 16);
     // 1024 SIMDs, two waves each; a segment costs a state written, read, chained and read, so it is at least 256 steps long
     const int64_t waves = pairs * p.slices, want = waves > 0 ? 2048 / waves : 1, most = steps / 256;
@@ -567,6 +583,9 @@ static WalkPlan walk_plan(int64_t pairs, int64_t steps, int dk, int dv) {
     p.segs = steps > 0 ? (int)ceil_div(steps, p.seg_steps) : 1;
     return p;
 }
+
+template <int N>
+using Count = std::integral_constant<int, N>;
 
 struct WalkWork {
     float *carry, *through;
@@ -591,31 +610,31 @@ template <typename T, bool BACK>
 int walk(const FishingDecayAttention* f, Strided q, Strided k, Strided v, const float* state, float* state_out, Strided out, int dk, int dv, bool state_t,
                 double read_scale, double write_scale, void* workspace, hipStream_t stream) {
     const int64_t pairs = f->batch * f->heads;
-    const WalkPlan p = walk_plan(pairs, f->steps, dk, dv);
-    const WalkWork w = walk_work(p, pairs, workspace);
     constexpr int V = vec_of<T>();
-    auto wide = [&](const Strided& s, int d) { return d % V == 0 && aligned16(s.p) && s.batch % V == 0 && s.step % V == 0 && s.head % V == 0; };
+    auto wide = [&](const Strided& s, int d) {
+        return d % V == 0 && aligned16(s.p) && s.batch % V == 0 && s.step % V == 0 && s.head % V == 0 && s.step < (int64_t)1 << 24;      // 32 rows in 32 bits
+    };
+    const bool vec = wide(q, dk) && wide(k, dk) && wide(v, dv) && wide(out, dv);
+    const WalkPlan p = walk_plan(pairs, f->steps, dk, dv, vec);
+    const WalkWork w = walk_work(p, pairs, workspace);
     const ChunkArgs a{q, k, v, out, f->log_decay, f->starts, f->starts_stride[0], f->starts_stride[1], state, state_out, f->steps, f->heads, dk, dv, state_t,
                       (float)read_scale, (float)write_scale, p.slices, p.segs, p.seg_steps, w.carry, w.through, w.odd};
-    const bool vec = wide(q, dk) && wide(k, dk) && wide(v, dv) && wide(out, dv);
     const dim3 grid((unsigned)(pairs * p.slices * p.segs));
-    auto run = [&](auto kernel) {
+    auto run = [&](auto tk, auto tv, auto rows) {
+        constexpr int NK = decltype(tk)::value, NV = decltype(tv)::value;
+        constexpr bool VEC = decltype(rows)::value;
         int rc = 0;
         if (p.segs > 1) {
-            rc = launch(kernel, grid, dim3(64), stream, a, true);
-            const int per = p.nk * p.nv * 256;
+            rc = launch(chunk_kernel<T, NK, NV, BACK, VEC, true>, grid, dim3(64), stream, a);
+            const int per = NK * NV * 256;
             if (!rc) rc = launch(chain_kernel, dim3((unsigned)ceil_div(per, 256), (unsigned)(pairs * p.slices)), dim3(256), stream, w.carry, w.through, p.segs, per);
         }
-        return rc ? rc : launch(kernel, grid, dim3(64), stream, a, false);
+        return rc ? rc : launch(chunk_kernel<T, NK, NV, BACK, VEC, false>, grid, dim3(64), stream, a);
     };
-    auto tiles = [&](auto wide_rows) {
-        constexpr bool W = decltype(wide_rows)::value;
-        return p.nv == 2 ? (p.nk == 2 ? run(chunk_kernel<T, 2, 2, BACK, W>) : p.nk == 4 ? run(chunk_kernel<T, 4, 2, BACK, W>)
-                            : p.nk == 6 ? run(chunk_kernel<T, 6, 2, BACK, W>) : run(chunk_kernel<T, 8, 2, BACK, W>))
-                         : (p.nk == 2 ? run(chunk_kernel<T, 2, 4, BACK, W>) : p.nk == 4 ? run(chunk_kernel<T, 4, 4, BACK, W>)
-                            : p.nk == 6 ? run(chunk_kernel<T, 6, 4, BACK, W>) : run(chunk_kernel<T, 8, 4, BACK, W>));
+    auto tiles = [&](auto tv, auto rows) {
+        return p.nk == 2 ? run(Count<2>{}, tv, rows) : p.nk == 4 ? run(Count<4>{}, tv, rows) : p.nk == 6 ? run(Count<6>{}, tv, rows) : run(Count<8>{}, tv, rows);
     };
-    const int rc = vec ? tiles(std::true_type{}) : tiles(std::false_type{});
+    const int rc = !vec ? tiles(Count<2>{}, std::false_type{}) : p.nv == 2 ? tiles(Count<2>{}, std::true_type{}) : tiles(Count<4>{}, std::true_type{});
     if (rc) return rc;
     const int64_t groups = ceil_div(pairs, kOddGroup);
     return launch(odd_kernel<T, BACK>, dim3((unsigned)(groups < 1024 ? groups : 1024)), dim3(256), stream, a, pairs);
