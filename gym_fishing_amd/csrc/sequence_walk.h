@@ -151,9 +151,13 @@ struct Rows {
             }
         } else if (EVEN && rows == STEPS) {
             const int c = chunk_of(0) * EPC;
-            const uint32_t mine = ((uint32_t)row_of(0) * (uint32_t)step + (c < d ? c : 0)) * (uint32_t)sizeof(T);
+            uint32_t mine = ((uint32_t)row_of(0) * (uint32_t)step + (c < d ? c : 0)) * (uint32_t)sizeof(T);
+            const uint32_t next = (uint32_t)(PER * (int)sizeof(T)) * (uint32_t)step;
 #pragma unroll
-            for (int s = 0; s < LOADS; ++s) x[s] = at(p + (int64_t)(s * PER) * step, mine);
+            for (int s = 0; s < LOADS; ++s) {
+                x[s] = at(p, mine);
+                mine += next;
+            }
         } else {
 #pragma unroll
             for (int s = 0; s < LOADS; ++s) {
@@ -312,6 +316,7 @@ __global__ void __launch_bounds__(64, (NK * NV >= 24 ? 1 : 2)) chunk_kernel(Chun
         }
         through = st ? 0.0f : through * pass;
 
+        T* o_front = op + t0 * a.out.step;
         Quad q[TS][NK], p[TS][TS], p_rest[TS][TS];     // [step tile][...]; scores: four y in registers, x in lanes
         if (!LOCAL) {
 #pragma unroll
@@ -376,21 +381,16 @@ __global__ void __launch_bounds__(64, (NK * NV >= 24 ? 1 : 2)) chunk_kernel(Chun
                         for (int t = 0; t < TS; ++t) o[t] = L::mma(r0, r1, q[t][c], q[t][c + 1], o[t]);
                     }
                 }
-                if (st) {                          // what is shut out may not be a number
-#pragma unroll
-                    for (int t = 0; t < TS; ++t)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) o[t][r] = into[t] == 0.0f ? 0.0f : o[t][r];
-                }
 #pragma unroll
                 for (int t = 0; t < TS; ++t) {
+                    if (t > 0 && rows <= 16 * t) continue;             // (uniform: the last chunk of an episode batch is often short)
                     o[t] = L::over_steps(v, p[t], o[t] * into[t]);
                     if (L::SPLIT) o[t] = L::over_steps(v, p_rest[t], o[t]);
                     const int step = 16 * t + i, col = m * 16 + 4 * g;
                     if (step < rows) {
-                        uint32_t mine = (i * (uint32_t)a.out.step + col) * (uint32_t)sizeof(T);
+                        uint32_t mine = ((uint32_t)step * (uint32_t)a.out.step + 4 * g) * (uint32_t)sizeof(T);
                         asm("" : "+v"(mine));
-                        T* to = VEC ? (T*)((char*)(op + (t0 + 16 * t) * a.out.step) + mine) : op + (t0 + step) * a.out.step + col;
+                        T* to = (VEC ? (T*)((char*)o_front + mine) : o_front + step * a.out.step + 4 * g) + m * 16;
 #pragma unroll
                         for (int r = 0; r < 4; ++r) odd += o[t][r] * 0.0f;         // NaN from anything that is not a finite number
                         if (VEC) {
@@ -412,10 +412,6 @@ __global__ void __launch_bounds__(64, (NK * NV >= 24 ? 1 : 2)) chunk_kernel(Chun
 #pragma unroll
                 for (int r = 0; r < 4; ++r) rest[t][r] *= w[t][r];
                 y[t] = L::round(rest[t]);
-            }
-            if (st) {
-#pragma unroll
-                for (int c = 0; c < NK; ++c) S[c][m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
             }
 #pragma unroll
             for (int c = 0; c < NK; ++c) S[c][m] = L::over_steps(kc[c], y, S[c][m] * pass);
