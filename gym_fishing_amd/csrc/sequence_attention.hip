@@ -115,22 +115,22 @@ static int attention_step(const FishingDecayAttention* a, hipStream_t stream) {
     return go(step_kernel_recurrent<T, 1>);
 }
 
-extern template int walk<float, true>(const FishingDecayAttention*, Strided, Strided, Strided, const float*, float*, Strided, int, int, bool, double, double, void*, hipStream_t);
-extern template int walk<bf16, true>(const FishingDecayAttention*, Strided, Strided, Strided, const float*, float*, Strided, int, int, bool, double, double, void*, hipStream_t);
+extern template int walk<float, true>(const FishingDecayAttention*, Strided, Strided, Strided, const float*, float*, Strided, int, int, bool, bool, double, double, void*, hipStream_t);
+extern template int walk<bf16, true>(const FishingDecayAttention*, Strided, Strided, Strided, const float*, float*, Strided, int, int, bool, bool, double, double, void*, hipStream_t);
 
 template <typename T>
 static int attention_forward(const FishingDecayAttention* a, void* work, hipStream_t stream) {
     return walk<T, false>(a, strided(a->q, a->q_stride), strided(a->k, a->k_stride), strided(a->v, a->v_stride), a->state, a->state_out,
-                               strided((const void*)a->out, a->out_stride), a->dk, a->dv, false, a->scale, 1.0, work, stream);
+                               strided((const void*)a->out, a->out_stride), a->dk, a->dv, false, true, a->scale, 1.0, work, stream);
 }
 
 template <typename T>
 static int attention_backward(const FishingDecayAttention* a, void* work, hipStream_t stream) {
     const Strided q = strided(a->q, a->q_stride), k = strided(a->k, a->k_stride), v = strided(a->v, a->v_stride), g = strided(a->dout, a->dout_stride);
     // dq: read with do the state that (v, k) build;  dk, dv: read with v, k the state's gradient that (do, q), (q, do) build backwards
-    int rc = walk<T, false>(a, g, v, k, a->state, nullptr, strided((const void*)a->dq, a->dq_stride), a->dv, a->dk, true, a->scale, 1.0, work, stream);
-    if (!rc) rc = walk<T, true>(a, v, g, q, a->dstate_out, nullptr, strided((const void*)a->dk_out, a->dk_stride), a->dv, a->dk, true, 1.0, a->scale, work, stream);
-    if (!rc) rc = walk<T, true>(a, k, q, g, a->dstate_out, a->dstate, strided((const void*)a->dv_out, a->dv_stride), a->dk, a->dv, false, 1.0, a->scale, work, stream);
+    int rc = walk<T, false>(a, g, v, k, a->state, nullptr, strided((const void*)a->dq, a->dq_stride), a->dv, a->dk, true, false, a->scale, 1.0, work, stream);
+    if (!rc) rc = walk<T, true>(a, v, g, q, a->dstate_out, nullptr, strided((const void*)a->dk_out, a->dk_stride), a->dv, a->dk, true, false, 1.0, a->scale, work, stream);
+    if (!rc) rc = walk<T, true>(a, k, q, g, a->dstate_out, a->dstate, strided((const void*)a->dv_out, a->dv_stride), a->dk, a->dv, false, a->dstate != nullptr, 1.0, a->scale, work, stream);
     return rc;
 }
 

@@ -26,9 +26,10 @@ __device__ __forceinline__ float log_decay_of(const float* log_decay, int h) { r
 // so a chunk is four small products on the matrix cores.  The layouts chain without a shuffle: the tile k q^T has its columns in
 // lanes and four rows y in registers, which is the second operand of v^T (k q^T); a state tile k^T v likewise is the first of S^T q^T;
 // the outputs come as four neighbouring columns of one step per lane.  k and v are read by columns through the transposing LDS read
-// (bf16) or element reads (f32).  bf16: scores, the state's copy and the decayed v, which the products need in bf16, are carried as
-// two bf16 terms (16 bits; the decayed v as three: the state is an answer in float32): one term would lose 1.7x the output's own
-// rounding, and the matrix cores have the time.
+// (bf16) or element reads (f32).  bf16: the products need scores, the state and
+// the decayed v in bf16.  The state's copy is rounded once, as the output is; the scores go as two bf16 terms (16 bits) and the decayed
+// v as two or, where the state is an answer in float32, three: every one of them rounded once would add up to 2x the output's own
+// rounding, this way it is 1.0 - 1.4x.
 // A wave alone needs no barriers; the next chunk's rows are loaded into registers while this one is computed.  Bound by HBM: q, k, v
 // read, out written once.
 
@@ -201,7 +202,7 @@ struct ChunkArgs {
     float* state_out;
     int64_t steps;
     int32_t heads, dk, dv;
-    bool state_t;
+    bool state_t, exact_state;
     float read_scale, write_scale;
     int32_t slices, segs;
     int64_t seg_steps;
@@ -238,15 +239,23 @@ __global__ void __launch_bounds__(64, (NK * NV >= 24 ? 1 : 2)) chunk_kernel(Chun
     const float ld = __int_as_float(uniform(__float_as_int(log_decay_of(a.log_decay, (int)h)))), l2 = ld * 1.4426950408889634f;
     const float whole = __int_as_float(uniform(__float_as_int((float)exp((double)ld * CH))));     // the factor that compounds: rounded once
 
-    // what a chunk without a start weighs a score of steps d apart with, in order, in tiles t apart
-    float near[TS][4];
+    // What a whole chunk without a start weighs its terms with, per lane: a score of steps d apart, in order, in tiles t apart; a step's
+    // k v^T behind the chunk; the state in front of the chunk at a step.  In LDS: the registers are the rows' in flight.
+    __shared__ f32x4 near_of[TS][64], behind_of[TS][64];
+    __shared__ float ahead_of[TS][64];
 #pragma unroll
-    for (int t = 0; t < TS; ++t)
+    for (int t = 0; t < TS; ++t) {
+        f32x4 x, y4;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int y = 4 * g + r, d = BACK ? y - i + 16 * t : i + 16 * t - y;
-            near[t][r] = d >= 0 ? __builtin_amdgcn_exp2f(d * l2) * (a.read_scale * a.write_scale) : 0.0f;
+            x[r] = d >= 0 ? __builtin_amdgcn_exp2f(d * l2) * (a.read_scale * a.write_scale) : 0.0f;
+            y4[r] = a.write_scale * __builtin_amdgcn_exp2f((BACK ? 16 * t + y + 1 : CH - 1 - (16 * t + y)) * l2);
         }
+        near_of[t][lane] = x;
+        behind_of[t][lane] = y4;
+        ahead_of[t][lane] = a.read_scale * __builtin_amdgcn_exp2f((BACK ? CH - 1 - (16 * t + i) : 16 * t + i + 1) * l2);
+    }
 
     f32x4 S[NK][NV];
     {
@@ -292,27 +301,27 @@ __global__ void __launch_bounds__(64, (NK * NV >= 24 ? 1 : 2)) chunk_kernel(Chun
         rv.put(vs, rows, cols);
         const uint32_t st = (uint32_t)__ballot(started != 0 && lane < rows);
         __syncthreads();
-        // the weights of each step's k v^T behind the chunk, and of the state in front of it at each step (made anew: kept, they are
-        // registers that the rows in flight need)
-        float w[TS][4], into[TS], pass = whole;
-        int from = 0, to = rows;
-        uint32_t cuts[TS];
-        if (st || rows != CH) {                   // uniform: few chunks
-            pass = st ? 0.0f : exp2f(rows * l2);
-            if (!BACK && st) from = 31 - __clz(st);
-            if (BACK && st) to = __ffs(st) - 1;
-        }
+        f32x4 w[TS];
+        float into[TS], pass = whole;
 #pragma unroll
         for (int t = 0; t < TS; ++t) {
+            w[t] = behind_of[t][lane];
+            into[t] = ahead_of[t][lane];
+        }
+        if (st || rows != CH) {                   // uniform: few chunks
+            pass = st ? 0.0f : exp2f(rows * l2);
+            const int from = !BACK && st ? 31 - __clz(st) : 0, to = BACK && st ? __ffs(st) - 1 : rows;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int y = 16 * t + 4 * g + r;
-                w[t][r] = y >= from && y < to ? a.write_scale * __builtin_amdgcn_exp2f((BACK ? y + 1 : rows - 1 - y) * l2) : 0.0f;
+            for (int t = 0; t < TS; ++t) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int y = 16 * t + 4 * g + r;
+                    w[t][r] = y >= from && y < to ? a.write_scale * __builtin_amdgcn_exp2f((BACK ? y + 1 : rows - 1 - y) * l2) : 0.0f;
+                }
+                const int step = 16 * t + i;
+                const uint32_t upto = (2u << step) - 1u, cuts = BACK ? st & ~upto : st & upto;
+                into[t] = cuts || step >= rows ? 0.0f : a.read_scale * __builtin_amdgcn_exp2f((BACK ? rows - 1 - step : step + 1) * l2);
             }
-            const int step = 16 * t + i;
-            const uint32_t upto = (2u << step) - 1u;
-            cuts[t] = BACK ? st & ~upto : st & upto;
-            into[t] = cuts[t] || step >= rows ? 0.0f : a.read_scale * __builtin_amdgcn_exp2f((BACK ? rows - 1 - step : step + 1) * l2);
         }
         through = st ? 0.0f : through * pass;
 
@@ -335,10 +344,10 @@ __global__ void __launch_bounds__(64, (NK * NV >= 24 ? 1 : 2)) chunk_kernel(Chun
                     if (BACK ? t <= ky : t >= ky) {        // (else no pair of these tiles is in order)
 #pragma unroll
                         for (int c = 0; c < NK; c += 2) z = L::mma(k[c], k[c + 1], q[t][c], q[t][c + 1], z);
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) z[r] *= near[BACK ? ky - t : t - ky][r];
+                        z *= near_of[BACK ? ky - t : t - ky][lane];
                         if (st) {
-                            const int lo = !BACK && cuts[t] ? 31 - __clz(cuts[t]) : 0, hi = BACK && cuts[t] ? __ffs(cuts[t]) - 1 : CH;
+                            const uint32_t upto = (2u << (16 * t + i)) - 1u, cuts = BACK ? st & ~upto : st & upto;
+                            const int lo = !BACK && cuts ? 31 - __clz(cuts) : 0, hi = BACK && cuts ? __ffs(cuts) - 1 : CH;
 #pragma unroll
                             for (int r = 0; r < 4; ++r) {
                                 const int y = 16 * ky + 4 * g + r;
@@ -375,11 +384,6 @@ __global__ void __launch_bounds__(64, (NK * NV >= 24 ? 1 : 2)) chunk_kernel(Chun
                     const Quad s0 = L::round(S[c][m]), s1 = L::round(S[c + 1][m]);
 #pragma unroll
                     for (int t = 0; t < TS; ++t) o[t] = L::mma(s0, s1, q[t][c], q[t][c + 1], o[t]);
-                    if (L::SPLIT) {
-                        const Quad r0 = L::round(S[c][m] - L::wide(s0)), r1 = L::round(S[c + 1][m] - L::wide(s1));
-#pragma unroll
-                        for (int t = 0; t < TS; ++t) o[t] = L::mma(r0, r1, q[t][c], q[t][c + 1], o[t]);
-                    }
                 }
 #pragma unroll
                 for (int t = 0; t < TS; ++t) {
@@ -408,9 +412,7 @@ __global__ void __launch_bounds__(64, (NK * NV >= 24 ? 1 : 2)) chunk_kernel(Chun
             Quad y[TS];
 #pragma unroll
             for (int t = 0; t < TS; ++t) {
-                rest[t] = L::wide(v[t]);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) rest[t][r] *= w[t][r];
+                rest[t] = L::wide(v[t]) * w[t];
                 y[t] = L::round(rest[t]);
             }
 #pragma unroll
@@ -418,6 +420,7 @@ __global__ void __launch_bounds__(64, (NK * NV >= 24 ? 1 : 2)) chunk_kernel(Chun
             if (L::SPLIT) {
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
+                    if (e == 1 && !a.exact_state) break;
 #pragma unroll
                     for (int t = 0; t < TS; ++t) {
                         rest[t] -= L::wide(y[t]);
@@ -603,7 +606,7 @@ static WalkWork walk_work(const WalkPlan& p, int64_t pairs, void* at) {
 }
 
 template <typename T, bool BACK>
-int walk(const FishingDecayAttention* f, Strided q, Strided k, Strided v, const float* state, float* state_out, Strided out, int dk, int dv, bool state_t,
+int walk(const FishingDecayAttention* f, Strided q, Strided k, Strided v, const float* state, float* state_out, Strided out, int dk, int dv, bool state_t, bool exact_state,
                 double read_scale, double write_scale, void* workspace, hipStream_t stream) {
     const int64_t pairs = f->batch * f->heads;
     constexpr int V = vec_of<T>();
@@ -613,7 +616,7 @@ int walk(const FishingDecayAttention* f, Strided q, Strided k, Strided v, const 
     const bool vec = wide(q, dk) && wide(k, dk) && wide(v, dv) && wide(out, dv);
     const WalkPlan p = walk_plan(pairs, f->steps, dk, dv, vec);
     const WalkWork w = walk_work(p, pairs, workspace);
-    const ChunkArgs a{q, k, v, out, f->log_decay, f->starts, f->starts_stride[0], f->starts_stride[1], state, state_out, f->steps, f->heads, dk, dv, state_t,
+    const ChunkArgs a{q, k, v, out, f->log_decay, f->starts, f->starts_stride[0], f->starts_stride[1], state, state_out, f->steps, f->heads, dk, dv, state_t, exact_state,
                       (float)read_scale, (float)write_scale, p.slices, p.segs, p.seg_steps, w.carry, w.through, w.odd};
     const dim3 grid((unsigned)(pairs * p.slices * p.segs));
     auto run = [&](auto tk, auto tv, auto rows) {
