@@ -33,6 +33,14 @@ __device__ __forceinline__ float log_decay_of(const float* log_decay, int h) { r
 // A wave alone needs no barriers; the next chunk's rows are loaded into registers while this one is computed.  Bound by HBM: q, k, v
 // read, out written once.
 
+// The value, not to be worked with ahead of this place: what is computed of lane numbers for the rare chunk would otherwise be
+// computed once and kept, some sixty registers of it
+__device__ __forceinline__ int here(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+__device__ __forceinline__ uint32_t here(uint32_t x) { return (uint32_t)here((int)x); }
+
 template <typename T>
 struct Lanes;
 template <>
@@ -120,9 +128,10 @@ struct Lanes<float> {
     static __device__ __forceinline__ f32x4 wide(Quad x) { return x; }
 };
 
-// A chunk's rows of one operand on their way from memory, 16 bytes a lane and load.  Nothing is masked on the way in: columns behind
-// d and rows behind the last read ones that exist, and become zeros on the way to LDS, where a uniform test finds whole chunks.
-// VEC: the address is a uniform one and 32 bits of the lane's own.
+// A chunk's rows of one operand on their way from memory, 16 bytes a lane and load.  Rows behind the last and columns behind d are
+// zeros.  VEC: buffer loads, which answer zeros for what lies behind the buffer: its length ends the rows, and a lane of columns
+// behind d points there.  (Steps of at least d, 32 of them in 31 bits: the plan's business.)  No branch and no mask: with either the
+// compiler could not count the loads and waited for one operand's before it sent the next's.
 template <typename T, int TILES, int STEPS, bool VEC>
 struct Rows {
     static constexpr int EPC = 16 / (int)sizeof(T), CHUNKS = TILES * 16 / EPC, LOADS = STEPS * CHUNKS / 64, PITCH = TILES * 16 * (int)sizeof(T) + 16;
@@ -131,65 +140,43 @@ struct Rows {
     static_assert(STEPS * CHUNKS % 64 == 0, "whole loads");
     u32x4 x[LOADS];
 
-    static __device__ __forceinline__ int row_of(int s) { return EVEN ? threadIdx.x / CHUNKS + s * PER : (s * 64 + threadIdx.x) / CHUNKS; }
-    static __device__ __forceinline__ int chunk_of(int s) { return EVEN ? threadIdx.x % CHUNKS : (s * 64 + threadIdx.x) % CHUNKS; }
-
-    static __device__ __forceinline__ u32x4 at(const T* base, uint32_t bytes) {
-        asm("" : "+v"(bytes));                    // (kept next to the load: hoisted, it becomes a 64-bit pair of registers per load)
-        return *(const u32x4*)((const char*)base + bytes);
+    static __device__ __forceinline__ int row_of(int s) { return EVEN ? (int)threadIdx.x / CHUNKS + s * PER : (s * 64 + (int)threadIdx.x) / CHUNKS; }
+    static __device__ __forceinline__ int chunk_of(int s) { return EVEN ? (int)threadIdx.x % CHUNKS : (s * 64 + (int)threadIdx.x) % CHUNKS; }
+    // a lane's place from a chunk's first row on
+    static __device__ __forceinline__ uint32_t place(int s, int64_t step, int d) {
+        const int c = chunk_of(s) * EPC;
+        return c < d ? ((uint32_t)row_of(s) * (uint32_t)step + c) * (uint32_t)sizeof(T) : 0x80000000u;
+    }
+    uint32_t at[EVEN ? 1 : LOADS];
+    __device__ __forceinline__ void init(int64_t step, int d) {
+        if constexpr (VEC) {
+#pragma unroll
+            for (int s = 0; s < (EVEN ? 1 : LOADS); ++s) at[s] = place(s, step, d);
+        }
     }
     // p: the chunk's first row (uniform)
     __device__ __forceinline__ void load(const T* p, int64_t step, int rows, int d) {
-        if constexpr (!VEC) {
+        if constexpr (VEC) {
+            const auto buffer = __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, (uint32_t)((uint32_t)(rows - 1) * (uint32_t)step + d) * (uint32_t)sizeof(T), 0x00020000);
+            const uint32_t next = (uint32_t)(PER * (int)sizeof(T)) * (uint32_t)step;
+#pragma unroll
+            for (int s = 0; s < LOADS; ++s) x[s] = __builtin_amdgcn_raw_buffer_load_b128(buffer, EVEN ? at[0] + s * next : at[EVEN ? 0 : s], 0, 0);
+        } else {
 #pragma unroll
             for (int s = 0; s < LOADS; ++s) {
                 const int r = row_of(s), c = chunk_of(s) * EPC;
                 const T* from = p + (r < rows ? r : rows - 1) * step;
                 Pack<T, EPC> y;
 #pragma unroll
-                for (int e = 0; e < EPC; ++e) y.e[e] = from[c + e < d ? c + e : 0];
+                for (int e = 0; e < EPC; ++e) y.e[e] = r < rows && c + e < d ? from[c + e] : from_f32<T>(0.0f);
                 x[s] = *(const u32x4*)&y;
-            }
-        } else if (EVEN && rows == STEPS) {
-            const int c = chunk_of(0) * EPC;
-            uint32_t mine = ((uint32_t)row_of(0) * (uint32_t)step + (c < d ? c : 0)) * (uint32_t)sizeof(T);
-            const uint32_t next = (uint32_t)(PER * (int)sizeof(T)) * (uint32_t)step;
-#pragma unroll
-            for (int s = 0; s < LOADS; ++s) {
-                x[s] = at(p, mine);
-                mine += next;
-            }
-        } else {
-#pragma unroll
-            for (int s = 0; s < LOADS; ++s) {
-                const int r = row_of(s), c = chunk_of(s) * EPC;
-                x[s] = at(p, ((uint32_t)(r < rows ? r : rows - 1) * (uint32_t)step + (c < d ? c : 0)) * (uint32_t)sizeof(T));
             }
         }
     }
-    __device__ __forceinline__ void put(char* lds, int rows, int d) {
-        if (rows != STEPS || d < TILES * 16) {
-#pragma unroll
-            for (int s = 0; s < LOADS; ++s) {
-                const int r = row_of(s), c = chunk_of(s) * EPC;
-                if constexpr (VEC) {
-                    if (r >= rows || c >= d) x[s] = u32x4{0, 0, 0, 0};
-                } else {
-                    Pack<T, EPC> y = *(const Pack<T, EPC>*)&x[s];
-#pragma unroll
-                    for (int e = 0; e < EPC; ++e) y.e[e] = r < rows && c + e < d ? y.e[e] : from_f32<T>(0.0f);
-                    x[s] = *(const u32x4*)&y;
-                }
-            }
-        }
+    __device__ __forceinline__ void put(char* lds) const {
         char* to = lds + threadIdx.x / CHUNKS * PITCH + threadIdx.x % CHUNKS * 16;
 #pragma unroll
-        for (int s = 0; s < LOADS; ++s) {
-            if (EVEN)
-                *(u32x4*)(to + s * PER * PITCH) = x[s];
-            else
-                *(u32x4*)(lds + row_of(s) * PITCH + chunk_of(s) * 16) = x[s];
-        }
+        for (int s = 0; s < LOADS; ++s) *(u32x4*)(EVEN ? to + s * PER * PITCH : lds + row_of(s) * PITCH + chunk_of(s) * 16) = x[s];
     }
 };
 
@@ -209,6 +196,24 @@ struct ChunkArgs {
     float *carry, *through;    // per (pair, slice, segment): the state behind it in lane order, and what it lets through
     uint32_t* odd;             // per (pair, slice, segment): some result is infinite or NaN
 };
+
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+template <typename R>
+__device__ __forceinline__ void store_quad(R rows, uint32_t at, int further, Lanes<bf16>::Quad x) {
+    union {
+        Lanes<bf16>::Quad q;
+        u32x2 u;
+    } y{x};
+    __builtin_amdgcn_raw_buffer_store_b64(y.u, rows, at, further, 0);
+}
+template <typename R>
+__device__ __forceinline__ void store_quad(R rows, uint32_t at, int further, f32x4 x) {
+    union {
+        f32x4 q;
+        u32x4 u;
+    } y{x};
+    __builtin_amdgcn_raw_buffer_store_b128(y.u, rows, at, further, 0);
+}
 
 // LOCAL: only the state that a segment adds (from zero; the first from the state carried in), for the segments to be chained.
 template <typename T, int NK, int NV, bool BACK, bool VEC, bool LOCAL>
@@ -279,6 +284,10 @@ __global__ void __launch_bounds__(64, (NK * NV >= 24 ? 1 : 2)) chunk_kernel(Chun
 
     RK rq, rk;
     RV rv;
+    rq.init(a.q.step, a.dk);
+    rk.init(a.k.step, a.dk);
+    rv.init(a.v.step, cols);
+    const uint32_t starts_at = (uint32_t)lane * (uint32_t)a.starts_step;
     uint32_t started = 0;                         // the lane's step begins an episode (tested behind the wait for the rows)
     auto front = [&](int x) { return t_lo + (int64_t)(BACK ? chunks - 1 - x : x) * CH; };
     auto count = [&](int64_t t0) { return t_hi - t0 < CH ? (int)(t_hi - t0) : CH; };
@@ -288,7 +297,14 @@ __global__ void __launch_bounds__(64, (NK * NV >= 24 ? 1 : 2)) chunk_kernel(Chun
         if (!LOCAL) rq.load(qp + t0 * a.q.step, a.q.step, rows, a.dk);
         rk.load(kp + t0 * a.k.step, a.k.step, rows, a.dk);
         rv.load(vp + t0 * a.v.step, a.v.step, rows, cols);
-        if (a.starts) started = a.starts[n * a.starts_batch + (t0 + (lane < rows ? lane : 0)) * a.starts_step];
+        if (a.starts) {
+            const uint8_t* from = a.starts + n * a.starts_batch + t0 * a.starts_step;
+            if constexpr (VEC)
+                started = __builtin_amdgcn_raw_buffer_load_b8(__builtin_amdgcn_make_buffer_rsrc((void*)from, 0, (uint32_t)(rows - 1) * (uint32_t)a.starts_step + 1, 0x00020000),
+                                                              starts_at, 0, 0);
+            else
+                started = from[(lane < rows ? lane : 0) * a.starts_step];
+        }
     };
     float odd = 0.0f, through = 1.0f;
     if (chunks > 0) fetch(0);
@@ -296,9 +312,9 @@ __global__ void __launch_bounds__(64, (NK * NV >= 24 ? 1 : 2)) chunk_kernel(Chun
         const int64_t t0 = front(x);
         const int rows = count(t0);
         __syncthreads();
-        if (!LOCAL) rq.put(qs, rows, a.dk);
-        rk.put(ks, rows, a.dk);
-        rv.put(vs, rows, cols);
+        if (!LOCAL) rq.put(qs);
+        rk.put(ks);
+        rv.put(vs);
         const uint32_t st = (uint32_t)__ballot(started != 0 && lane < rows);
         __syncthreads();
         f32x4 w[TS];
@@ -309,16 +325,17 @@ __global__ void __launch_bounds__(64, (NK * NV >= 24 ? 1 : 2)) chunk_kernel(Chun
             into[t] = ahead_of[t][lane];
         }
         if (st || rows != CH) {                   // uniform: few chunks
+            const int g4 = here(4 * g), i0 = here(i);
             pass = st ? 0.0f : exp2f(rows * l2);
             const int from = !BACK && st ? 31 - __clz(st) : 0, to = BACK && st ? __ffs(st) - 1 : rows;
 #pragma unroll
             for (int t = 0; t < TS; ++t) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const int y = 16 * t + 4 * g + r;
+                    const int y = 16 * t + g4 + r;
                     w[t][r] = y >= from && y < to ? a.write_scale * __builtin_amdgcn_exp2f((BACK ? y + 1 : rows - 1 - y) * l2) : 0.0f;
                 }
-                const int step = 16 * t + i;
+                const int step = 16 * t + i0;
                 const uint32_t upto = (2u << step) - 1u, cuts = BACK ? st & ~upto : st & upto;
                 into[t] = cuts || step >= rows ? 0.0f : a.read_scale * __builtin_amdgcn_exp2f((BACK ? rows - 1 - step : step + 1) * l2);
             }
@@ -326,6 +343,7 @@ __global__ void __launch_bounds__(64, (NK * NV >= 24 ? 1 : 2)) chunk_kernel(Chun
         through = st ? 0.0f : through * pass;
 
         T* o_front = op + t0 * a.out.step;
+        const auto o_rows = __builtin_amdgcn_make_buffer_rsrc(o_front, 0, 0x7fffffff, 0x00020000);
         Quad q[TS][NK], p[TS][TS], p_rest[TS][TS];     // [step tile][...]; scores: four y in registers, x in lanes
         if (!LOCAL) {
 #pragma unroll
@@ -346,11 +364,12 @@ __global__ void __launch_bounds__(64, (NK * NV >= 24 ? 1 : 2)) chunk_kernel(Chun
                         for (int c = 0; c < NK; c += 2) z = L::mma(k[c], k[c + 1], q[t][c], q[t][c + 1], z);
                         z *= near_of[BACK ? ky - t : t - ky][lane];
                         if (st) {
-                            const uint32_t upto = (2u << (16 * t + i)) - 1u, cuts = BACK ? st & ~upto : st & upto;
+                            const int g4 = here(4 * g);
+                            const uint32_t upto = (2u << here(16 * t + i)) - 1u, cuts = BACK ? st & ~upto : st & upto;
                             const int lo = !BACK && cuts ? 31 - __clz(cuts) : 0, hi = BACK && cuts ? __ffs(cuts) - 1 : CH;
 #pragma unroll
                             for (int r = 0; r < 4; ++r) {
-                                const int y = 16 * ky + 4 * g + r;
+                                const int y = 16 * ky + g4 + r;
                                 z[r] = y >= lo && y < hi ? z[r] : 0.0f;
                             }
                         }
@@ -362,6 +381,12 @@ __global__ void __launch_bounds__(64, (NK * NV >= 24 ? 1 : 2)) chunk_kernel(Chun
         }
 
         __builtin_amdgcn_sched_barrier(0);
+        uint32_t o_at[TS];                        // a lane's place in the output's rows; behind everything for steps that are not
+#pragma unroll
+        for (int t = 0; t < TS; ++t) {
+            const int step = here(16 * t + i);
+            o_at[t] = step < rows ? ((uint32_t)step * (uint32_t)a.out.step + 4 * g) * (uint32_t)sizeof(T) : 0xffffffffu;
+        }
         Quad kc[NK][TS];
 #pragma unroll
         for (int t = 0; t < TS; ++t)
@@ -383,27 +408,25 @@ __global__ void __launch_bounds__(64, (NK * NV >= 24 ? 1 : 2)) chunk_kernel(Chun
                 for (int c = 0; c < NK; c += 2) {
                     const Quad s0 = L::round(S[c][m]), s1 = L::round(S[c + 1][m]);
 #pragma unroll
-                    for (int t = 0; t < TS; ++t) o[t] = L::mma(s0, s1, q[t][c], q[t][c + 1], o[t]);
+                    for (int t = 0; t < TS; ++t)
+                        o[t] = L::mma(s0, s1, q[t][c], q[t][c + 1], o[t]);
                 }
 #pragma unroll
                 for (int t = 0; t < TS; ++t) {
-                    if (t > 0 && rows <= 16 * t) continue;             // (uniform: the last chunk of an episode batch is often short)
                     o[t] = L::over_steps(v, p[t], o[t] * into[t]);
                     if (L::SPLIT) o[t] = L::over_steps(v, p_rest[t], o[t]);
                     const int step = 16 * t + i, col = m * 16 + 4 * g;
-                    if (step < rows) {
-                        uint32_t mine = ((uint32_t)step * (uint32_t)a.out.step + 4 * g) * (uint32_t)sizeof(T);
-                        asm("" : "+v"(mine));
-                        T* to = (VEC ? (T*)((char*)o_front + mine) : o_front + step * a.out.step + 4 * g) + m * 16;
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) odd += o[t][r] * 0.0f;         // NaN from anything that is not a finite number
-                        if (VEC) {
-                            if (col < cols) *(Quad*)to = L::round(o[t]);
-                        } else {
+                    for (int r = 0; r < 4; ++r) odd += o[t][r] * 0.0f;       // NaN from anything that is not a finite number
+                    if constexpr (VEC) {
+                        // a buffer store, which drops a lane whose offset is behind the buffer: behind a branch the stores could not be
+                        // counted, and the wait for the next chunk's rows would be one for these as well
+                        store_quad(o_rows, here(col) < cols ? o_at[t] : 0xffffffffu, m * 16 * (int)sizeof(T), L::round(o[t]));
+                    } else if (step < rows) {
+                        T* to = o_front + step * a.out.step + col;
 #pragma unroll
-                            for (int r = 0; r < 4; ++r)
-                                if (col + r < cols) to[r] = from_f32<T>(o[t][r]);
-                        }
+                        for (int r = 0; r < 4; ++r)
+                            if (col + r < cols) to[r] = from_f32<T>(o[t][r]);
                     }
                 }
             }
@@ -609,11 +632,12 @@ template <typename T, bool BACK>
 int walk(const FishingDecayAttention* f, Strided q, Strided k, Strided v, const float* state, float* state_out, Strided out, int dk, int dv, bool state_t, bool exact_state,
                 double read_scale, double write_scale, void* workspace, hipStream_t stream) {
     const int64_t pairs = f->batch * f->heads;
+    if (f->steps <= 1) q.step = k.step = v.step = out.step = kMaxHeadDim;         // (a single step has no next one: any stride will do)
     constexpr int V = vec_of<T>();
     auto wide = [&](const Strided& s, int d) {
-        return d % V == 0 && aligned16(s.p) && s.batch % V == 0 && s.step % V == 0 && s.head % V == 0 && s.step < (int64_t)1 << 24;      // 32 rows in 32 bits
+        return d % V == 0 && aligned16(s.p) && s.batch % V == 0 && s.step % V == 0 && s.head % V == 0 && s.step >= d && s.step < (int64_t)1 << 24;
     };
-    const bool vec = wide(q, dk) && wide(k, dk) && wide(v, dv) && wide(out, dv);
+    const bool vec = wide(q, dk) && wide(k, dk) && wide(v, dv) && wide(out, dv) && f->starts_stride[1] < (int64_t)1 << 24;
     const WalkPlan p = walk_plan(pairs, f->steps, dk, dv, vec);
     const WalkWork w = walk_work(p, pairs, workspace);
     const ChunkArgs a{q, k, v, out, f->log_decay, f->starts, f->starts_stride[0], f->starts_stride[1], state, state_out, f->steps, f->heads, dk, dv, state_t, exact_state,
