@@ -20,6 +20,7 @@ import sys
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG, "csrc")
+CSRC_SEQUENCE = os.path.join(PKG, "csrc_sequence")       # the sequence operators: float32 sums, none of csrc's NumPy rounding rules
 LIB_DIR = os.path.join(PKG, "_lib")
 LIB_PATH = os.path.join(LIB_DIR, "libfishing_hip.so")
 # Per-kernel register / LDS table of the library that was built (hipcc's own remarks, written next to the .so).  bench.py
@@ -50,11 +51,11 @@ TU_FLAGS = {"fishing_step.hip": ["-fno-slp-vectorize", "-mllvm", "-amdgpu-kernar
 
 
 def sources():
-    return sorted(glob.glob(os.path.join(CSRC, "*.hip")))
+    return [f for d in (CSRC, CSRC_SEQUENCE) for f in sorted(glob.glob(os.path.join(d, "*.hip")))]
 
 
 def _deps():
-    return sources() + sorted(glob.glob(os.path.join(CSRC, "*.h"))) + [
+    return sources() + [f for d in (CSRC, CSRC_SEQUENCE) for f in sorted(glob.glob(os.path.join(d, "*.h")))] + [
         os.path.join(os.path.dirname(PKG), "include", "fishing_hip.h")]
 
 
@@ -71,7 +72,7 @@ def hipcc_path():
 
 
 def build(force=False, verbose=False, extra_flags=(), out=None):
-    """Compile every csrc/*.hip into one shared library.  Returns its path.
+    """Compile every csrc/*.hip and csrc_sequence/*.hip into one shared library.  Returns its path.
     `out` + `extra_flags` build an experimental variant next to the default library
     (scripts/build_variants.py: today the host-side UBSan build; the product always loads LIB_PATH)."""
     if out is not None:

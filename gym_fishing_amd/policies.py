@@ -1,7 +1,8 @@
 """The reference's non-learned policies (gym_fishing/models/policies.py:4-67) on top of the
-HIP env: MSY constant quota, constant escapement, and the BMSY growth-curve sweep.
+HIP env: MSY constant quota, constant escapement, and the BMSY growth-curve sweep; and `memory`
+(memory_policy.py), a trainable one that remembers its episode.
 
-All three return `(action, obs)` from `predict(obs)` SB3-style, work with the scalar
+The reference's three return `(action, obs)` from `predict(obs)` SB3-style, work with the scalar
 protocol and with N-env tensors, and carry `kernel_policy = (policy_id, param)` so that
 `env.simulate(model)` / `env.rollout(policy=...)` can run them inside the fused rollout
 kernel (csrc/fishing_rollout.hip) instead of calling predict() per step.
@@ -10,6 +11,7 @@ import numpy as np
 import torch
 
 from ._capi import POLICY_ESCAPEMENT, POLICY_MSY
+from .memory_policy import memory  # noqa: F401
 from .spaces import is_discrete
 
 

@@ -6,7 +6,8 @@ producing the same `[time, state, action, reward, rep]` table.
 * N-env tensor protocol: every env is one rep; a model that carries `kernel_policy`
   (policies.msy / policies.escapement, or the strings "random" / ("constant", a)) runs inside
   the fused rollout kernel and the table is cut from its `[T][4][N]` record; any other model
-  is driven step by step with batched predict().
+  is driven step by step with batched predict(); one with `recurrent = True` (policies.memory) is handed the
+  state its last step returned and the done flags (simulate_mdp_vec does so for any model, as the reference's does).
 * simulate_mdp_vec: the reference's own N-env helper (shared_env.py:57-79), row for row: Tmax + 1 rows per env
   and batch, time-major, no break on done (the batch auto-resets like SB3's VecEnv), the RAW ACTION of the
   previous step in the action column (pinned by tests/golden/reference_vec_sims.npz).
@@ -39,6 +40,13 @@ def _kernel_policy(model):
     return getattr(model, "kernel_policy", None)
 
 
+def _predict(model, obs, state, mask):
+    """One predict() of the simulate helpers: models that remember get their state back, the others the observation alone."""
+    if getattr(model, "recurrent", False):
+        return model.predict(obs, state=state, mask=mask)
+    return model.predict(obs)[0], None
+
+
 class _StringPolicy:
     """predict() for the policy strings the fused kernel understands, for the step-by-step path: a constant action, or
     uniform random actions from torch's generator (NOT the in-kernel Philox policy stream)."""
@@ -65,10 +73,10 @@ def simulate_mdp(env, model, reps=1):
     rows = []
     for rep in range(reps):
         obs = env.reset()
-        quota, reward = 0.0, 0.0
+        quota, reward, state = 0.0, 0.0, None
         for t in range(env.Tmax):
             rows.append([t, env.get_fish_population(obs), quota, reward, int(rep)])
-            action, _ = model.predict(obs)
+            action, state = _predict(model, obs, state, None)
             obs, reward, done, _ = env.step(action)
             if isinstance(action, np.ndarray):
                 action = action.reshape(-1)[0]
@@ -190,10 +198,10 @@ def _simulate_mdp_batched(env, model, n_eval_episodes):
                 traj = env.rollout(env.Tmax, policy=kp[0], param=kp[1], record=True)
             else:
                 traj = torch.zeros((env.Tmax, 4, env.num_envs), dtype=env.dtype, device=env.device)
-                obs = env.state
+                obs, state = env.state, None
                 for t in range(env.Tmax):
                     traj[t, 0] = obs.reshape(-1)
-                    action, _ = model.predict(obs)
+                    action, state = _predict(model, obs, state, None)
                     a = torch.as_tensor(action, device=env.device).reshape(-1)
                     traj[t, 1] = a.to(env.dtype)
                     obs, rew, done, _ = env.step(a)
