@@ -43,14 +43,18 @@ static inline int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b
 
 // This launch's own status, as hipLaunchKernel returns it
 template <typename... P, typename... A>
-inline int launch(void (*kernel)(P...), dim3 grid, dim3 block, hipStream_t stream, A&&... args) {
+inline int launch_lds(void (*kernel)(P...), dim3 grid, dim3 block, size_t lds, hipStream_t stream, A&&... args) {
     std::tuple<P...> packed{static_cast<P>(args)...};
     return std::apply(
         [&](auto&... a) {
             void* argv[] = {(void*)&a...};
-            return (int)hipLaunchKernel((const void*)kernel, grid, block, argv, 0, stream);
+            return (int)hipLaunchKernel((const void*)kernel, grid, block, argv, lds, stream);
         },
         packed);
+}
+template <typename... P, typename... A>
+inline int launch(void (*kernel)(P...), dim3 grid, dim3 block, hipStream_t stream, A&&... args) {
+    return launch_lds(kernel, grid, block, 0, stream, args...);
 }
 
 // Workspace carving: 256-byte aligned blocks in the caller's buffer

@@ -58,26 +58,25 @@ __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(const I* token
     for (int d = threadIdx.x; d < digits; d += kSortThreads) count[(int64_t)d * gridDim.x + blockIdx.x] = bin[d];
 }
 
-// exclusive sum over count[digits * blocks], one workgroup
-__global__ void __launch_bounds__(1024) sort_scan_kernel(uint32_t* count, int32_t n) {
-    __shared__ uint32_t sum[1024];
-    const int per = (n + 1023) / 1024, lo = threadIdx.x * per, hi = lo + per < n ? lo + per : n;
-    uint32_t s = 0;
-    for (int i = lo; i < hi; ++i) s += count[i];
-    sum[threadIdx.x] = s;
+constexpr int kMaxBlocks = 512;
+
+// a workgroup per digit: its blocks' counts become exclusive sums, count[digits * blocks + digit] their total
+__global__ void __launch_bounds__(kMaxBlocks) sort_scan_kernel(uint32_t* count, int32_t blocks, int32_t digits) {
+    __shared__ uint32_t sum[kMaxBlocks / 64];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    uint32_t* c = count + (int64_t)blockIdx.x * blocks;
+    const uint32_t mine = threadIdx.x < (uint32_t)blocks ? c[threadIdx.x] : 0;
+    uint32_t s = mine;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint32_t x = __shfl_up(s, d);
+        if (lane >= d) s += x;
+    }
+    if (lane == 63) sum[wave] = s;
     __syncthreads();
-    for (int d = 1; d < 1024; d <<= 1) {
-        const uint32_t x = threadIdx.x >= d ? sum[threadIdx.x - d] : 0;
-        __syncthreads();
-        sum[threadIdx.x] += x;
-        __syncthreads();
-    }
-    uint32_t run = sum[threadIdx.x] - s;
-    for (int i = lo; i < hi; ++i) {
-        const uint32_t x = count[i];
-        count[i] = run;
-        run += x;
-    }
+    for (int w = 0; w < wave; ++w) s += sum[w];
+    if (threadIdx.x < (uint32_t)blocks) c[threadIdx.x] = s - mine;
+    if (threadIdx.x == kMaxBlocks - 1) count[(int64_t)digits * blocks + blockIdx.x] = s;
 }
 
 template <typename I, bool FIRST>
@@ -86,7 +85,25 @@ __global__ void __launch_bounds__(kSortThreads) sort_place_kernel(const I* token
     __shared__ uint32_t base[kMaxDigits];
     __shared__ uint32_t in_wave[kSortWaves][kMaxDigits];
     const int digits = 1 << bits, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    for (int d = threadIdx.x; d < digits; d += kSortThreads) base[d] = count[(int64_t)d * gridDim.x + blockIdx.x];
+    // where this block's share of each digit begins: the digits before it, and the blocks before this one
+    if (threadIdx.x < kMaxDigits) {
+        const uint32_t total = threadIdx.x < (uint32_t)digits ? count[(int64_t)digits * gridDim.x + threadIdx.x] : 0;
+        uint32_t s = total;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const uint32_t x = __shfl_up(s, d);
+            if (lane >= d) s += x;
+        }
+        if (lane == 63) in_wave[0][wave] = s;
+        base[threadIdx.x] = s - total;
+    }
+    __syncthreads();
+    if (threadIdx.x < (uint32_t)digits) {
+        uint32_t s = base[threadIdx.x] + count[(int64_t)threadIdx.x * gridDim.x + blockIdx.x];
+        for (int w = 0; w < wave; ++w) s += in_wave[0][w];
+        base[threadIdx.x] = s;
+    }
+    __syncthreads();
     const int64_t lo = (int64_t)blockIdx.x * tile, hi = lo + tile < n ? lo + tile : n;
     for (int64_t i0 = lo; i0 < hi; i0 += kSortThreads) {
         for (int d = threadIdx.x; d < kSortWaves * digits; d += kSortThreads) in_wave[d >> bits][d & (digits - 1)] = 0;
@@ -136,7 +153,7 @@ __device__ __forceinline__ void mark_starts(uint32_t* start, int64_t from, int64
 template <typename T, int V, int G>
 __global__ void __launch_bounds__(256) embedding_sum_kernel(const T* dout, int64_t dout_stride, const uint32_t* key, const uint32_t* row, int64_t n, int64_t vocab,
                                                             int32_t dim, int32_t chunk, float scale, T* dtable, float* partial, uint32_t* start) {
-    constexpr int U = 8;
+    constexpr int U = 16;
     const int lane = threadIdx.x % G;
     const int64_t c = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
     const int64_t p0 = c * chunk, p1 = p0 + chunk < n ? p0 + chunk : n;
@@ -168,24 +185,34 @@ __global__ void __launch_bounds__(256) embedding_sum_kernel(const T* dout, int64
         for (int e = 0; e < V; ++e) acc[e] = 0.0f;
         first = false;
     };
-    for (int64_t p = p0; p < p1; p += U) {
-        uint32_t k[U];
-        Pack<T, V> x[U];
+    uint32_t k[U], from[U];
+    auto index = [&](int64_t p) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int64_t at = p + u < p1 ? p + u : p1 - 1;
             k[u] = key[at];
-            if (mine && k[u] < vocab) x[u] = *(const Pack<T, V>*)(dout + (int64_t)row[at] * dout_stride + col);
+            from[u] = row[at];
         }
+    };
+    index(p0);
+    for (int64_t p = p0; p < p1; p += U) {
+        uint32_t now[U];
+        Pack<T, V> x[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            now[u] = k[u];
+            if (mine && now[u] < vocab) x[u] = *(const Pack<T, V>*)(dout + (int64_t)from[u] * dout_stride + col);
+        }
+        if (p + U < p1) index(p + U);              // (the next rows' places arrive with this batch's rows)
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             if (p + u < p1) {
-                if ((int64_t)k[u] != cur) {
+                if ((int64_t)now[u] != cur) {
                     flush(false);
-                    if (marks) mark_starts<G>(start, cur + 1, k[u], (uint32_t)(p + u), lane);
-                    cur = k[u];
+                    if (marks) mark_starts<G>(start, cur + 1, now[u], (uint32_t)(p + u), lane);
+                    cur = now[u];
                 }
-                if (mine && k[u] < vocab) {
+                if (mine && now[u] < vocab) {
 #pragma unroll
                     for (int e = 0; e < V; ++e) acc[e] += to_f32(x[u].e[e]);
                 }
@@ -215,6 +242,53 @@ __global__ void __launch_bounds__(256) embedding_join_kernel(const uint32_t* sta
     }
 }
 
+// ---- small tables (a few hundred tokens: the quota levels) need no sort: a workgroup keeps the sums of its share of the rows for 64 of
+// the columns in LDS, one lane a column, so that a column's additions keep their order without a word between lanes.  A workgroup is one wave.  ----
+constexpr int kTableRows = 16, kSmallTable = 256;
+
+template <typename T, typename I>
+__global__ void __launch_bounds__(64) embedding_table_kernel(const T* dout, int64_t dout_stride, const I* token, int64_t n, int32_t vocab, int32_t dim, int64_t share,
+                                                             float* partial) {
+    extern __shared__ float sums[];                        // [vocab][64]
+    const int lane = threadIdx.x, col = blockIdx.y * 64 + lane;
+    for (int v = 0; v < vocab; ++v) sums[v * 64 + lane] = 0.0f;
+    const int64_t lo = blockIdx.x * share, hi = lo + share < n ? lo + share : n;
+    const T* from = dout + (col < dim ? col : 0);
+    for (int64_t i = lo; i < hi; i += kTableRows) {
+        T x[kTableRows];
+        int at[kTableRows];
+#pragma unroll
+        for (int u = 0; u < kTableRows; ++u) {
+            const int64_t r = i + u < hi ? i + u : hi - 1;
+            const int64_t t = (int64_t)token[r];
+            at[u] = i + u < hi && t >= 0 && t < vocab ? (int)t : -1;
+            x[u] = from[r * dout_stride];
+        }
+#pragma unroll
+        for (int u = 0; u < kTableRows; ++u)
+            if (at[u] >= 0) sums[at[u] * 64 + lane] += to_f32(x[u]);
+    }
+    if (col >= dim) return;
+    float* to = partial + (int64_t)blockIdx.x * vocab * dim + col;
+    for (int v = 0; v < vocab; ++v) to[(int64_t)v * dim] = sums[v * 64 + lane];
+}
+
+// the shares' tables added in order; L lanes take every L-th
+template <typename T>
+__global__ void __launch_bounds__(256) embedding_table_join_kernel(const float* partial, int shares, int64_t size, float scale, T* dtable) {
+    __shared__ float part[4][64];
+    const int c = threadIdx.x & 63, l = threadIdx.x >> 6;
+    const int64_t at = (int64_t)blockIdx.x * 64 + c;
+    float s = 0.0f;
+    if (at < size) {
+#pragma unroll 8
+        for (int x = l; x < shares; x += 4) s += partial[x * size + at];
+    }
+    part[l][c] = s;
+    __syncthreads();
+    if (l == 0 && at < size) dtable[at] = from_f32<T>((part[0][c] + part[1][c] + part[2][c] + part[3][c]) * scale);
+}
+
 struct SortPlan {
     int bits, passes, digit_bits;
     int64_t tile;
@@ -229,9 +303,9 @@ static SortPlan sort_plan(int64_t n, int64_t vocab) {
     while (((int64_t)1 << s.bits) <= vocab) ++s.bits;         // keys 0 .. vocab
     s.passes = (s.bits + 7) / 8;
     s.digit_bits = (s.bits + s.passes - 1) / s.passes;
-    s.tile = round_up(ceil_div(n > 0 ? n : 1, 512), 2 * kSortThreads);
+    s.tile = round_up(ceil_div(n > 0 ? n : 1, kMaxBlocks), 2 * kSortThreads);
     s.blocks = (int)ceil_div(n > 0 ? n : 1, s.tile);
-    s.chunk = n >= (1 << 19) ? 256 : n >= (1 << 16) ? 64 : 16;
+    s.chunk = n >= (1 << 20) ? 128 : n >= (1 << 18) ? 64 : n >= (1 << 16) ? 32 : 16;
     s.chunks = ceil_div(n, s.chunk);
     return s;
 }
@@ -249,7 +323,7 @@ static EmbeddingWork embedding_work(const SortPlan& s, int64_t n, int64_t vocab,
         w.key[k] = c.take<uint32_t>(n);
         w.row[k] = c.take<uint32_t>(n);
     }
-    w.count = c.take<uint32_t>((int64_t)s.blocks << s.digit_bits);
+    w.count = c.take<uint32_t>((int64_t)(s.blocks + 1) << s.digit_bits);
     w.start = c.take<uint32_t>(vocab + 1);
     w.partial = c.take<float>(2 * s.chunks * dim);
     w.bytes = c.used;
@@ -274,12 +348,31 @@ static int embedding_forward(int64_t n, int64_t vocab, int64_t dim, const T* tab
     return go(embedding_kernel<T, I, 1>, (int)dim);
 }
 
+// How a small table's rows are shared out: so many waves that a share's table (written and read once) stays small beside its rows
+static int64_t table_shares(int64_t n, int64_t vocab, int64_t dim) {
+    const int64_t slices = ceil_div(dim, 64), fit = 160 * 1024 / (vocab * 256);               // tables of a CU's LDS
+    int64_t shares = 256 * (fit < 16 ? fit : 16) / slices;
+    const int64_t most = n / (2 * vocab);
+    if (shares > most) shares = most;
+    return shares > 0 ? shares : 1;
+}
+
+static bool table_fits(int64_t n, int64_t vocab) { return vocab <= kSmallTable && n >= 16 * vocab; }
+
 template <typename T, typename I>
 static int embedding_backward(int64_t n, int64_t vocab, int64_t dim, const T* dout, int64_t dout_stride, const I* token, float scale, T* dtable, void* workspace,
                               hipStream_t stream) {
+    int rc = 0;
+    if (table_fits(n, vocab)) {
+        const int64_t shares = table_shares(n, vocab, dim), share = ceil_div(n, shares);
+        const dim3 grid((unsigned)ceil_div(n, share), (unsigned)ceil_div(dim, 64));
+        float* partial = (float*)workspace;
+        rc = launch_lds(embedding_table_kernel<T, I>, grid, dim3(64), (size_t)vocab * 256, stream, dout, dout_stride, token, n, (int32_t)vocab, (int32_t)dim, share, partial);
+        if (rc) return rc;
+        return launch(embedding_table_join_kernel<T>, dim3((unsigned)ceil_div(vocab * dim, 64)), dim3(256), stream, partial, (int)grid.x, vocab * dim, scale, dtable);
+    }
     const SortPlan s = sort_plan(n, vocab);
     const EmbeddingWork w = embedding_work(s, n, vocab, dim, workspace);
-    int rc = 0;
     if (n > 0) {
         for (int p = 0; p < s.passes && !rc; ++p) {
             const int shift = p * s.digit_bits, digits = 1 << s.digit_bits;
@@ -287,7 +380,7 @@ static int embedding_backward(int64_t n, int64_t vocab, int64_t dim, const T* do
             const dim3 grid(s.blocks), block(kSortThreads);
             rc = p == 0 ? launch(sort_count_kernel<I, true>, grid, block, stream, token, key, n, vocab, s.tile, shift, digits, w.count)
                         : launch(sort_count_kernel<I, false>, grid, block, stream, token, key, n, vocab, s.tile, shift, digits, w.count);
-            if (!rc) rc = launch(sort_scan_kernel, dim3(1), dim3(1024), stream, w.count, s.blocks << s.digit_bits);
+            if (!rc) rc = launch(sort_scan_kernel, dim3(digits), dim3(kMaxBlocks), stream, w.count, s.blocks, digits);
             if (!rc)
                 rc = p == 0 ? launch(sort_place_kernel<I, true>, grid, block, stream, token, key, row, n, vocab, s.tile, shift, s.digit_bits, w.count, w.key[0], w.row[0])
                             : launch(sort_place_kernel<I, false>, grid, block, stream, token, key, row, n, vocab, s.tile, shift, s.digit_bits, w.count, w.key[p & 1], w.row[p & 1]);
@@ -334,6 +427,7 @@ int fishing_embedding_forward(int32_t dtype, int32_t index_bytes, int64_t n, int
 
 int64_t fishing_embedding_workspace(int64_t n, int64_t vocab, int64_t dim) {
     if (int rc = embedding_check(FISHING_DTYPE_F32, 4, n, vocab, dim)) return rc;
+    if (table_fits(n, vocab)) return round_up(table_shares(n, vocab, dim) * vocab * dim * 4, 256);
     return embedding_work(sort_plan(n, vocab), n, vocab, dim, nullptr).bytes;
 }
 
