@@ -103,7 +103,7 @@ SIGNATURES = {
     "fishing_reset_normals_f32": (c_i32, [c_i64, c_i64, c_u64, c_u64, c_i32, c_vp, c_vp, c_vp]),
     "fishing_math_f64": (c_i32, [c_i64, c_i32, c_vp, c_vp, c_vp]),
     "fishing_embedding_forward": (c_i32, [c_i32, c_i32, c_i64, c_i64, c_i64, c_vp, c_i64, c_vp, ctypes.c_float, c_vp, c_vp]),
-    "fishing_embedding_workspace": (c_i64, [c_i64, c_i64, c_i64]),
+    "fishing_embedding_workspace": (c_i64, [c_i32, c_i64, c_i64, c_i64]),
     "fishing_embedding_backward": (c_i32, [c_i32, c_i32, c_i64, c_i64, c_i64, c_vp, c_i64, c_vp, ctypes.c_float, c_vp, c_vp, c_i64, c_vp]),
     "fishing_decay_attention_step": (c_i32, [_AP, c_vp]),
     "fishing_decay_attention_workspace": (c_i64, [_AP, c_i32]),

@@ -242,53 +242,6 @@ __global__ void __launch_bounds__(256) embedding_join_kernel(const uint32_t* sta
     }
 }
 
-// ---- small tables (a few hundred tokens: the quota levels) need no sort: a workgroup keeps the sums of its share of the rows for 64 of
-// the columns in LDS, one lane a column, so that a column's additions keep their order without a word between lanes.  A workgroup is one wave.  ----
-constexpr int kTableRows = 16, kSmallTable = 256;
-
-template <typename T, typename I>
-__global__ void __launch_bounds__(64) embedding_table_kernel(const T* dout, int64_t dout_stride, const I* token, int64_t n, int32_t vocab, int32_t dim, int64_t share,
-                                                             float* partial) {
-    extern __shared__ float sums[];                        // [vocab][64]
-    const int lane = threadIdx.x, col = blockIdx.y * 64 + lane;
-    for (int v = 0; v < vocab; ++v) sums[v * 64 + lane] = 0.0f;
-    const int64_t lo = blockIdx.x * share, hi = lo + share < n ? lo + share : n;
-    const T* from = dout + (col < dim ? col : 0);
-    for (int64_t i = lo; i < hi; i += kTableRows) {
-        T x[kTableRows];
-        int at[kTableRows];
-#pragma unroll
-        for (int u = 0; u < kTableRows; ++u) {
-            const int64_t r = i + u < hi ? i + u : hi - 1;
-            const int64_t t = (int64_t)token[r];
-            at[u] = i + u < hi && t >= 0 && t < vocab ? (int)t : -1;
-            x[u] = from[r * dout_stride];
-        }
-#pragma unroll
-        for (int u = 0; u < kTableRows; ++u)
-            if (at[u] >= 0) sums[at[u] * 64 + lane] += to_f32(x[u]);
-    }
-    if (col >= dim) return;
-    float* to = partial + (int64_t)blockIdx.x * vocab * dim + col;
-    for (int v = 0; v < vocab; ++v) to[(int64_t)v * dim] = sums[v * 64 + lane];
-}
-
-// the shares' tables added in order; L lanes take every L-th
-template <typename T>
-__global__ void __launch_bounds__(256) embedding_table_join_kernel(const float* partial, int shares, int64_t size, float scale, T* dtable) {
-    __shared__ float part[4][64];
-    const int c = threadIdx.x & 63, l = threadIdx.x >> 6;
-    const int64_t at = (int64_t)blockIdx.x * 64 + c;
-    float s = 0.0f;
-    if (at < size) {
-#pragma unroll 8
-        for (int x = l; x < shares; x += 4) s += partial[x * size + at];
-    }
-    part[l][c] = s;
-    __syncthreads();
-    if (l == 0 && at < size) dtable[at] = from_f32<T>((part[0][c] + part[1][c] + part[2][c] + part[3][c]) * scale);
-}
-
 struct SortPlan {
     int bits, passes, digit_bits;
     int64_t tile;
@@ -297,7 +250,7 @@ struct SortPlan {
     int64_t chunks;
 };
 
-static SortPlan sort_plan(int64_t n, int64_t vocab) {
+static SortPlan sort_plan(int64_t n, int64_t vocab, int64_t lanes) {
     SortPlan s;
     s.bits = 1;
     while (((int64_t)1 << s.bits) <= vocab) ++s.bits;         // keys 0 .. vocab
@@ -305,7 +258,11 @@ static SortPlan sort_plan(int64_t n, int64_t vocab) {
     s.digit_bits = (s.bits + s.passes - 1) / s.passes;
     s.tile = round_up(ceil_div(n > 0 ? n : 1, kMaxBlocks), 2 * kSortThreads);
     s.blocks = (int)ceil_div(n > 0 ? n : 1, s.tile);
-    s.chunk = n >= (1 << 20) ? 128 : n >= (1 << 18) ? 64 : n >= (1 << 16) ? 32 : 16;
+    // A chunk is a group's: so long that about 4096 waves of groups share the rows (64 waves' worth of rows in flight on every CU; 1034240
+    // rows of 256 f32: 256 rows a chunk 257 us with the join, 64 292; 413696 rows of 128 bf16: 64 49 us, 256 157), within 16 .. 256
+    const int64_t group = lanes <= 8 ? 8 : lanes <= 16 ? 16 : lanes <= 32 ? 32 : 64;
+    s.chunk = 16;
+    while (s.chunk < 256 && s.chunk * 4096 * (64 / group) < n * ceil_div(lanes, 64)) s.chunk *= 2;
     s.chunks = ceil_div(n, s.chunk);
     return s;
 }
@@ -330,6 +287,9 @@ static EmbeddingWork embedding_work(const SortPlan& s, int64_t n, int64_t vocab,
     return w;
 }
 
+// lanes that a row takes in 16-byte accesses
+static int64_t row_lanes(int32_t dtype, int64_t dim) { return ceil_div(dim, dtype == FISHING_DTYPE_F32 ? 4 : 8); }
+
 static int embedding_check(int32_t dtype, int32_t index_bytes, int64_t n, int64_t vocab, int64_t dim) {
     if (dtype != FISHING_DTYPE_F32 && dtype != FISHING_DTYPE_BF16) return FISHING_ERR_UNSUPPORTED;
     if (index_bytes != 4 && index_bytes != 8) return FISHING_ERR_UNSUPPORTED;
@@ -348,30 +308,11 @@ static int embedding_forward(int64_t n, int64_t vocab, int64_t dim, const T* tab
     return go(embedding_kernel<T, I, 1>, (int)dim);
 }
 
-// How a small table's rows are shared out: so many waves that a share's table (written and read once) stays small beside its rows
-static int64_t table_shares(int64_t n, int64_t vocab, int64_t dim) {
-    const int64_t slices = ceil_div(dim, 64), fit = 160 * 1024 / (vocab * 256);               // tables of a CU's LDS
-    int64_t shares = 256 * (fit < 16 ? fit : 16) / slices;
-    const int64_t most = n / (2 * vocab);
-    if (shares > most) shares = most;
-    return shares > 0 ? shares : 1;
-}
-
-static bool table_fits(int64_t n, int64_t vocab) { return vocab <= kSmallTable && n >= 16 * vocab; }
-
 template <typename T, typename I>
 static int embedding_backward(int64_t n, int64_t vocab, int64_t dim, const T* dout, int64_t dout_stride, const I* token, float scale, T* dtable, void* workspace,
                               hipStream_t stream) {
     int rc = 0;
-    if (table_fits(n, vocab)) {
-        const int64_t shares = table_shares(n, vocab, dim), share = ceil_div(n, shares);
-        const dim3 grid((unsigned)ceil_div(n, share), (unsigned)ceil_div(dim, 64));
-        float* partial = (float*)workspace;
-        rc = launch_lds(embedding_table_kernel<T, I>, grid, dim3(64), (size_t)vocab * 256, stream, dout, dout_stride, token, n, (int32_t)vocab, (int32_t)dim, share, partial);
-        if (rc) return rc;
-        return launch(embedding_table_join_kernel<T>, dim3((unsigned)ceil_div(vocab * dim, 64)), dim3(256), stream, partial, (int)grid.x, vocab * dim, scale, dtable);
-    }
-    const SortPlan s = sort_plan(n, vocab);
+    const SortPlan s = sort_plan(n, vocab, row_lanes(sizeof(T) == 4 ? FISHING_DTYPE_F32 : FISHING_DTYPE_BF16, dim));
     const EmbeddingWork w = embedding_work(s, n, vocab, dim, workspace);
     if (n > 0) {
         for (int p = 0; p < s.passes && !rc; ++p) {
@@ -425,10 +366,9 @@ int fishing_embedding_forward(int32_t dtype, int32_t index_bytes, int64_t n, int
                             : embedding_forward<bf16, int64_t>(n, vocab, dim, (const bf16*)table, table_stride, (const int64_t*)token, scale, (bf16*)out, st);
 }
 
-int64_t fishing_embedding_workspace(int64_t n, int64_t vocab, int64_t dim) {
-    if (int rc = embedding_check(FISHING_DTYPE_F32, 4, n, vocab, dim)) return rc;
-    if (table_fits(n, vocab)) return round_up(table_shares(n, vocab, dim) * vocab * dim * 4, 256);
-    return embedding_work(sort_plan(n, vocab), n, vocab, dim, nullptr).bytes;
+int64_t fishing_embedding_workspace(int32_t dtype, int64_t n, int64_t vocab, int64_t dim) {
+    if (int rc = embedding_check(dtype, 4, n, vocab, dim)) return rc;
+    return embedding_work(sort_plan(n, vocab, row_lanes(dtype, dim)), n, vocab, dim, nullptr).bytes;
 }
 
 int fishing_embedding_backward(int32_t dtype, int32_t index_bytes, int64_t n, int64_t vocab, int64_t dim, const void* dout, int64_t dout_stride, const void* token,
@@ -437,7 +377,7 @@ int fishing_embedding_backward(int32_t dtype, int32_t index_bytes, int64_t n, in
     if (n > 0 && dout_stride < dim) return FISHING_ERR_SIZE;
     if (!dtable || !workspace || (n > 0 && (!dout || !token))) return FISHING_ERR_NULL;
     if (!aligned16(workspace)) return FISHING_ERR_ALIGN;
-    if (workspace_bytes < fishing_embedding_workspace(n, vocab, dim)) return FISHING_ERR_SIZE;
+    if (workspace_bytes < fishing_embedding_workspace(dtype, n, vocab, dim)) return FISHING_ERR_SIZE;
     hipStream_t st = (hipStream_t)stream;
     if (dtype == FISHING_DTYPE_F32)
         return index_bytes == 4 ? embedding_backward<float, int32_t>(n, vocab, dim, (const float*)dout, dout_stride, (const int32_t*)token, scale, (float*)dtable, workspace, st)

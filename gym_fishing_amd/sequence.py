@@ -99,7 +99,7 @@ class _Embedding(torch.autograd.Function):
         lib, n = _capi.lib(), tokens.numel()
         grad = _rows(grad.reshape(n, dim))
         out = torch.empty((vocab, dim), dtype=grad.dtype, device=grad.device)
-        work = _workspace(lib.fishing_embedding_workspace(n, vocab, dim), grad.device)
+        work = _workspace(lib.fishing_embedding_workspace(_DTYPES[grad.dtype], n, vocab, dim), grad.device)
         _call(lib.fishing_embedding_backward, grad.device, _DTYPES[grad.dtype], tokens.element_size(), n, vocab, dim, grad.data_ptr(), _row_stride(grad),
               tokens.data_ptr(), ctx.scale, out.data_ptr(), work.data_ptr(), work.numel())
         return None, out, None

@@ -394,7 +394,7 @@ int fishing_math_f64(int64_t n, int32_t fn, const double* in, double* out, fishi
 int fishing_embedding_forward(int32_t dtype, int32_t index_bytes, int64_t n, int64_t vocab, int64_t dim, const void* table, int64_t table_stride, const void* token,
                               float scale, void* out, fishing_stream_t stream);
 /* dtable[v, :] = scale * sum of dout[i, :] over token[i] == v, for every v < vocab (zeros where none); contiguous [vocab, dim]. */
-int64_t fishing_embedding_workspace(int64_t n, int64_t vocab, int64_t dim);
+int64_t fishing_embedding_workspace(int32_t dtype, int64_t n, int64_t vocab, int64_t dim);
 int fishing_embedding_backward(int32_t dtype, int32_t index_bytes, int64_t n, int64_t vocab, int64_t dim, const void* dout, int64_t dout_stride, const void* token,
                                float scale, void* dtable, void* workspace, int64_t workspace_bytes, fishing_stream_t stream);
 

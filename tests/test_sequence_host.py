@@ -43,10 +43,10 @@ def test_embedding_arguments(lib):
     assert fwd(2, 4, 8, 5, 8, 64, 8, 64, 1.0, 64, None) == -7 and fwd(0, 2, 8, 5, 8, 64, 8, 64, 1.0, 64, None) == -7
     for n, vocab, dim in ((-1, 5, 8), (2 ** 31, 5, 8), (8, 0, 8), (8, 5, 0), (8, 5, 65537)):
         assert fwd(0, 4, n, vocab, dim, 64, 8, 64, 1.0, 64, None) == -4
-        assert lib.fishing_embedding_workspace(n, vocab, dim) == -4
+        assert lib.fishing_embedding_workspace(0, n, vocab, dim) == -4
     assert fwd(0, 4, 8, 5, 8, 64, 7, 64, 1.0, 64, None) == -4
     assert fwd(0, 4, 8, 5, 8, None, 8, 64, 1.0, 64, None) == -1 and fwd(0, 4, 0, 5, 8, None, 8, None, 1.0, None, None) == 0
-    need = lib.fishing_embedding_workspace(8, 5, 8)
+    need = lib.fishing_embedding_workspace(0, 8, 5, 8)
     assert need > 0
     assert bwd(0, 4, 8, 5, 8, 64, 8, 64, 1.0, 64, 256, need - 1, None) == -4
     assert bwd(0, 4, 8, 5, 8, 64, 8, 64, 1.0, 64, 260, need, None) == -3
