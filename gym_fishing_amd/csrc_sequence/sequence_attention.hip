@@ -94,7 +94,7 @@ static int attention_check(const FishingDecayAttention* a, bool one_step) {
     if (!a) return FISHING_ERR_NULL;
     if (a->dtype != FISHING_DTYPE_F32 && a->dtype != FISHING_DTYPE_BF16) return FISHING_ERR_UNSUPPORTED;
     if (a->batch < 0 || a->steps < 0 || a->heads < 1 || a->dk < 1 || a->dk > kMaxHeadDim || a->dv < 1 || a->dv > kMaxHeadDim) return FISHING_ERR_SIZE;
-    if (a->batch > 0x7fffffff / a->heads) return FISHING_ERR_SIZE;
+    if (a->heads > kMaxHeads || a->batch > 0x7fffffff / a->heads) return FISHING_ERR_SIZE;
     if (a->batch == 0) return FISHING_OK;
     if (!a->log_decay) return FISHING_ERR_NULL;
     if ((one_step || a->steps > 0) && (!a->q || !a->k || !a->v)) return FISHING_ERR_NULL;
@@ -105,11 +105,17 @@ static Strided strided(const void* p, const int64_t* s) { return Strided{p, s[0]
 
 template <typename T>
 static int attention_step(const FishingDecayAttention* a, hipStream_t stream) {
-    const int64_t pairs = a->batch * a->heads;
+    const int64_t block = batch_block(a->batch, a->heads), state = (int64_t)a->heads * a->dk * a->dv;
     auto go = [&](auto kernel) {
-        return launch(kernel, dim3((unsigned)ceil_div(pairs, 4)), dim3(256), stream, strided(a->q, a->q_stride), strided(a->k, a->k_stride), strided(a->v, a->v_stride),
-                      a->log_decay, a->starts, a->starts_stride[0], a->state, a->state_out, (T*)a->out, a->out_stride[0], a->out_stride[2], pairs, a->heads, a->dk, a->dv,
-                      (float)a->scale);
+        int rc = 0;
+        for (int64_t n = 0; n < a->batch && !rc; n += block) {
+            const int64_t pairs = (a->batch - n < block ? a->batch - n : block) * a->heads;
+            auto from = [&](const void* p, const int64_t* s) { return strided((const T*)p + n * s[0], s); };
+            rc = launch(kernel, dim3((unsigned)ceil_div(pairs, 4)), dim3(256), stream, from(a->q, a->q_stride), from(a->k, a->k_stride), from(a->v, a->v_stride), a->log_decay,
+                        a->starts ? a->starts + n * a->starts_stride[0] : nullptr, a->starts_stride[0], a->state + n * state, a->state_out + n * state,
+                        (T*)a->out + n * a->out_stride[0], a->out_stride[0], a->out_stride[2], pairs, a->heads, a->dk, a->dv, (float)a->scale);
+        }
+        return rc;
     };
     if (a->dv % 4 == 0 && aligned16(a->state) && aligned16(a->state_out)) return go(step_kernel_recurrent<T, 4>);
     return go(step_kernel_recurrent<T, 1>);
@@ -151,7 +157,7 @@ int fishing_decay_attention_step(const FishingDecayAttention* a, fishing_stream_
 int64_t fishing_decay_attention_workspace(const FishingDecayAttention* a, int32_t backward) {
     if (int rc = attention_check(a, false)) return rc;
     // the largest of its walks, which run one after the other, whichever way their rows are read
-    const int64_t pairs = a->batch * a->heads;
+    const int64_t pairs = batch_block(a->batch, a->heads) * a->heads;
     int64_t most = 0;
     for (int back = 0; back <= (backward ? 1 : 0); ++back)
         for (int wide = 0; wide < 2; ++wide) {

@@ -227,18 +227,19 @@ __global__ void __launch_bounds__(256) embedding_sum_kernel(const T* dout, int64
 template <typename T>
 __global__ void __launch_bounds__(256) embedding_join_kernel(const uint32_t* start, const float* partial, int64_t n, int64_t vocab, int32_t dim, int32_t chunk,
                                                              float scale, T* dtable) {
-    const int64_t v = blockIdx.x;
-    const int64_t s = n ? start[v] : 0, e = n ? start[v + 1] : 0;
-    const int64_t a = s / chunk, b = e > s ? (e - 1) / chunk : a;
-    if (e > s && a == b) return;
-    for (int col = threadIdx.x; col < dim; col += 256) {
-        float acc = 0.0f;
-        if (e > s) {
-            acc = partial[(2 * a + (s == a * chunk ? 0 : 1)) * dim + col];
+    for (int64_t v = blockIdx.x; v < vocab; v += gridDim.x) {
+        const int64_t s = n ? start[v] : 0, e = n ? start[v + 1] : 0;
+        const int64_t a = s / chunk, b = e > s ? (e - 1) / chunk : a;
+        if (e > s && a == b) continue;
+        for (int col = threadIdx.x; col < dim; col += 256) {
+            float acc = 0.0f;
+            if (e > s) {
+                acc = partial[(2 * a + (s == a * chunk ? 0 : 1)) * dim + col];
 #pragma unroll 8
-            for (int64_t c = a + 1; c <= b; ++c) acc += partial[2 * c * dim + col];
+                for (int64_t c = a + 1; c <= b; ++c) acc += partial[2 * c * dim + col];
+            }
+            dtable[v * dim + col] = from_f32<T>(acc * scale);
         }
-        dtable[v * dim + col] = from_f32<T>(acc * scale);
     }
 }
 
@@ -297,12 +298,19 @@ static int embedding_check(int32_t dtype, int32_t index_bytes, int64_t n, int64_
     return FISHING_OK;
 }
 
+constexpr int64_t kMaxGrid = (int64_t)1 << 22;      // workgroups of 256, whose threads count in 32 bits
+
 template <typename T, typename I>
 static int embedding_forward(int64_t n, int64_t vocab, int64_t dim, const T* table, int64_t table_stride, const I* token, float scale, T* out, hipStream_t stream) {
     constexpr int V = vec_of<T>();
     auto go = [&](auto kernel, int vecs) {
-        const int64_t per = vecs < 256 ? 256 / vecs : 1;
-        return launch(kernel, dim3((unsigned)ceil_div(n, 4 * per)), dim3(256), stream, table, table_stride, token, n, vocab, vecs, scale, out);
+        const int64_t block = (vecs < 256 ? 256 / vecs : 1) * 4 * kMaxGrid;       // rows of a launch
+        int rc = 0;
+        for (int64_t i = 0; i < n && !rc; i += block) {
+            const int64_t here = n - i < block ? n - i : block;
+            rc = launch(kernel, dim3((unsigned)ceil_div(here, block / kMaxGrid)), dim3(256), stream, table, table_stride, token + i, here, vocab, vecs, scale, out + i * dim);
+        }
+        return rc;
     };
     if (dim % V == 0 && table_stride % V == 0 && aligned16(table) && aligned16(out)) return go(embedding_kernel<T, I, V>, (int)(dim / V));
     return go(embedding_kernel<T, I, 1>, (int)dim);
@@ -342,7 +350,7 @@ static int embedding_backward(int64_t n, int64_t vocab, int64_t dim, const T* do
         }
         if (rc) return rc;
     }
-    return launch(embedding_join_kernel<T>, dim3((unsigned)vocab), dim3(256), stream, w.start, w.partial, n, vocab, (int32_t)dim, s.chunk, scale, dtable);
+    return launch(embedding_join_kernel<T>, dim3((unsigned)(vocab < kMaxGrid ? vocab : kMaxGrid)), dim3(256), stream, w.start, w.partial, n, vocab, (int32_t)dim, s.chunk, scale, dtable);
 }
 
 }  // namespace seq

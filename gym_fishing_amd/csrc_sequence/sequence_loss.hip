@@ -271,8 +271,7 @@ static int slab_sum(const float* slabs, int64_t slab, int64_t count, T* out, int
 
 template <typename T>
 __global__ void __launch_bounds__(256) zero_kernel(T* p, int64_t n) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i < n) p[i] = from_f32<T>(0.0f);
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) p[i] = from_f32<T>(0.0f);
 }
 
 // ---- the plan: tile sizes, pieces, shares ----
@@ -324,9 +323,13 @@ static int with_tile(int64_t b, F&& f) {
 }
 static int64_t part_levels(int64_t b) { return b == 256 ? 64 : b / 2; }      // levels of a wave's columns
 
+// The rows are walked in blocks, so that dz^T of a piece stays under 2^30 elements, the forward's pairs under 2^28 and dz^T's pitch
+// (2^21 rows: at most 8 MiB) within a staged tile's 32-bit offsets
+constexpr int64_t kBlockRows = (int64_t)1 << 21, kMaxPitch = (int64_t)1 << 23;
+
 struct LossPlan {
-    int64_t bk, dim_p, rows_p, piece;       // elements of a staged k step; padded depth and row count; levels of a piece
-    int64_t z;                              // forward: tile edge
+    int64_t block, bk, dim_p, rows_p, piece;       // rows of a block; elements of a staged k step; padded depth and block; levels of a piece
+    int64_t z;                                     // forward: tile edge
     int parts;
     Tiling dh;                              // of a whole piece; the last one's is made for its width
 };
@@ -335,12 +338,11 @@ template <typename T>
 static Tiling dw_tiling(const LossPlan& p, int64_t width, int64_t dim) { return tiling<T>(dim, width, p.rows_p, true); }
 
 template <typename T>
-static LossPlan loss_plan(int64_t rows, int64_t levels, int64_t dim) {
+static LossPlan loss_plan(int64_t rows, int64_t levels, int64_t dim, bool backward) {
     LossPlan p{};
     rows = rows > 0 ? rows : 1;
     p.bk = 128 / (int64_t)sizeof(T);
     p.dim_p = round_up(dim, p.bk);
-    p.rows_p = round_up(rows, p.bk);
     p.z = tiling<T>(rows, levels, dim, false).b;
     p.parts = (int)(ceil_div(levels, p.z) * (p.z / part_levels(p.z)));
     // A piece keeps dz^T for the two products: at most 24576 levels, at least 8192, and of those the width whose product for dW
@@ -359,7 +361,12 @@ static LossPlan loss_plan(int64_t rows, int64_t levels, int64_t dim) {
         }
         if (p.piece > levels) p.piece = levels;
     }
-    p.dh = tiling<T>(dim, rows, p.piece, true);
+    const int64_t widest = backward ? (p.piece > p.dim_p ? p.piece : p.dim_p) : (p.parts > p.dim_p / 4 ? p.parts : p.dim_p / 4) * 4;
+    p.block = (((int64_t)1 << 30) / widest) & ~(int64_t)255;
+    p.block = p.block < 256 ? 256 : p.block > kBlockRows ? kBlockRows : p.block;
+    p.block = p.block > rows ? rows : p.block;
+    p.rows_p = round_up(p.block, p.bk);
+    p.dh = tiling<T>(dim, p.block, p.piece, true);
     return p;
 }
 
@@ -367,7 +374,7 @@ template <typename T>
 struct LossWork {
     float *top = nullptr, *sum = nullptr, *taken = nullptr, *dh = nullptr, *dw = nullptr;
     T *h = nullptr, *w = nullptr, *dzt = nullptr;
-    int64_t dh_slab = 0, bytes = 0;
+    int64_t dh_slab = 0, dw_slab = 0, bytes = 0;
 };
 
 // the padded copies are counted whether the operands need them or not: the caller asks before the pointers are known
@@ -375,19 +382,21 @@ template <typename T>
 static LossWork<T> loss_work(const LossPlan& p, int64_t rows, int64_t levels, int64_t dim, bool backward, void* at) {
     Carve c(at);
     LossWork<T> w;
-    w.h = c.take<T>(rows * p.dim_p);
+    w.h = c.take<T>(p.block * p.dim_p);
     w.w = c.take<T>(levels * p.dim_p);
     if (backward) {
         w.dzt = c.take<T>(round_up(p.piece, 256) * p.rows_p);
-        w.dh_slab = round_up(rows * dim, 4);
+        w.dh_slab = round_up(p.block * dim, 4);
         if (p.dh.shares > 1 || p.piece < levels) w.dh = c.take<float>(p.dh.shares * w.dh_slab);
         const int64_t last = levels % p.piece, a = dw_tiling<T>(p, p.piece, dim).shares, b = last ? dw_tiling<T>(p, last, dim).shares : 1;
         const int64_t slabs_a = a > 1 ? a * round_up(p.piece * dim, 4) : 0, slabs_b = b > 1 ? b * round_up(last * dim, 4) : 0;
-        w.dw = c.take<float>(slabs_a > slabs_b ? slabs_a : slabs_b);
+        // several blocks of rows add to slabs of all levels, one block's pieces share slabs of their own levels
+        w.dw_slab = p.block < rows ? round_up(levels * dim, 4) : 0;
+        w.dw = c.take<float>(w.dw_slab ? a * w.dw_slab : slabs_a > slabs_b ? slabs_a : slabs_b);
     } else {
-        w.top = c.take<float>(rows * p.parts);
-        w.sum = c.take<float>(rows * p.parts);
-        w.taken = c.take<float>(rows);
+        w.top = c.take<float>(p.block * p.parts);
+        w.sum = c.take<float>(p.block * p.parts);
+        w.taken = c.take<float>(p.block);
     }
     w.bytes = c.used + 256;
     return w;
@@ -396,7 +405,7 @@ static LossWork<T> loss_work(const LossPlan& p, int64_t rows, int64_t levels, in
 static int loss_check(int32_t dtype, int64_t rows, int64_t levels, int64_t dim) {
     if (dtype != FISHING_DTYPE_F32 && dtype != FISHING_DTYPE_BF16) return FISHING_ERR_UNSUPPORTED;
     if (rows < 0 || rows > 0x7fffffff || levels < 1 || levels > 0x7ffffff || dim < 1 || dim > 65536) return FISHING_ERR_SIZE;
-    if (ceil_div(rows, 64) * ceil_div(levels, 64) > 0x7fffffff || ceil_div(rows, 64) * ceil_div(dim, 64) > 0x7fffffff) return FISHING_ERR_SIZE;    // workgroups of a launch
+    if (levels * round_up(dim, 64) > (int64_t)1 << 33) return FISHING_ERR_SIZE;    // threads of a launch over the head, in 32 bits
     return FISHING_OK;
 }
 
@@ -409,7 +418,7 @@ static int pad(const T* src, int64_t ld, int64_t rows, int64_t width, T* dst, in
 // the operand as it is where its rows are whole k steps at 16-byte addresses, its padded copy otherwise
 template <typename T>
 static int padded_operand(const LossPlan& p, const T* src, int64_t ld, int64_t rows, int64_t dim, T* copy, Operand<T>& o, hipStream_t stream) {
-    if (dim == p.dim_p && ld % vec_of<T>() == 0 && aligned16(src)) {
+    if (dim == p.dim_p && ld % vec_of<T>() == 0 && aligned16(src) && ld * (int64_t)sizeof(T) <= kMaxPitch) {
         o = Operand<T>{src, ld, rows, rows};
         return 0;
     }
@@ -420,23 +429,28 @@ static int padded_operand(const LossPlan& p, const T* src, int64_t ld, int64_t r
 template <typename T>
 static int loss_forward(int64_t rows, int64_t levels, int64_t dim, const T* h, int64_t h_ld, const T* w, int64_t w_ld, const void* target, int target_bytes, float* loss,
                         float* lse, void* workspace, hipStream_t stream) {
-    const LossPlan p = loss_plan<T>(rows, levels, dim);
+    const LossPlan p = loss_plan<T>(rows, levels, dim, false);
     const LossWork<T> k = loss_work<T>(p, rows, levels, dim, false, workspace);
     Operand<T> a, b;
-    int rc = padded_operand<T>(p, h, h_ld, rows, dim, k.h, a, stream);
-    if (!rc) rc = padded_operand<T>(p, w, w_ld, levels, dim, k.w, b, stream);
-    if (rc) return rc;
-    rc = with_tile<T, false, false>(p.z, [&](auto t) {
-        typedef decltype(t) Tile;
-        const int64_t tm = ceil_div(rows, Tile::EDGE), tn = ceil_div(levels, Tile::EDGE);
-        return launch(loss_part_kernel<T, typename Tile::G, Tile::EDGE, Tile::EDGE>, dim3((unsigned)(tm * tn)), dim3(Tile::G::THREADS), stream, a, b, p.dim_p, target, target_bytes,
-                      tm, tn, k.top, k.sum, k.taken);
-    });
-    if (rc) return rc;
-    auto join_parts = [&](auto kernel, int r, int l) {
-        return launch(kernel, dim3((unsigned)ceil_div(rows, r)), dim3(r * l), stream, k.top, k.sum, k.taken, target, target_bytes, rows, levels, p.parts, loss, lse);
-    };
-    return p.parts <= 8 ? join_parts(loss_join_kernel<256, 1>, 256, 1) : p.parts <= 64 ? join_parts(loss_join_kernel<32, 8>, 32, 8) : join_parts(loss_join_kernel<16, 64>, 16, 64);
+    int rc = padded_operand<T>(p, w, w_ld, levels, dim, k.w, b, stream);
+    for (int64_t r0 = 0; r0 < rows && !rc; r0 += p.block) {
+        const int64_t here = rows - r0 < p.block ? rows - r0 : p.block;
+        const void* y = (const char*)target + r0 * target_bytes;
+        rc = padded_operand<T>(p, h + r0 * h_ld, h_ld, here, dim, k.h, a, stream);
+        if (rc) break;
+        rc = with_tile<T, false, false>(p.z, [&](auto t) {
+            typedef decltype(t) Tile;
+            const int64_t tm = ceil_div(here, Tile::EDGE), tn = ceil_div(levels, Tile::EDGE);
+            return launch(loss_part_kernel<T, typename Tile::G, Tile::EDGE, Tile::EDGE>, dim3((unsigned)(tm * tn)), dim3(Tile::G::THREADS), stream, a, b, p.dim_p, y, target_bytes,
+                          tm, tn, k.top, k.sum, k.taken);
+        });
+        if (rc) break;
+        auto join_parts = [&](auto kernel, int r, int l) {
+            return launch(kernel, dim3((unsigned)ceil_div(here, r)), dim3(r * l), stream, k.top, k.sum, k.taken, y, target_bytes, here, levels, p.parts, loss + r0, lse + r0);
+        };
+        rc = p.parts <= 8 ? join_parts(loss_join_kernel<256, 1>, 256, 1) : p.parts <= 64 ? join_parts(loss_join_kernel<32, 8>, 32, 8) : join_parts(loss_join_kernel<16, 64>, 16, 64);
+    }
+    return rc;
 }
 
 template <typename T, typename O, bool A_MAJOR, bool B_MAJOR>
@@ -452,42 +466,52 @@ static int product(const Operand<T>& a, const Operand<T>& b, const Tiling& t, in
 template <typename T>
 static int loss_backward(int64_t rows, int64_t levels, int64_t dim, const T* h, int64_t h_ld, const T* w, int64_t w_ld, const void* target, int target_bytes, const float* lse,
                          const float* g, T* dh, T* dw, void* workspace, hipStream_t stream) {
-    const LossPlan p = loss_plan<T>(rows, levels, dim);
+    const LossPlan p = loss_plan<T>(rows, levels, dim, true);
     const LossWork<T> k = loss_work<T>(p, rows, levels, dim, true, workspace);
-    Operand<T> a{k.h, p.dim_p, rows, rows}, b;
-    int rc = pad<T>(h, h_ld, rows, dim, k.h, p.dim_p, target, target_bytes, levels, stream);
-    if (!rc) rc = padded_operand<T>(p, w, w_ld, levels, dim, k.w, b, stream);
-    for (int64_t v0 = 0; v0 < levels && !rc; v0 += p.piece) {
-        const int64_t width = levels - v0 < p.piece ? levels - v0 : p.piece, width_p = round_up(width, p.bk);
-        rc = with_tile<T, false, false>(tiling<T>(rows, width, dim, false).b, [&](auto t) {
-            typedef decltype(t) Tile;
-            const int64_t tm = ceil_div(rows, Tile::EDGE), tn = ceil_div(width, Tile::EDGE);
-            return launch(loss_dz_kernel<T, typename Tile::G, Tile::EDGE, Tile::EDGE>, dim3((unsigned)(tm * tn)), dim3(Tile::G::THREADS), stream, a, b, p.dim_p, target, target_bytes,
-                          levels, v0, tm, tn, lse, g, k.dzt, p.rows_p);
-        });
-        if (rc) break;
-        // dh[r][d]: m = d, n = r, k = the piece's levels, both operands k-major; W's rows beyond the last meet zeros of dz
-        const Operand<T> wd{b.p + v0 * b.ld, b.ld, p.dim_p, width}, zr{k.dzt, p.rows_p, p.rows_p, width_p};
-        Tiling t = width == p.piece ? p.dh : tiling<T>(dim, rows, width, true);
-        if (t.shares > p.dh.shares) {                       // (the first piece's slabs are all there are)
-            t.share = round_up(ceil_div(width_p, p.dh.shares), p.bk);
-            t.shares = ceil_div(width_p, t.share);
+    const Tiling whole = dw_tiling<T>(p, p.piece, dim);
+    Operand<T> b;
+    int rc = padded_operand<T>(p, w, w_ld, levels, dim, k.w, b, stream);
+    for (int64_t r0 = 0; r0 < rows && !rc; r0 += p.block) {
+        const int64_t here = rows - r0 < p.block ? rows - r0 : p.block, here_p = round_up(here, p.bk);
+        const void* y = (const char*)target + r0 * target_bytes;
+        const Operand<T> a{k.h, p.dim_p, here, here};
+        rc = pad<T>(h + r0 * h_ld, h_ld, here, dim, k.h, p.dim_p, y, target_bytes, levels, stream);
+        for (int64_t v0 = 0; v0 < levels && !rc; v0 += p.piece) {
+            const int64_t width = levels - v0 < p.piece ? levels - v0 : p.piece, width_p = round_up(width, p.bk);
+            rc = with_tile<T, false, false>(tiling<T>(here, width, dim, false).b, [&](auto t) {
+                typedef decltype(t) Tile;
+                const int64_t tm = ceil_div(here, Tile::EDGE), tn = ceil_div(width, Tile::EDGE);
+                return launch(loss_dz_kernel<T, typename Tile::G, Tile::EDGE, Tile::EDGE>, dim3((unsigned)(tm * tn)), dim3(Tile::G::THREADS), stream, a, b, p.dim_p, y, target_bytes,
+                              levels, v0, tm, tn, lse + r0, g + r0, k.dzt, here_p);
+            });
+            if (rc) break;
+            // dh[r][d]: m = d, n = r, k = the piece's levels, both operands k-major; W's rows beyond the last meet zeros of dz
+            const Operand<T> wd{b.p + v0 * b.ld, b.ld, p.dim_p, width}, zr{k.dzt, here_p, here_p, width_p};
+            Tiling t = width == p.piece ? p.dh : tiling<T>(dim, here, width, true);
+            if (t.shares > p.dh.shares) {                       // (the first piece's slabs are all there are)
+                t.share = round_up(ceil_div(width_p, p.dh.shares), p.bk);
+                t.shares = ceil_div(width_p, t.share);
+            }
+            rc = k.dh ? product<T, float, true, true>(wd, zr, t, width_p, dim, here, v0 > 0, k.dh, dim, k.dh_slab, stream)
+                      : product<T, T, true, true>(wd, zr, t, width_p, dim, here, false, dh + r0 * dim, dim, 0, stream);
+            if (rc) break;
+            // dW[v][d]: m = d, n = v, k = rows; h's rows beyond the last meet zeros of dz.  (A share behind the last block's rows adds
+            // nothing to its slab.)
+            const Operand<T> hd{k.h, p.dim_p, p.dim_p, here}, zv{k.dzt, here_p, width, width};
+            t = k.dw_slab ? whole : dw_tiling<T>(p, width, dim);
+            if (k.dw_slab) {
+                rc = product<T, float, true, false>(hd, zv, t, here_p, dim, width, r0 > 0, k.dw + v0 * dim, dim, k.dw_slab, stream);
+            } else if (t.shares > 1) {
+                const int64_t slab = round_up(width * dim, 4);
+                rc = product<T, float, true, false>(hd, zv, t, here_p, dim, width, false, k.dw, dim, slab, stream);
+                if (!rc) rc = slab_sum<T>(k.dw, slab, t.shares, dw + v0 * dim, width * dim, stream);
+            } else {
+                rc = product<T, T, true, false>(hd, zv, t, here_p, dim, width, false, dw + v0 * dim, dim, 0, stream);
+            }
         }
-        rc = k.dh ? product<T, float, true, true>(wd, zr, t, width_p, dim, rows, v0 > 0, k.dh, dim, k.dh_slab, stream)
-                  : product<T, T, true, true>(wd, zr, t, width_p, dim, rows, false, dh, dim, 0, stream);
-        if (rc) break;
-        // dW[v][d]: m = d, n = v, k = rows; h's rows beyond the last meet zeros of dz
-        const Operand<T> hd{k.h, p.dim_p, p.dim_p, rows}, zv{k.dzt, p.rows_p, width, width};
-        t = dw_tiling<T>(p, width, dim);
-        if (t.shares > 1) {
-            const int64_t slab = round_up(width * dim, 4);
-            rc = product<T, float, true, false>(hd, zv, t, p.rows_p, dim, width, false, k.dw, dim, slab, stream);
-            if (!rc) rc = slab_sum<T>(k.dw, slab, t.shares, dw + v0 * dim, width * dim, stream);
-        } else {
-            rc = product<T, T, true, false>(hd, zv, t, p.rows_p, dim, width, false, dw + v0 * dim, dim, 0, stream);
-        }
+        if (!rc && k.dh) rc = slab_sum<T>(k.dh, k.dh_slab, p.dh.shares, dh + r0 * dim, here * dim, stream);
     }
-    if (!rc && k.dh) rc = slab_sum<T>(k.dh, k.dh_slab, p.dh.shares, dh, rows * dim, stream);
+    if (!rc && k.dw_slab) rc = slab_sum<T>(k.dw, k.dw_slab, whole.shares, dw, levels * dim, stream);
     return rc;
 }
 
@@ -500,8 +524,8 @@ extern "C" {
 
 int64_t fishing_cross_entropy_workspace(int32_t dtype, int64_t rows, int64_t levels, int64_t dim, int32_t backward) {
     if (int rc = loss_check(dtype, rows, levels, dim)) return rc;
-    return dtype == FISHING_DTYPE_F32 ? loss_work<float>(loss_plan<float>(rows, levels, dim), rows, levels, dim, backward != 0, nullptr).bytes
-                                      : loss_work<bf16>(loss_plan<bf16>(rows, levels, dim), rows, levels, dim, backward != 0, nullptr).bytes;
+    return dtype == FISHING_DTYPE_F32 ? loss_work<float>(loss_plan<float>(rows, levels, dim, backward != 0), rows, levels, dim, backward != 0, nullptr).bytes
+                                      : loss_work<bf16>(loss_plan<bf16>(rows, levels, dim, backward != 0), rows, levels, dim, backward != 0, nullptr).bytes;
 }
 
 int fishing_cross_entropy_forward(int32_t dtype, int32_t target_bytes, int64_t rows, int64_t levels, int64_t dim, const void* hidden, int64_t hidden_stride, const void* head,
@@ -530,7 +554,8 @@ int fishing_cross_entropy_backward(int32_t dtype, int32_t target_bytes, int64_t 
     if (workspace_bytes < fishing_cross_entropy_workspace(dtype, rows, levels, dim, 1)) return FISHING_ERR_SIZE;
     hipStream_t st = (hipStream_t)stream;
     if (rows == 0) {
-        const dim3 grid((unsigned)ceil_div(levels * dim, 256));
+        const int64_t blocks = ceil_div(levels * dim, 256);
+        const dim3 grid((unsigned)(blocks < 65536 ? blocks : 65536));
         return dtype == FISHING_DTYPE_F32 ? launch(zero_kernel<float>, grid, dim3(256), st, (float*)dhead, levels * dim)
                                           : launch(zero_kernel<bf16>, grid, dim3(256), st, (bf16*)dhead, levels * dim);
     }

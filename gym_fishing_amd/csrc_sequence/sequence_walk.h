@@ -13,8 +13,15 @@ struct Strided {
     int64_t batch, step, head;
 };
 
-// exp(-inf * 0) would be NaN: a decay of zero is carried as a logarithm far below float32's range
-__device__ __forceinline__ float log_decay_of(const float* log_decay, int h) { return fmaxf(log_decay[h], -1.0e4f); }
+// exp(-inf * 0) would be NaN: a decay of zero is carried as a logarithm far below float32's range (and NaN stays NaN)
+__device__ __forceinline__ float log_decay_of(const float* log_decay, int h) { return log_decay[h] < -1.0e4f ? -1.0e4f : log_decay[h]; }
+
+// Batches are walked in blocks whose launches' threads count in 32 bits: 2^22 (batch, head) pairs, four 64-lane waves each at most
+constexpr int kMaxHeads = 65536;
+static int64_t batch_block(int64_t batch, int heads) {
+    const int64_t most = ((int64_t)1 << 22) / heads;
+    return batch < most ? batch : most;
+}
 
 // ---- whole episodes, a chunk of 32 (f32: 16) steps at a time: one wave owns a (batch, head), up to 64 columns of its state, and a run of steps ----
 //
@@ -631,19 +638,20 @@ static WalkWork walk_work(const WalkPlan& p, int64_t pairs, void* at) {
 template <typename T, bool BACK>
 int walk(const FishingDecayAttention* f, Strided q, Strided k, Strided v, const float* state, float* state_out, Strided out, int dk, int dv, bool state_t, bool exact_state,
                 double read_scale, double write_scale, void* workspace, hipStream_t stream) {
-    const int64_t pairs = f->batch * f->heads;
     if (f->steps <= 1) q.step = k.step = v.step = out.step = kMaxHeadDim;         // (a single step has no next one: any stride will do)
     constexpr int V = vec_of<T>();
     auto wide = [&](const Strided& s, int d) {
         return d % V == 0 && aligned16(s.p) && s.batch % V == 0 && s.step % V == 0 && s.head % V == 0 && s.step >= d && s.step < (int64_t)1 << 24;
     };
     const bool vec = wide(q, dk) && wide(k, dk) && wide(v, dv) && wide(out, dv) && f->starts_stride[1] < (int64_t)1 << 24;
-    const WalkPlan p = walk_plan(pairs, f->steps, dk, dv, vec);
-    const WalkWork w = walk_work(p, pairs, workspace);
-    const ChunkArgs a{q, k, v, out, f->log_decay, f->starts, f->starts_stride[0], f->starts_stride[1], state, state_out, f->steps, f->heads, dk, dv, state_t, exact_state,
+    const int64_t block = batch_block(f->batch, f->heads);
+    const WalkPlan p = walk_plan(block * f->heads, f->steps, dk, dv, vec);
+    const WalkWork w = walk_work(p, block * f->heads, workspace);
+    ChunkArgs a{q, k, v, out, f->log_decay, f->starts, f->starts_stride[0], f->starts_stride[1], state, state_out, f->steps, f->heads, dk, dv, state_t, exact_state,
                       (float)read_scale, (float)write_scale, p.slices, p.segs, p.seg_steps, w.carry, w.through, w.odd};
-    const dim3 grid((unsigned)(pairs * p.slices * p.segs));
+    int64_t pairs = 0;
     auto run = [&](auto tk, auto tv, auto rows) {
+        const dim3 grid((unsigned)(pairs * p.slices * p.segs));
         constexpr int NK = decltype(tk)::value, NV = decltype(tv)::value;
         constexpr bool VEC = decltype(rows)::value;
         int rc = 0;
@@ -657,10 +665,20 @@ int walk(const FishingDecayAttention* f, Strided q, Strided k, Strided v, const 
     auto tiles = [&](auto tv, auto rows) {
         return p.nk == 2 ? run(Count<2>{}, tv, rows) : p.nk == 4 ? run(Count<4>{}, tv, rows) : p.nk == 6 ? run(Count<6>{}, tv, rows) : run(Count<8>{}, tv, rows);
     };
-    const int rc = !vec ? tiles(Count<2>{}, std::false_type{}) : p.nv == 2 ? tiles(Count<2>{}, std::true_type{}) : tiles(Count<4>{}, std::true_type{});
-    if (rc) return rc;
-    const int64_t groups = ceil_div(pairs, kOddGroup);
-    return launch(odd_kernel<T, BACK>, dim3((unsigned)(groups < 1024 ? groups : 1024)), dim3(256), stream, a, pairs);
+    int rc = 0;
+    for (int64_t n = 0; n < f->batch && !rc; n += block) {
+        pairs = (f->batch - n < block ? f->batch - n : block) * f->heads;
+        rc = !vec ? tiles(Count<2>{}, std::false_type{}) : p.nv == 2 ? tiles(Count<2>{}, std::true_type{}) : tiles(Count<4>{}, std::true_type{});
+        if (rc) break;
+        const int64_t groups = ceil_div(pairs, kOddGroup);
+        rc = launch(odd_kernel<T, BACK>, dim3((unsigned)(groups < 1024 ? groups : 1024)), dim3(256), stream, a, pairs);
+        // the next block's corners
+        for (Strided* s : {&a.q, &a.k, &a.v, &a.out}) s->p = (const T*)s->p + block * s->batch;
+        if (a.starts) a.starts += block * a.starts_batch;
+        if (a.state) a.state += block * f->heads * dk * dv;
+        if (a.state_out) a.state_out += block * f->heads * dk * dv;
+    }
+    return rc;
 }
 
 }  // namespace seq

@@ -27,7 +27,7 @@ from torch.autograd.function import once_differentiable
 from . import _capi
 from ._capi import DTYPE_BF16, DTYPE_F32, FishingDecayAttention, FishingLibraryError
 
-MAX_HEAD_DIM = 128
+MAX_HEAD_DIM, MAX_HEADS = 128, 65536
 _DTYPES = {torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16}
 _RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
@@ -214,8 +214,8 @@ def _check_heads(q, k, v, log_decay, state, dims):
     heads, dk, dv = q.shape[-2], q.shape[-1], v.shape[-1]
     if not (1 <= dk <= MAX_HEAD_DIM and 1 <= dv <= MAX_HEAD_DIM):
         raise ValueError("head dimensions must be in 1 .. %d, got q, k: %d and v: %d" % (MAX_HEAD_DIM, dk, dv))
-    if heads < 1:
-        raise ValueError("at least one head is needed")
+    if not 1 <= heads <= MAX_HEADS:
+        raise ValueError("1 .. %d heads are needed, got %d" % (MAX_HEADS, heads))
     _tensor(log_decay, "log_decay", 1, (torch.float32,), dev)
     if log_decay.shape[0] != heads:
         raise ValueError("log_decay must hold one value for each of %d heads, got %d" % (heads, log_decay.shape[0]))
@@ -315,6 +315,10 @@ def decay_attention_step(q, k, v, log_decay, state, starts=None, scale=None, out
         a.starts = starts.data_ptr()
         a.starts_stride[0] = starts.stride(0)
     _call(_capi.lib().fishing_decay_attention_step, dev, ctypes.byref(a))
+    # written behind torch's back: a recorded graph that saved them has to notice
+    for x in (state_out, out):
+        if not x.is_inference():
+            torch.autograd.graph.increment_version(x)
     return out
 
 

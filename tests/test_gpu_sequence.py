@@ -465,3 +465,110 @@ def test_captured_and_replayed_between_eager_work():
         assert torch.equal(out, eager) and torch.equal(moving, want_state)
         for w, o in zip(worlds, outs):
             assert all(torch.equal(x, y) for x, y in zip(o, train(*w)))
+
+
+# ---- calls that take more than one launch's block, and what else sizes and strides do ----
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("rows,levels,dim", [((1 << 21) + 300, 5, 8), (65536 + 100, 20000, 8)])
+def test_cross_entropy_over_blocks_of_rows(rows, levels, dim, dtype):
+    """The weights are zero but for some rows of each block, whose gradients are then the whole of the head's."""
+    at = torch.cat([torch.arange(0, 40), torch.arange(rows // 2, rows // 2 + 40), torch.arange(rows - 140, rows - 60), torch.arange(rows - 40, rows)]).cuda()
+    hidden, head = rand(rows, dim, seed=1, dtype=dtype).requires_grad_(), rand(levels, dim, seed=2, dtype=dtype, scale=0.5).requires_grad_()
+    target = torch.randint(0, levels, (rows,), generator=torch.Generator().manual_seed(3)).to(torch.int32).cuda()
+    target[at[1]], target[at[-1]] = -1, levels
+    grad = torch.zeros(rows, device="cuda")
+    grad[at] = rand(len(at), seed=4)
+    loss = sequence.cross_entropy(hidden, head, target)
+    dhidden, dhead = torch.autograd.grad(loss, (hidden, head), grad)
+    want, bound = ref.loss(hidden.detach()[at], head, target[at], grad[at])
+    ref.check(loss[at], want["loss"], bound["loss"], "loss")
+    ref.check(dhidden[at], want["dhidden"], bound["dhidden"], "dhidden")
+    ref.check(dhead, want["dhead"], bound["dhead"], "dhead")
+    others = torch.ones(rows, dtype=torch.bool, device="cuda")
+    others[at] = False
+    assert not dhidden[others].any()
+
+
+def test_cross_entropy_rows_far_apart():
+    """300 rows 16 MiB from each other: more than a tile's offsets reach."""
+    rows, levels, dim, far = 300, 70, 64, (1 << 22) + 64
+    pool = torch.empty(rows * far, device="cuda")
+    hidden, head = pool.as_strided((rows, dim), (far, 1)), pool.as_strided((levels, dim), (far, 1), 4096)
+    hidden.copy_(rand(rows, dim, seed=1))
+    head.copy_(rand(levels, dim, seed=2))
+    target = torch.arange(rows, device="cuda") % levels
+    leaves = [x.detach().requires_grad_() for x in (hidden, head)]
+    near = [x.detach().contiguous().requires_grad_() for x in (hidden, head)]
+    assert leaves[0].stride(0) == far
+    loss, want = sequence.cross_entropy(*leaves, target), sequence.cross_entropy(*near, target)
+    assert torch.equal(loss, want)
+    assert all(torch.equal(x, y) for x, y in zip(torch.autograd.grad(loss.sum(), leaves), torch.autograd.grad(want.sum(), near)))
+
+
+def test_attention_over_blocks_of_the_batch():
+    batch, steps, heads, d = (1 << 21) + 3, 2, 2, 4
+    g = torch.Generator(device="cuda").manual_seed(1)
+    q, k, v, go = (torch.randn((batch, steps, heads, d), generator=g, device="cuda") for _ in range(4))
+    s0, gs = (torch.randn((batch, heads, d, d), generator=g, device="cuda") for _ in range(2))
+    cut = torch.rand((batch, steps), generator=g, device="cuda") < 0.3
+    ld = torch.tensor([-0.3, -0.01], device="cuda")
+    at = torch.cat([torch.arange(0, 9), torch.arange(batch - 9, batch)]).cuda()
+    leaves = [x.requires_grad_() for x in (q, k, v, s0)]
+    got = sequence.decay_attention(q, k, v, ld, starts=cut, state=s0, scale=0.5, return_state=True)
+    got = list(got) + list(torch.autograd.grad(got, leaves, [go, gs]))
+    args = (q[at], k[at], v[at], ld, cut[at], s0[at], 0.5, go[at], gs[at])
+    want, bound = ref.attention(*args), ref.attention_bounds(*args)
+    for name, x in zip(("out", "state", "dq", "dk", "dv", "dstate"), got):
+        ref.check(x[at], want[name], bound[name], name)
+    with torch.no_grad():
+        state = s0.clone()
+        for t in range(steps):
+            out = sequence.decay_attention_step(q[:, t], k[:, t], v[:, t], ld, state, starts=cut[:, t], scale=0.5)
+            ref.check(out[at], want["out"][:, t], bound["out"][:, t], "step %d" % t)
+    ref.check(state[at], want["state"], bound["state"], "state")
+    assert torch.isfinite(out).all() and torch.isfinite(state).all()
+
+
+def test_embedding_over_blocks_of_rows_and_a_wide_vocabulary():
+    n = (1 << 24) + 50                                     # 257 columns are read one by one, four rows a workgroup
+    table = rand(3, 257, seed=1, dtype=torch.bfloat16)
+    tokens = (torch.arange(n, device="cuda") % 4 - 1).to(torch.int32)
+    out = sequence.embedding(tokens, table)
+    for at in (slice(0, 60), slice((1 << 24) - 30, (1 << 24) + 30), slice(n - 20, n)):
+        there = (tokens[at] >= 0).unsqueeze(1)
+        assert torch.equal(out[at], torch.where(there, table[tokens[at].long().clamp(min=0)], torch.zeros((), dtype=torch.bfloat16, device="cuda")))
+    del out
+    vocab = (1 << 22) + 9
+    wide = torch.zeros((vocab, 1), device="cuda", requires_grad=True)
+    met = torch.tensor([0, 5, vocab - 1, 5, vocab - 2, 1 << 22], device="cuda")
+    got = torch.autograd.grad(sequence.embedding(met, wide), wide, torch.arange(1.0, 7.0, device="cuda").unsqueeze(1))[0]
+    want = torch.zeros((vocab, 1), device="cuda")
+    want[met] = torch.tensor([1.0, 6.0, 3.0, 6.0, 5.0, 6.0], device="cuda").unsqueeze(1)
+    assert torch.equal(got, want)
+
+
+def test_the_step_counts_as_a_write():
+    """A recorded graph that saved the state refuses to go back once the step has moved it on."""
+    q, k, v = (rand(2, 1, 8, seed=i) for i in range(3))
+    ld, state, out = torch.tensor([-0.1], device="cuda"), rand(2, 1, 8, 8, seed=4), torch.empty((2, 1, 8), device="cuda")
+    for target in (state, out):
+        w = torch.ones((), device="cuda", requires_grad=True)
+        y = (target * w).sum()
+        with torch.no_grad():
+            sequence.decay_attention_step(q, k, v, ld, state, out=out)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    with torch.inference_mode():
+        s = state.clone()
+        sequence.decay_attention_step(q, k, v, ld, s)
+
+
+def test_a_decay_that_is_not_a_number():
+    q, k, v = (rand(1, 40, 2, 16, seed=i) for i in range(3))
+    ld = torch.tensor([float("nan"), -0.1], device="cuda")
+    out = sequence.decay_attention(q, k, v, ld)
+    assert torch.isnan(out[:, 1:, 0]).all()
+    assert torch.equal(out[:, :, 1], sequence.decay_attention(q, k, v, torch.tensor([-0.1, -0.1], device="cuda"))[:, :, 1])
+    state = torch.ones((1, 2, 16, 16), device="cuda")
+    assert torch.isnan(sequence.decay_attention_step(q[:, 0], k[:, 0], v[:, 0], ld, state)[:, 0]).all()

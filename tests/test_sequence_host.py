@@ -108,3 +108,21 @@ def test_the_struct_is_the_headers(tmp_path):
     subprocess.run(["gcc", "-std=c99", "-I", os.path.join(ROOT, "include"), str(src), "-o", str(exe)], check=True)
     got = [int(x) for x in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split()]
     assert got == [ctypes.sizeof(_capi.FishingDecayAttention)] + [getattr(_capi.FishingDecayAttention, n).offset for n in names]
+
+
+def test_large_calls_have_a_plan_that_fits(lib):
+    """Rows and batches are walked in blocks: workspaces stop growing with them, and what no launch could count is refused."""
+    work = lib.fishing_cross_entropy_workspace
+    for d, size in ((0, 4), (1, 2)):
+        for levels, dim in ((5, 8), (100, 128), (20000, 8), (32771, 1024), (3, 65536)):
+            assert work(d, 1 << 23, levels, dim, 1) == work(d, 1 << 30, levels, dim, 1) < 40 << 30
+            assert work(d, 1 << 23, levels, dim, 0) == work(d, 1 << 30, levels, dim, 0) < 12 << 30
+    assert work(0, 4, 1 << 26, 1024, 0) == -4 and work(1, 4, 1 << 26, 1024, 1) == -4
+    a = _capi.FishingDecayAttention()
+    a.heads, a.dk, a.dv, a.steps, a.batch, a.log_decay = 2, 4, 4, 2, 1 << 21, 64
+    a.q = a.k = a.v = 64
+    need = lib.fishing_decay_attention_workspace(a, 1)
+    a.batch = 1 << 29
+    assert lib.fishing_decay_attention_workspace(a, 1) == need < 1 << 28
+    a.heads, a.batch = 65537, 1
+    assert lib.fishing_decay_attention_workspace(a, 0) == -4 and lib.fishing_decay_attention_step(a, None) == -4
