@@ -200,7 +200,7 @@ struct ChunkArgs {
     float read_scale, write_scale;
     int32_t slices, segs;
     int64_t seg_steps;
-    float *carry, *through;    // per (pair, slice, segment): the state behind it in lane order, and what it lets through
+    float *carry, *through;    // the state behind a segment, per (pair, 16 columns, segment) in lane order, and what a segment lets through, per (pair, segment)
     uint32_t* odd;             // per (pair, slice, segment): some result is infinite or NaN
 };
 
@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(64, (NK * NV >= 24 ? 1 : 2)) chunk_kernel(Chun
     const int rest = (int)id - (int)pair * (int)units, slice = uniform((int)((uint32_t)rest / (uint32_t)a.segs)), seg = rest - slice * a.segs;
     if (LOCAL && seg == a.segs - 1) return;                  // nothing follows it
     const int64_t n = uniform((int)((uint32_t)pair / (uint32_t)a.heads)), h = pair - n * a.heads;
-    const int col0 = slice * NV * 16, cols = a.dv - col0;
+    const int col0 = slice * NV * 16, cols = a.dv - col0, col_tiles = (a.dv + 15) / 16;
     const T* qp = (const T*)a.q.p + n * a.q.batch + h * a.q.head;
     const T* kp = (const T*)a.k.p + n * a.k.batch + h * a.k.head;
     const T* vp = (const T*)a.v.p + n * a.v.batch + h * a.v.head + col0;
@@ -271,7 +271,7 @@ __global__ void __launch_bounds__(64, (NK * NV >= 24 ? 1 : 2)) chunk_kernel(Chun
 
     f32x4 S[NK][NV];
     {
-        float* from = a.carry + (id - 1) * (NK * NV * 256);
+        const float* from = a.carry + ((pair * col_tiles + col0 / 16) * a.segs + seg - 1) * (NK * 256);
         const float* s0 = a.state ? a.state + pair * (int64_t)a.dk * a.dv : nullptr;
 #pragma unroll
         for (int c = 0; c < NK; ++c)
@@ -279,7 +279,7 @@ __global__ void __launch_bounds__(64, (NK * NV >= 24 ? 1 : 2)) chunk_kernel(Chun
             for (int m = 0; m < NV; ++m) {
                 S[c][m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
                 if (seg > 0) {
-                    if (!LOCAL) S[c][m] = *(const f32x4*)(from + (c * NV + m) * 256 + lane * 4);
+                    if (!LOCAL && col0 / 16 + m < col_tiles) S[c][m] = *(const f32x4*)(from + (m * a.segs * NK + c) * 256 + lane * 4);
                 } else if (s0) {
                     const int col = m * 16 + i, row = L::state_row(c, g);
 #pragma unroll
@@ -464,12 +464,13 @@ __global__ void __launch_bounds__(64, (NK * NV >= 24 ? 1 : 2)) chunk_kernel(Chun
     }
 
     if (LOCAL) {
-        float* to = a.carry + id * (NK * NV * 256);
+        float* to = a.carry + ((pair * col_tiles + col0 / 16) * a.segs + seg) * (NK * 256);
 #pragma unroll
         for (int c = 0; c < NK; ++c)
 #pragma unroll
-            for (int m = 0; m < NV; ++m) *(f32x4*)(to + (c * NV + m) * 256 + lane * 4) = S[c][m];
-        if (lane == 0) a.through[id] = through;
+            for (int m = 0; m < NV; ++m)
+                if (col0 / 16 + m < col_tiles) *(f32x4*)(to + (m * a.segs * NK + c) * 256 + lane * 4) = S[c][m];
+        if (lane == 0 && slice == 0) a.through[pair * a.segs + seg] = through;
         return;
     }
     if (a.state_out && seg == a.segs - 1) {
@@ -495,19 +496,31 @@ __global__ void __launch_bounds__(64, (NK * NV >= 24 ? 1 : 2)) chunk_kernel(Chun
 }
 
 // the states behind a pair's segments, chained: carry[s] = through[s] carry[s - 1] + carry[s]
-static __global__ void __launch_bounds__(256) chain_kernel(float* carry, const float* through, int32_t segs, int32_t per) {
+static __global__ void __launch_bounds__(256) chain_kernel(float* carry, const float* through, int32_t segs, int32_t per, int32_t col_tiles) {
     const int64_t group = blockIdx.y;
     const int at = blockIdx.x * 256 + threadIdx.x;
     if (at >= per) return;
     float* c = carry + group * segs * per + at;
-    const float* p = through + group * segs;
+    const float* p = through + group / col_tiles * segs;
     float s = c[0];
-#pragma unroll 8
-    for (int x = 1; x < segs - 1; ++x) {
-        const float f = p[x];
-        s = (f == 0.0f ? 0.0f : f * s) + c[(int64_t)x * per];
-        c[(int64_t)x * per] = s;
-    }
+    int x = 1;
+    auto batch = [&](auto n) {                  // loads sent together: behind a store to the same array the compiler sends none ahead
+        constexpr int U = decltype(n)::value;
+        for (; x + U <= segs - 1; x += U) {
+            float next[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) next[u] = c[(int64_t)(x + u) * per];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const float f = p[x + u];
+                s = (f == 0.0f ? 0.0f : f * s) + next[u];
+                c[(int64_t)(x + u) * per] = s;
+            }
+        }
+    };
+    batch(std::integral_constant<int, 16>{});
+    batch(std::integral_constant<int, 4>{});
+    batch(std::integral_constant<int, 1>{});
 }
 
 // ---- the recurrence itself, one step after the other, for pairs whose results are not all finite numbers: a product's masked terms
@@ -581,9 +594,13 @@ __global__ void __launch_bounds__(256) odd_kernel(ChunkArgs a, int64_t pairs) {
         const int here = pairs - p0 < kOddGroup ? (int)(pairs - p0) : kOddGroup;
         if (threadIdx.x < kOddGroup) odd[threadIdx.x] = 0;
         __syncthreads();
+        bool any = false;
         for (int x = threadIdx.x; x < here * per; x += 256)
-            if (a.odd[p0 * per + x]) odd[x / per] = 1;
-        __syncthreads();
+            if (a.odd[p0 * per + x]) {
+                odd[x / per] = 1;
+                any = true;
+            }
+        if (!__syncthreads_or(any)) continue;
         for (int x = 0; x < here; ++x) {
             if (!odd[x]) continue;
             for (int col = 0; col < a.dv; col += 32) recurrent<T, BACK>(a, p0 + x, col, row);
@@ -595,7 +612,7 @@ __global__ void __launch_bounds__(256) odd_kernel(ChunkArgs a, int64_t pairs) {
 // How a walk over (batch, heads) pairs is cut: column slices of the state, and, where there are few waves and many steps, segments of
 // the steps, whose states are computed first (from k and v alone) and chained.
 struct WalkPlan {
-    int nk, nv, slices, segs;
+    int nk, nv, slices, segs;                // tiles of 16 rows and of 16 columns a wave
     int64_t seg_steps;
 };
 
@@ -605,7 +622,7 @@ static WalkPlan walk_plan(int64_t pairs, int64_t steps, int dk, int dv, bool wid
     p.nv = dv <= 32 || !wide ? 2 : 4;            // (rows that are not whole 16-byte accesses: one width is enough)
     p.slices = (int)ceil_div(dv, p.nv * 16);
     // 1024 SIMDs, two waves each; a segment costs a state written, read, chained and read, so it is at least 256 steps long
-    const int64_t waves = pairs * p.slices, want = waves > 0 ? 2048 / waves : 1, most = steps / 256;
+    const int64_t waves = pairs * p.slices, want = waves > 0 ? (p.nk * p.nv >= 24 ? 1024 : 2048) / waves : 1, most = steps / 256;
     int64_t segs = want < most ? want : most;
     if (segs < 2) segs = 1;
     p.seg_steps = segs > 1 ? round_up(ceil_div(steps, segs), 32) : (steps > 0 ? steps : 1);
@@ -622,14 +639,13 @@ struct WalkWork {
     int64_t bytes;
 };
 
-static WalkWork walk_work(const WalkPlan& p, int64_t pairs, void* at) {
+static WalkWork walk_work(const WalkPlan& p, int64_t pairs, int dv, void* at) {
     Carve c(at);
     WalkWork w{};
-    const int64_t units = pairs * p.slices * p.segs;
-    w.odd = c.take<uint32_t>(units);
+    w.odd = c.take<uint32_t>(pairs * p.slices * p.segs);
     if (p.segs > 1) {
-        w.through = c.take<float>(units);
-        w.carry = c.take<float>(units * p.nk * p.nv * 256);
+        w.through = c.take<float>(pairs * p.segs);
+        w.carry = c.take<float>(pairs * ceil_div(dv, 16) * p.segs * p.nk * 256);
     }
     w.bytes = c.used + 256;
     return w;
@@ -646,7 +662,7 @@ int walk(const FishingDecayAttention* f, Strided q, Strided k, Strided v, const 
     const bool vec = wide(q, dk) && wide(k, dk) && wide(v, dv) && wide(out, dv) && f->starts_stride[1] < (int64_t)1 << 24;
     const int64_t block = batch_block(f->batch, f->heads);
     const WalkPlan p = walk_plan(block * f->heads, f->steps, dk, dv, vec);
-    const WalkWork w = walk_work(p, block * f->heads, workspace);
+    const WalkWork w = walk_work(p, block * f->heads, dv, workspace);
     ChunkArgs a{q, k, v, out, f->log_decay, f->starts, f->starts_stride[0], f->starts_stride[1], state, state_out, f->steps, f->heads, dk, dv, state_t, exact_state,
                       (float)read_scale, (float)write_scale, p.slices, p.segs, p.seg_steps, w.carry, w.through, w.odd};
     int64_t pairs = 0;
@@ -656,9 +672,13 @@ int walk(const FishingDecayAttention* f, Strided q, Strided k, Strided v, const 
         constexpr bool VEC = decltype(rows)::value;
         int rc = 0;
         if (p.segs > 1) {
-            rc = launch(chunk_kernel<T, NK, NV, BACK, VEC, true>, grid, dim3(64), stream, a);
-            const int per = NK * NV * 256;
-            if (!rc) rc = launch(chain_kernel, dim3((unsigned)ceil_div(per, 256), (unsigned)(pairs * p.slices)), dim3(256), stream, w.carry, w.through, p.segs, per);
+            // without outputs narrow slices fit two waves on a SIMD (16381 steps, 8 heads of 128 x 128: 26 us, with 4 tiles 44)
+            constexpr int LV = NK >= 6 ? 2 : NV;
+            const int per = NK * 256, col_tiles = (int)ceil_div(dv, 16);
+            ChunkArgs local = a;
+            local.slices = (int)ceil_div(dv, LV * 16);
+            rc = launch(chunk_kernel<T, NK, LV, BACK, VEC, true>, dim3((unsigned)(pairs * local.slices * p.segs)), dim3(64), stream, local);
+            if (!rc) rc = launch(chain_kernel, dim3((unsigned)ceil_div(per, 256), (unsigned)(pairs * col_tiles)), dim3(256), stream, w.carry, w.through, p.segs, per, col_tiles);
         }
         return rc ? rc : launch(chunk_kernel<T, NK, NV, BACK, VEC, false>, grid, dim3(64), stream, a);
     };
