@@ -161,7 +161,7 @@ int64_t fishing_decay_attention_workspace(const FishingDecayAttention* a, int32_
     int64_t most = 0;
     for (int back = 0; back <= (backward ? 1 : 0); ++back)
         for (int wide = 0; wide < 2; ++wide) {
-            const int64_t b = walk_work(walk_plan(pairs, a->steps, back ? a->dv : a->dk, back ? a->dk : a->dv, wide != 0), pairs, back ? a->dk : a->dv, nullptr).bytes;
+            const int64_t b = walk_work(walk_plan(a->dtype, pairs, a->steps, back ? a->dv : a->dk, back ? a->dk : a->dv, wide != 0), pairs, back ? a->dk : a->dv, nullptr).bytes;
             most = b > most ? b : most;
         }
     return most;

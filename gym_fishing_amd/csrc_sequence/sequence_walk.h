@@ -118,6 +118,7 @@ struct Lanes<float> {
         a = *(const Quad*)(rows + y * pitch + (32 * c + 4 * g) * 4);
         b = *(const Quad*)(rows + y * pitch + (32 * c + 16 + 4 * g) * 4);
     }
+    static __device__ __forceinline__ Quad row_quad(const char* rows, int pitch, int y, int c) { return *(const Quad*)(rows + y * pitch + (16 * c + 4 * (threadIdx.x >> 4 & 3)) * 4); }
     static __device__ __forceinline__ int state_row(int c, int g) { return 16 * c + 4 * g; }
     static __device__ __forceinline__ f32x4 mma(Quad a0, Quad a1, Quad b0, Quad b1, f32x4 acc) {
 #pragma unroll
@@ -222,9 +223,15 @@ __device__ __forceinline__ void store_quad(R rows, uint32_t at, int further, f32
     __builtin_amdgcn_raw_buffer_store_b128(y.u, rows, at, further, 0);
 }
 
+// Waves on a SIMD, by the registers that state, rows in flight and operands take: two where nothing spills, else one
+constexpr int waves_a_simd(int nk, int nv, bool vec, bool local) {
+    return local ? (nk * nv >= 24 ? 1 : 2) : nk * nv > 16 || nk == 8 || (!vec && nk >= 6) ? 1 : 2;
+}
+
 // LOCAL: only the state that a segment adds (from zero; the first from the state carried in), for the segments to be chained.
 template <typename T, int NK, int NV, bool BACK, bool VEC, bool LOCAL>
-__global__ void __launch_bounds__(64, (NK * NV >= 24 ? 1 : 2)) chunk_kernel(ChunkArgs a) {
+__global__ void __launch_bounds__(64, waves_a_simd(NK, NV, VEC, LOCAL)) chunk_kernel(ChunkArgs a) {
+    static_assert(sizeof(T) == 4 || NK % 2 == 0, "bf16 rows are multiplied 32 elements at a time");
     typedef Lanes<T> L;
     typedef typename L::Quad Quad;
     constexpr int TS = L::TILES, CH = 16 * TS;
@@ -357,18 +364,21 @@ __global__ void __launch_bounds__(64, (NK * NV >= 24 ? 1 : 2)) chunk_kernel(Chun
             for (int t = 0; t < TS; ++t)
 #pragma unroll
                 for (int c = 0; c < NK / 2; ++c) L::row_quads(qs, RK::PITCH, 16 * t + i, c, q[t][2 * c], q[t][2 * c + 1]);
+            if constexpr (NK & 1) q[0][NK - 1] = L::row_quad(qs, RK::PITCH, i, NK - 1);
 #pragma unroll
             for (int ky = 0; ky < TS; ++ky) {
                 __builtin_amdgcn_sched_barrier(0);
                 Quad k[NK];
 #pragma unroll
                 for (int c = 0; c < NK / 2; ++c) L::row_quads(ks, RK::PITCH, 16 * ky + i, c, k[2 * c], k[2 * c + 1]);
+                if constexpr (NK & 1) k[NK - 1] = L::row_quad(ks, RK::PITCH, i, NK - 1);
 #pragma unroll
                 for (int t = 0; t < TS; ++t) {
                     f32x4 z = {0.0f, 0.0f, 0.0f, 0.0f};
                     if (BACK ? t <= ky : t >= ky) {        // (else no pair of these tiles is in order)
 #pragma unroll
-                        for (int c = 0; c < NK; c += 2) z = L::mma(k[c], k[c + 1], q[t][c], q[t][c + 1], z);
+                        for (int c = 0; c < NK - 1; c += 2) z = L::mma(k[c], k[c + 1], q[t][c], q[t][c + 1], z);
+                        if constexpr (NK & 1) z = L::over_steps({k[NK - 1]}, {q[t][NK - 1]}, z);
                         z *= near_of[BACK ? ky - t : t - ky][lane];
                         if (st) {
                             const int g4 = here(4 * g);
@@ -412,12 +422,13 @@ __global__ void __launch_bounds__(64, (NK * NV >= 24 ? 1 : 2)) chunk_kernel(Chun
 #pragma unroll
                 for (int t = 0; t < TS; ++t) o[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int c = 0; c < NK; c += 2) {
+                for (int c = 0; c < NK - 1; c += 2) {
                     const Quad s0 = L::round(S[c][m]), s1 = L::round(S[c + 1][m]);
 #pragma unroll
                     for (int t = 0; t < TS; ++t)
                         o[t] = L::mma(s0, s1, q[t][c], q[t][c + 1], o[t]);
                 }
+                if constexpr (NK & 1) o[0] = L::over_steps({S[NK - 1][m]}, {q[0][NK - 1]}, o[0]);
 #pragma unroll
                 for (int t = 0; t < TS; ++t) {
                     o[t] = L::over_steps(v, p[t], o[t] * into[t]);
@@ -616,13 +627,20 @@ struct WalkPlan {
     int64_t seg_steps;
 };
 
-static WalkPlan walk_plan(int64_t pairs, int64_t steps, int dk, int dv, bool wide) {
+static WalkPlan walk_plan(int32_t dtype, int64_t pairs, int64_t steps, int dk, int dv, bool wide) {
     WalkPlan p;
-    p.nk = dk <= 32 ? 2 : dk <= 64 ? 4 : dk <= 96 ? 6 : 8;
-    p.nv = dv <= 32 || !wide ? 2 : 4;            // (rows that are not whole 16-byte accesses: one width is enough)
+    p.nk = (int)ceil_div(dk, 16);
+    p.nk = p.nk < 2 ? 2 : p.nk == 7 ? 8 : p.nk;
+    if (dtype == FISHING_DTYPE_BF16) p.nk += p.nk & 1;
+    // columns a wave: as many tiles as multiply the least (each slice computes the scores anew; a tile behind dv is work for nothing);
+    // rows that are not whole 16-byte accesses: one width is enough
+    p.nv = 2;
+    auto cost = [&](int nv) { return ceil_div(dv, 16 * nv) * (p.nk + nv * (2 * p.nk + 1)); };
+    for (int nv = 3; nv <= 4 && wide; ++nv)
+        if (cost(nv) <= cost(p.nv)) p.nv = nv;
     p.slices = (int)ceil_div(dv, p.nv * 16);
-    // 1024 SIMDs, two waves each; a segment costs a state written, read, chained and read, so it is at least 256 steps long
-    const int64_t waves = pairs * p.slices, want = waves > 0 ? (p.nk * p.nv >= 24 ? 1024 : 2048) / waves : 1, most = steps / 256;
+    // 1024 SIMDs; a segment costs a state written, read, chained and read, so it is at least 256 steps long
+    const int64_t waves = pairs * p.slices, want = waves > 0 ? 1024 * waves_a_simd(p.nk, p.nv, wide, false) / waves : 1, most = steps / 256;
     int64_t segs = want < most ? want : most;
     if (segs < 2) segs = 1;
     p.seg_steps = segs > 1 ? round_up(ceil_div(steps, segs), 32) : (steps > 0 ? steps : 1);
@@ -661,7 +679,7 @@ int walk(const FishingDecayAttention* f, Strided q, Strided k, Strided v, const 
     };
     const bool vec = wide(q, dk) && wide(k, dk) && wide(v, dv) && wide(out, dv) && f->starts_stride[1] < (int64_t)1 << 24;
     const int64_t block = batch_block(f->batch, f->heads);
-    const WalkPlan p = walk_plan(block * f->heads, f->steps, dk, dv, vec);
+    const WalkPlan p = walk_plan(f->dtype, block * f->heads, f->steps, dk, dv, vec);
     const WalkWork w = walk_work(p, block * f->heads, dv, workspace);
     ChunkArgs a{q, k, v, out, f->log_decay, f->starts, f->starts_stride[0], f->starts_stride[1], state, state_out, f->steps, f->heads, dk, dv, state_t, exact_state,
                       (float)read_scale, (float)write_scale, p.slices, p.segs, p.seg_steps, w.carry, w.through, w.odd};
@@ -673,7 +691,7 @@ int walk(const FishingDecayAttention* f, Strided q, Strided k, Strided v, const 
         int rc = 0;
         if (p.segs > 1) {
             // without outputs narrow slices fit two waves on a SIMD (16381 steps, 8 heads of 128 x 128: 26 us, with 4 tiles 44)
-            constexpr int LV = NK >= 6 ? 2 : NV;
+            constexpr int LV = NK >= 5 ? 2 : NV;
             const int per = NK * 256, col_tiles = (int)ceil_div(dv, 16);
             ChunkArgs local = a;
             local.slices = (int)ceil_div(dv, LV * 16);
@@ -683,12 +701,16 @@ int walk(const FishingDecayAttention* f, Strided q, Strided k, Strided v, const 
         return rc ? rc : launch(chunk_kernel<T, NK, NV, BACK, VEC, false>, grid, dim3(64), stream, a);
     };
     auto tiles = [&](auto tv, auto rows) {
+        if constexpr (sizeof(T) == 4) {
+            if (p.nk == 3) return run(Count<3>{}, tv, rows);
+            if (p.nk == 5) return run(Count<5>{}, tv, rows);
+        }
         return p.nk == 2 ? run(Count<2>{}, tv, rows) : p.nk == 4 ? run(Count<4>{}, tv, rows) : p.nk == 6 ? run(Count<6>{}, tv, rows) : run(Count<8>{}, tv, rows);
     };
     int rc = 0;
     for (int64_t n = 0; n < f->batch && !rc; n += block) {
         pairs = (f->batch - n < block ? f->batch - n : block) * f->heads;
-        rc = !vec ? tiles(Count<2>{}, std::false_type{}) : p.nv == 2 ? tiles(Count<2>{}, std::true_type{}) : tiles(Count<4>{}, std::true_type{});
+        rc = !vec ? tiles(Count<2>{}, std::false_type{}) : p.nv == 2 ? tiles(Count<2>{}, std::true_type{}) : p.nv == 3 ? tiles(Count<3>{}, std::true_type{}) : tiles(Count<4>{}, std::true_type{});
         if (rc) break;
         const int64_t groups = ceil_div(pairs, kOddGroup);
         rc = launch(odd_kernel<T, BACK>, dim3((unsigned)(groups < 1024 ? groups : 1024)), dim3(256), stream, a, pairs);

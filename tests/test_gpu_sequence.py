@@ -572,3 +572,19 @@ def test_a_decay_that_is_not_a_number():
     assert torch.equal(out[:, :, 1], sequence.decay_attention(q, k, v, torch.tensor([-0.1, -0.1], device="cuda"))[:, :, 1])
     state = torch.ones((1, 2, 16, 16), device="cuda")
     assert torch.isnan(sequence.decay_attention_step(q[:, 0], k[:, 0], v[:, 0], ld, state)[:, 0]).all()
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("dk", [24, 40, 48, 72, 80, 96, 112, 128])
+@pytest.mark.parametrize("dv", [8, 40, 48, 80, 96, 104])
+def test_every_count_of_tiles(dk, dv, dtype):
+    """Rows and columns of the state in every number of 16-wide tiles, whole and in segments of the steps, with everything at once."""
+    for batch, steps, seed in ((2, 70, dk + dv), (1, 515, dk * dv)):
+        q, k, v, ld, cut, s0, g, gs = make(batch, steps, 2, dk, dv, dtype, batch == 2, 0.03, True, seed=seed)
+        leaves = [x.detach().requires_grad_() for x in (q, k, v, s0)]
+        got = sequence.decay_attention(*leaves[:3], ld, starts=cut, state=leaves[3], scale=0.3, return_state=True)
+        grads = torch.autograd.grad(got, leaves, [g, gs])
+        args = (q, k, v, ld, cut, s0, 0.3, g, gs)
+        want, bound = ref.attention(*args), ref.attention_bounds(*args)
+        for name, x in zip(("out", "state", "dq", "dk", "dv", "dstate"), list(got) + list(grads)):
+            ref.check(x, want[name], bound[name], name)
