@@ -639,8 +639,12 @@ static WalkPlan walk_plan(int32_t dtype, int64_t pairs, int64_t steps, int dk, i
     for (int nv = 3; nv <= 4 && wide; ++nv)
         if (cost(nv) <= cost(p.nv)) p.nv = nv;
     p.slices = (int)ceil_div(dv, p.nv * 16);
-    // 1024 SIMDs; a segment costs a state written, read, chained and read, so it is at least 256 steps long
-    const int64_t waves = pairs * p.slices, want = waves > 0 ? 1024 * waves_a_simd(p.nk, p.nv, wide, false) / waves : 1, most = steps / 256;
+    // Segments: as many waves as 1024 SIMDs hold (three each of the small states), of at least 8 chunks each, for a segment costs a
+    // state written, read, chained and read.  (97 x 1009 steps, 3 heads of 48 x 80, f32, with gradients: at least 16 chunks and two
+    // waves 666 us, 8 and three 527, 6 and four 565.)
+    const bool f32 = dtype == FISHING_DTYPE_F32;
+    const int64_t waves = pairs * p.slices, each = p.nk * p.nv <= (f32 ? 9 : 6) ? 3 : waves_a_simd(p.nk, p.nv, wide, false);
+    const int64_t want = waves > 0 ? 1024 * each / waves : 1, most = steps / (f32 ? 128 : 256);
     int64_t segs = want < most ? want : most;
     if (segs < 2) segs = 1;
     p.seg_steps = segs > 1 ? round_up(ceil_div(steps, segs), 32) : (steps > 0 ? steps : 1);
