@@ -258,6 +258,32 @@ __global__ void __launch_bounds__(64, waves_a_simd(NK, NV, VEC, LOCAL)) chunk_ke
     const float ld = __int_as_float(uniform(__float_as_int(log_decay_of(a.log_decay, (int)h)))), l2 = ld * 1.4426950408889634f;
     const float whole = __int_as_float(uniform(__float_as_int((float)exp((double)ld * CH))));     // the factor that compounds: rounded once
 
+    RK rq, rk;
+    RV rv;
+    rq.init(a.q.step, a.dk);
+    rk.init(a.k.step, a.dk);
+    rv.init(a.v.step, cols);
+    const uint32_t starts_at = (uint32_t)lane * (uint32_t)a.starts_step;
+    uint32_t started = 0;                         // the lane's step begins an episode (tested behind the wait for the rows)
+    auto front = [&](int x) { return t_lo + (int64_t)(BACK ? chunks - 1 - x : x) * CH; };
+    auto count = [&](int64_t t0) { return t_hi - t0 < CH ? (int)(t_hi - t0) : CH; };
+    auto fetch = [&](int x) {
+        const int64_t t0 = front(x);
+        const int rows = count(t0);
+        if (!LOCAL) rq.load(qp + t0 * a.q.step, a.q.step, rows, a.dk);
+        rk.load(kp + t0 * a.k.step, a.k.step, rows, a.dk);
+        rv.load(vp + t0 * a.v.step, a.v.step, rows, cols);
+        if (a.starts) {
+            const uint8_t* from = a.starts + n * a.starts_batch + t0 * a.starts_step;
+            if constexpr (VEC)
+                started = __builtin_amdgcn_raw_buffer_load_b8(__builtin_amdgcn_make_buffer_rsrc((void*)from, 0, (uint32_t)(rows - 1) * (uint32_t)a.starts_step + 1, 0x00020000),
+                                                              starts_at, 0, 0);
+            else
+                started = from[(lane < rows ? lane : 0) * a.starts_step];
+        }
+    };
+    if (chunks > 0) fetch(0);                     // (on their way while the weights are computed)
+
     // What a whole chunk without a start weighs its terms with, per lane: a score of steps d apart, in order, in tiles t apart; a step's
     // k v^T behind the chunk; the state in front of the chunk at a step.  In LDS: the registers are the rows' in flight.
     __shared__ f32x4 near_of[TS][64], behind_of[TS][64];
@@ -296,32 +322,7 @@ __global__ void __launch_bounds__(64, waves_a_simd(NK, NV, VEC, LOCAL)) chunk_ke
             }
     }
 
-    RK rq, rk;
-    RV rv;
-    rq.init(a.q.step, a.dk);
-    rk.init(a.k.step, a.dk);
-    rv.init(a.v.step, cols);
-    const uint32_t starts_at = (uint32_t)lane * (uint32_t)a.starts_step;
-    uint32_t started = 0;                         // the lane's step begins an episode (tested behind the wait for the rows)
-    auto front = [&](int x) { return t_lo + (int64_t)(BACK ? chunks - 1 - x : x) * CH; };
-    auto count = [&](int64_t t0) { return t_hi - t0 < CH ? (int)(t_hi - t0) : CH; };
-    auto fetch = [&](int x) {
-        const int64_t t0 = front(x);
-        const int rows = count(t0);
-        if (!LOCAL) rq.load(qp + t0 * a.q.step, a.q.step, rows, a.dk);
-        rk.load(kp + t0 * a.k.step, a.k.step, rows, a.dk);
-        rv.load(vp + t0 * a.v.step, a.v.step, rows, cols);
-        if (a.starts) {
-            const uint8_t* from = a.starts + n * a.starts_batch + t0 * a.starts_step;
-            if constexpr (VEC)
-                started = __builtin_amdgcn_raw_buffer_load_b8(__builtin_amdgcn_make_buffer_rsrc((void*)from, 0, (uint32_t)(rows - 1) * (uint32_t)a.starts_step + 1, 0x00020000),
-                                                              starts_at, 0, 0);
-            else
-                started = from[(lane < rows ? lane : 0) * a.starts_step];
-        }
-    };
     float odd = 0.0f, through = 1.0f;
-    if (chunks > 0) fetch(0);
     for (int x = 0; x < chunks; ++x) {
         const int64_t t0 = front(x);
         const int rows = count(t0);
