@@ -26,6 +26,15 @@ struct Operand {
     int64_t k_rows;   // k-major: rows that exist
 };
 
+// The tile of a workgroup: an XCD's workgroups stand on 8 x 4 tiles, not on 32 x 1, so that what they read of both operands stays in its L2
+__device__ __forceinline__ void tile_of(int64_t id, int64_t tiles_m, int64_t tiles_n, int64_t& tm, int64_t& tn) {
+    constexpr int64_t ROWS = 8;
+    const int64_t run = xcd_run(id, tiles_m * tiles_n), group = uniform(run / (ROWS * tiles_n)), first = group * ROWS, in = run - first * tiles_n;
+    const int64_t rows = tiles_m - first < ROWS ? tiles_m - first : ROWS;
+    tn = uniform(in / rows);
+    tm = first + in - tn * rows;
+}
+
 #define FISHING_LDS(p) ((__attribute__((address_space(3))) void*)(p))
 #define FISHING_GLOBAL(p) ((const __attribute__((address_space(1))) void*)(p))
 

@@ -69,8 +69,8 @@ __global__ void __launch_bounds__(G::THREADS, 2)
     loss_part_kernel(Operand<T> h, Operand<T> w, int64_t k, const void* target, int target_bytes, int64_t tiles_m, int64_t tiles_n, float* top, float* sum, float* taken) {
     __shared__ __attribute__((aligned(16))) char lds0[G::BYTES];
     __shared__ __attribute__((aligned(16))) char lds1[G::BYTES];
-    const int64_t tile = xcd_run(blockIdx.x, tiles_m * tiles_n);
-    const int64_t tn = uniform(tile / tiles_m), tm = tile - tn * tiles_m;
+    int64_t tm, tn;
+    tile_of(blockIdx.x, tiles_m, tiles_n, tm, tn);
     // the target's column in this tile, or -1; read behind the product's barriers
     __shared__ int column[BM];
     if (threadIdx.x < BM) {
@@ -161,8 +161,8 @@ __global__ void __launch_bounds__(G::THREADS, 2)
                    const float* g, T* dzt, int64_t ld) {
     __shared__ __attribute__((aligned(16))) char lds0[G::BYTES];
     __shared__ __attribute__((aligned(16))) char lds1[G::BYTES];
-    const int64_t tile = xcd_run(blockIdx.x, tiles_m * tiles_n);
-    const int64_t tn = uniform(tile / tiles_m), tm = tile - tn * tiles_m;
+    int64_t tm, tn;
+    tile_of(blockIdx.x, tiles_m, tiles_n, tm, tn);
     // per row of the tile, read behind the product's barriers: lse (infinite for a padded target: a share of zero), the loss's
     // gradient, the target's column or -1
     __shared__ float row_lse[BM], row_g[BM];
@@ -207,8 +207,8 @@ __global__ void __launch_bounds__(G::THREADS, 2)
     product_kernel(Operand<T> a, Operand<T> b, int64_t k, int64_t share, int64_t m, int64_t n, int64_t tiles_m, int64_t tiles_n, bool add, O* out, int64_t ld, int64_t slab) {
     __shared__ __attribute__((aligned(16))) char lds0[G::BYTES];
     __shared__ __attribute__((aligned(16))) char lds1[G::BYTES];
-    const int64_t tile = xcd_run(blockIdx.x, tiles_m * tiles_n);
-    const int64_t tn = uniform(tile / tiles_m), tm = tile - tn * tiles_m;
+    int64_t tm, tn;
+    tile_of(blockIdx.x, tiles_m, tiles_n, tm, tn);
     const int64_t lo = blockIdx.y * share, hi = lo + share < k ? lo + share : k;
     f32x4 acc[G::MT][G::NT];
     G::run(lds0, lds1, a, tm * BM, b, tn * BN, lo, hi, acc);
