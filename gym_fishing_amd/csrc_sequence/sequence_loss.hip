@@ -37,13 +37,27 @@ __device__ __forceinline__ float sum16(float x) {
     return x + rotated<1>(x);
 }
 
-// rows of `width` to rows of `padded`, zeros behind; rows of padded targets become zeros, whatever they hold (NaN times a zero dz is NaN)
+// Rows of `width` to rows of `padded`, zeros behind; rows of padded targets become zeros, whatever they hold (NaN times a zero dz is
+// NaN).  The two operands' copies are one launch: the second's blocks come behind the first's.
 template <typename T>
-__global__ void __launch_bounds__(256) pad_kernel(const T* src, int64_t ld, int64_t rows, int32_t width, T* dst, int32_t padded, const void* target, int target_bytes,
-                                                  int64_t levels) {
+struct PadJob {
+    const T* src;
+    int64_t ld, rows;
+    T* dst;
+    const void* target;       // of the rows, or none
+};
+
+template <typename T>
+__global__ void __launch_bounds__(256) pad_kernel(PadJob<T> first, PadJob<T> second, int64_t first_blocks, int32_t width, int32_t padded, int target_bytes, int64_t levels) {
+    const bool behind = blockIdx.x >= first_blocks;
+    const PadJob<T> job = behind ? second : first;
+    const int64_t block = behind ? blockIdx.x - first_blocks : blockIdx.x, ld = job.ld, rows = job.rows;
+    const T* src = job.src;
+    T* dst = job.dst;
+    const void* target = job.target;
     constexpr int V = vec_of<T>();
     const int per = padded / V;
-    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t at = block * 256 + threadIdx.x;
     const int64_t row = at / per;
     const int c = (int)(at - row * per) * V;
     if (row >= rows) return;
@@ -420,21 +434,21 @@ static int loss_check(int32_t dtype, int64_t rows, int64_t levels, int64_t dim) 
     return FISHING_OK;
 }
 
+// the copies that are asked for, in one launch
 template <typename T>
-static int pad(const T* src, int64_t ld, int64_t rows, int64_t width, T* dst, int64_t padded, const void* target, int target_bytes, int64_t levels, hipStream_t stream) {
-    return launch(pad_kernel<T>, dim3((unsigned)ceil_div(rows * (padded / vec_of<T>()), 256)), dim3(256), stream, src, ld, rows, (int32_t)width, dst, (int32_t)padded, target,
-                  target_bytes, levels);
+static int pads(const PadJob<T>& a, const PadJob<T>& b, const LossPlan& p, int64_t dim, int target_bytes, int64_t levels, hipStream_t stream) {
+    auto blocks = [&](const PadJob<T>& j) { return j.src ? ceil_div(j.rows * (p.dim_p / vec_of<T>()), 256) : 0; };
+    const int64_t first = blocks(a), second = blocks(b);
+    if (first + second == 0) return 0;
+    return launch(pad_kernel<T>, dim3((unsigned)(first + second)), dim3(256), stream, a, b, first, (int32_t)dim, (int32_t)p.dim_p, target_bytes, levels);
 }
 
-// the operand as it is where its rows are whole k steps at 16-byte addresses, its padded copy otherwise
+// the operand as it is where its rows are whole k steps at 16-byte addresses, its padded copy (whose job is then set) otherwise
 template <typename T>
-static int padded_operand(const LossPlan& p, const T* src, int64_t ld, int64_t rows, int64_t dim, T* copy, Operand<T>& o, hipStream_t stream) {
-    if (dim == p.dim_p && ld % vec_of<T>() == 0 && aligned16(src) && ld * (int64_t)sizeof(T) <= kMaxPitch) {
-        o = Operand<T>{src, ld, rows, rows};
-        return 0;
-    }
-    o = Operand<T>{copy, p.dim_p, rows, rows};
-    return pad<T>(src, ld, rows, dim, copy, p.dim_p, nullptr, 4, 0, stream);
+static Operand<T> padded_operand(const LossPlan& p, const T* src, int64_t ld, int64_t rows, int64_t dim, T* copy, PadJob<T>& job) {
+    if (dim == p.dim_p && ld % vec_of<T>() == 0 && aligned16(src) && ld * (int64_t)sizeof(T) <= kMaxPitch) return Operand<T>{src, ld, rows, rows};
+    job = PadJob<T>{src, ld, rows, copy, nullptr};
+    return Operand<T>{copy, p.dim_p, rows, rows};
 }
 
 template <typename T>
@@ -442,12 +456,15 @@ static int loss_forward(int64_t rows, int64_t levels, int64_t dim, const T* h, i
                         float* lse, void* workspace, hipStream_t stream) {
     const LossPlan p = loss_plan<T>(rows, levels, dim, false);
     const LossWork<T> k = loss_work<T>(p, rows, levels, dim, false, workspace);
-    Operand<T> a, b;
-    int rc = padded_operand<T>(p, w, w_ld, levels, dim, k.w, b, stream);
+    PadJob<T> w_job{};
+    const Operand<T> b = padded_operand<T>(p, w, w_ld, levels, dim, k.w, w_job);
+    int rc = 0;
     for (int64_t r0 = 0; r0 < rows && !rc; r0 += p.block) {
         const int64_t here = rows - r0 < p.block ? rows - r0 : p.block;
         const void* y = (const char*)target + r0 * target_bytes;
-        rc = padded_operand<T>(p, h + r0 * h_ld, h_ld, here, dim, k.h, a, stream);
+        PadJob<T> h_job{};
+        const Operand<T> a = padded_operand<T>(p, h + r0 * h_ld, h_ld, here, dim, k.h, h_job);
+        rc = pads(h_job, r0 ? PadJob<T>{} : w_job, p, dim, target_bytes, levels, stream);
         if (rc) break;
         rc = with_tile<T, false, false>(p.z, [&](auto t) {
             typedef decltype(t) Tile;
@@ -481,13 +498,14 @@ static int loss_backward(int64_t rows, int64_t levels, int64_t dim, const T* h, 
     const LossPlan p = loss_plan<T>(rows, levels, dim, true);
     const LossWork<T> k = loss_work<T>(p, rows, levels, dim, true, workspace);
     const Tiling whole = dw_tiling<T>(p, p.piece, dim);
-    Operand<T> b;
-    int rc = padded_operand<T>(p, w, w_ld, levels, dim, k.w, b, stream);
+    PadJob<T> w_job{};
+    const Operand<T> b = padded_operand<T>(p, w, w_ld, levels, dim, k.w, w_job);
+    int rc = 0;
     for (int64_t r0 = 0; r0 < rows && !rc; r0 += p.block) {
         const int64_t here = rows - r0 < p.block ? rows - r0 : p.block, here_p = round_up(here, p.bk);
         const void* y = (const char*)target + r0 * target_bytes;
         const Operand<T> a{k.h, p.dim_p, here, here};
-        rc = pad<T>(h + r0 * h_ld, h_ld, here, dim, k.h, p.dim_p, y, target_bytes, levels, stream);
+        rc = pads(PadJob<T>{h + r0 * h_ld, h_ld, here, k.h, y}, r0 ? PadJob<T>{} : w_job, p, dim, target_bytes, levels, stream);
         for (int64_t v0 = 0; v0 < levels && !rc; v0 += p.piece) {
             const int64_t width = levels - v0 < p.piece ? levels - v0 : p.piece, width_p = round_up(width, p.bk);
             rc = with_tile<T, false, false>(tiling<T>(here, width, dim, false).b, [&](auto t) {
