@@ -5,7 +5,8 @@ namespace fishing {
 namespace seq {
 
 // out[i] = scale * table[token[i]]; a token outside [0, vocab) is padding: a row of zeros.
-// A block owns 256 / vecs rows at a time (vecs accesses a row), four times over; bound by the rows written.
+// A block owns 256 / vecs rows at a time (vecs accesses a row), four times over, so that four rows' loads are in flight; bound by the
+// rows written: 1034240 x 256 f32 220 us, 4.8 TB/s; 413696 x 128 bf16 23 us, 4.6 TB/s; 4096 x 64 bf16 4 us, the launch's own.
 template <typename T, typename I, int V, bool PAST>
 __global__ void __launch_bounds__(256) embedding_kernel(const T* table, int64_t table_stride, const I* token, int64_t n, int64_t vocab,
                                                         int32_t vecs, float scale, T* out) {
@@ -43,7 +44,10 @@ __global__ void __launch_bounds__(256) embedding_kernel(const T* table, int64_t 
 // ---- the gradient: dtable[v] = scale * sum of dout[i] over the i with token[i] == v, in ascending i ----
 // A stable radix sort of (token, i) by up to 8 bits a pass puts a token's rows side by side; then chunks of the sorted order
 // are summed in float32 registers, and runs that cross a chunk's border leave a partial row that the last kernel adds in
-// chunk order.  No atomics: the same bits every time.
+// chunk order.  No atomics on sums: the same bits every time.  Bound by the rows read once, in the tokens' order: 1034240 x 256 f32,
+// 100 tokens: sorting 23 us, sums 206 (5.1 TB/s), join 10; 413696 x 128 bf16, 10001 tokens, two passes: sorting 29, sums 38
+// (2.8 TB/s: runs are 40 rows long), join 10.  (A table of partial sums in LDS, for few tokens, took 452 us where this takes 240; its
+// float atomics 1354.)
 constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64, kMaxDigits = 256;
 
 __device__ __forceinline__ uint32_t key_of(int64_t t, int64_t vocab) { return t >= 0 && t < vocab ? (uint32_t)t : (uint32_t)vocab; }

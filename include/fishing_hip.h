@@ -403,7 +403,8 @@ int fishing_embedding_backward(int32_t dtype, int32_t index_bytes, int64_t n, in
  *   out_t = scale * q_t S_t
  * q, k: [batch, steps, heads, dk], v, out: [batch, steps, heads, dv] with unit stride in the last axis and the element strides
  * {batch, step, head} given; starts: bytes with strides {batch, step}, nullable; state, state_out: float32 [batch, heads, dk, dv]
- * contiguous, nullable except for the single step.  dk, dv in 1 .. 128.  steps = 0 hands the state through. */
+ * contiguous, nullable except for the single step.  dk, dv in 1 .. 128, heads in 1 .. 65536.  steps = 0 hands the state through.
+ * Outputs overlap neither each other nor an operand (over whole episodes state_out is not state either). */
 typedef struct FishingDecayAttention {
     int32_t dtype, heads, dk, dv;
     int64_t batch, steps;
