@@ -122,22 +122,26 @@ static int attention_step(const FishingDecayAttention* a, hipStream_t stream) {
     return go(step_kernel_recurrent<T, 1>);
 }
 
-extern template int walk<float, true>(const FishingDecayAttention*, Strided, Strided, Strided, const float*, float*, Strided, int, int, bool, bool, double, double, void*, hipStream_t);
-extern template int walk<bf16, true>(const FishingDecayAttention*, Strided, Strided, Strided, const float*, float*, Strided, int, int, bool, bool, double, double, void*, hipStream_t);
+extern template int walk<float, true>(const FishingDecayAttention*, Strided, Strided, Strided, const float*, float*, Strided, int, int, bool, bool, double, double, Shared*, void*, hipStream_t);
+extern template int walk<bf16, true>(const FishingDecayAttention*, Strided, Strided, Strided, const float*, float*, Strided, int, int, bool, bool, double, double, Shared*, void*, hipStream_t);
 
 template <typename T>
 static int attention_forward(const FishingDecayAttention* a, void* work, hipStream_t stream) {
     return walk<T, false>(a, strided(a->q, a->q_stride), strided(a->k, a->k_stride), strided(a->v, a->v_stride), a->state, a->state_out,
-                               strided((const void*)a->out, a->out_stride), a->dk, a->dv, false, true, a->scale, 1.0, work, stream);
+                               strided((const void*)a->out, a->out_stride), a->dk, a->dv, false, true, a->scale, 1.0, nullptr, work, stream);
 }
 
 template <typename T>
 static int attention_backward(const FishingDecayAttention* a, void* work, hipStream_t stream) {
     const Strided q = strided(a->q, a->q_stride), k = strided(a->k, a->k_stride), v = strided(a->v, a->v_stride), g = strided(a->dout, a->dout_stride);
-    // dq: read with do the state that (v, k) build;  dk, dv: read with v, k the state's gradient that (do, q), (q, do) build backwards
-    int rc = walk<T, false>(a, g, v, k, a->state, nullptr, strided((const void*)a->dq, a->dq_stride), a->dv, a->dk, true, false, a->scale, 1.0, work, stream);
-    if (!rc) rc = walk<T, true>(a, v, g, q, a->dstate_out, nullptr, strided((const void*)a->dk_out, a->dk_stride), a->dv, a->dk, true, false, 1.0, a->scale, work, stream);
-    if (!rc) rc = walk<T, true>(a, k, q, g, a->dstate_out, a->dstate, strided((const void*)a->dv_out, a->dv_stride), a->dk, a->dv, false, a->dstate != nullptr, 1.0, a->scale, work, stream);
+    // dq: read with do the state that (v, k) build;  dk, dv: read with v, k the state's gradient that (do, q), (q, do) build backwards,
+    // in segments from the same states
+    Shared both;
+    int rc = walk<T, false>(a, g, v, k, a->state, nullptr, strided((const void*)a->dq, a->dq_stride), a->dv, a->dk, true, false, a->scale, 1.0, nullptr, work, stream);
+    if (!rc) rc = walk<T, true>(a, v, g, q, a->dstate_out, nullptr, strided((const void*)a->dk_out, a->dk_stride), a->dv, a->dk, true, false, 1.0, a->scale, &both, work, stream);
+    if (!rc)
+        rc = walk<T, true>(a, k, q, g, a->dstate_out, a->dstate, strided((const void*)a->dv_out, a->dv_stride), a->dk, a->dv, false, a->dstate != nullptr, 1.0, a->scale, &both,
+                           work, stream);
     return rc;
 }
 
@@ -157,14 +161,18 @@ int fishing_decay_attention_step(const FishingDecayAttention* a, fishing_stream_
 
 int64_t fishing_decay_attention_workspace(const FishingDecayAttention* a, int32_t backward) {
     if (int rc = attention_check(a, false)) return rc;
-    // the largest of its walks, which run one after the other, whichever way their rows are read
+    // the largest of its walks, which run one after the other, whichever way their rows are read; dk's and dv's share dk's states
     const int64_t pairs = batch_block(a->batch, a->heads) * a->heads;
-    int64_t most = 0;
+    int64_t most = 0, flags = 0;
     for (int back = 0; back <= (backward ? 1 : 0); ++back)
         for (int wide = 0; wide < 2; ++wide) {
-            const int64_t b = walk_work(walk_plan(a->dtype, pairs, a->steps, back ? a->dv : a->dk, back ? a->dk : a->dv, wide != 0), pairs, back ? a->dk : a->dv, nullptr).bytes;
+            const int rows = back ? a->dv : a->dk, cols = back ? a->dk : a->dv;
+            const WalkPlan p = walk_plan(a->dtype, pairs, a->steps, rows, cols, wide != 0);
+            const int64_t b = walk_work(p, pairs, cols, nullptr, nullptr).bytes, f = round_up(pairs * ceil_div(a->dv, 32) * p.segs * (int64_t)sizeof(uint32_t), 256);
             most = b > most ? b : most;
+            if (back && p.segs > 1) flags = f > flags ? f : flags;
         }
+    most += flags;
     return most;
 }
 

@@ -5,8 +5,8 @@
 namespace fishing {
 namespace seq {
 
-template int walk<float, true>(const FishingDecayAttention*, Strided, Strided, Strided, const float*, float*, Strided, int, int, bool, bool, double, double, void*, hipStream_t);
-template int walk<bf16, true>(const FishingDecayAttention*, Strided, Strided, Strided, const float*, float*, Strided, int, int, bool, bool, double, double, void*, hipStream_t);
+template int walk<float, true>(const FishingDecayAttention*, Strided, Strided, Strided, const float*, float*, Strided, int, int, bool, bool, double, double, Shared*, void*, hipStream_t);
+template int walk<bf16, true>(const FishingDecayAttention*, Strided, Strided, Strided, const float*, float*, Strided, int, int, bool, bool, double, double, Shared*, void*, hipStream_t);
 
 }  // namespace seq
 }  // namespace fishing

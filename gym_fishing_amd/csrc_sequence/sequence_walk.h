@@ -76,6 +76,9 @@ struct Lanes<bf16> {
     }
     // the state tile c's row 4 g + r
     static __device__ __forceinline__ int state_row(int c, int g) { return 32 * (c >> 1) + 8 * g + 4 * (c & 1); }
+    // of row x: its tile, and its place in a tile's 16 (4 g + r)
+    static __device__ __forceinline__ int row_tile(int x) { return 2 * (x >> 5) + (x >> 2 & 1); }
+    static __device__ __forceinline__ int row_place(int x) { return 4 * (x >> 3 & 3) + (x & 3); }
     static __device__ __forceinline__ f32x4 mma(Quad a0, Quad a1, Quad b0, Quad b1, f32x4 acc) {
         union {
             Quad q[2];
@@ -122,6 +125,8 @@ struct Lanes<float> {
     }
     static __device__ __forceinline__ Quad row_quad(const char* rows, int pitch, int y, int c) { return *(const Quad*)(rows + y * pitch + (16 * c + 4 * (threadIdx.x >> 4 & 3)) * 4); }
     static __device__ __forceinline__ int state_row(int c, int g) { return 16 * c + 4 * g; }
+    static __device__ __forceinline__ int row_tile(int x) { return x >> 4; }
+    static __device__ __forceinline__ int row_place(int x) { return x & 15; }
     static __device__ __forceinline__ f32x4 mma(Quad a0, Quad a1, Quad b0, Quad b1, f32x4 acc) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a0[e], b0[e], acc, 0, 0, 0);
@@ -205,6 +210,7 @@ struct ChunkArgs {
     int64_t seg_steps;
     float *carry, *through;    // the state behind a segment, per (pair, 16 columns, segment) in lane order, and what a segment lets through, per (pair, segment)
     uint32_t* odd;             // per (pair, slice, segment): some result is infinite or NaN
+    int32_t carry_nk;          // not 0: the carry is that of a walk whose state is this one's transposed, this many tiles of rows
 };
 
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
@@ -313,7 +319,15 @@ __global__ void __launch_bounds__(64, waves_a_simd(NK, NV, VEC, LOCAL)) chunk_ke
 #pragma unroll
             for (int m = 0; m < NV; ++m) {
                 S[c][m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-                if (seg > 0) {
+                if (BACK && !LOCAL && seg > 0 && a.carry_nk) {
+                    const int col = col0 + m * 16 + i, row = L::state_row(c, g), tiles = (a.dk + 15) / 16;
+                    const float* other = a.carry + ((pair * tiles + (row >> 4)) * a.segs + seg - 1) * (a.carry_nk * 256) + L::row_tile(col) * 256 + (L::row_place(col) >> 2) * 64 +
+                                         (col & 3);
+                    if (row < tiles * 16 && col < a.carry_nk * 16) {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) S[c][m][r] = other[((row & 15) + r) * 4];
+                    }
+                } else if (seg > 0) {
                     if (!LOCAL && col0 / 16 + m < col_tiles) S[c][m] = *(const f32x4*)(from + (m * a.segs * NK + c) * 256 + lane * 4);
                 } else if (s0) {
                     const int col = m * 16 + i, row = L::state_row(c, g);
@@ -664,21 +678,30 @@ struct WalkWork {
     int64_t bytes;
 };
 
-static WalkWork walk_work(const WalkPlan& p, int64_t pairs, int dv, void* at) {
+static WalkWork walk_work(const WalkPlan& p, int64_t pairs, int dv, float* carry, void* at) {
     Carve c(at);
     WalkWork w{};
     w.odd = c.take<uint32_t>(pairs * p.slices * p.segs);
-    if (p.segs > 1) {
+    w.carry = carry;
+    if (p.segs > 1 && !carry) {
         w.through = c.take<float>(pairs * p.segs);
         w.carry = c.take<float>(pairs * ceil_div(dv, 16) * p.segs * p.nk * 256);
     }
-    w.bytes = c.used + 256;
+    w.bytes = round_up(c.used, 256);
     return w;
 }
 
+// What a walk in segments leaves to one whose state is its own transposed, from the same terms: the states it starts its segments from
+struct Shared {
+    int nk = 0, segs = 1;
+    int64_t seg_steps = 0;
+    float* carry = nullptr;
+    int64_t bytes = 0;         // of the workspace, not to be written
+};
+
 template <typename T, bool BACK>
 int walk(const FishingDecayAttention* f, Strided q, Strided k, Strided v, const float* state, float* state_out, Strided out, int dk, int dv, bool state_t, bool exact_state,
-                double read_scale, double write_scale, void* workspace, hipStream_t stream) {
+                double read_scale, double write_scale, Shared* shared, void* workspace, hipStream_t stream) {
     if (f->steps <= 1) q.step = k.step = v.step = out.step = kMaxHeadDim;         // (a single step has no next one: any stride will do)
     constexpr int V = vec_of<T>();
     auto wide = [&](const Strided& s, int d) {
@@ -686,17 +709,29 @@ int walk(const FishingDecayAttention* f, Strided q, Strided k, Strided v, const 
     };
     const bool vec = wide(q, dk) && wide(k, dk) && wide(v, dv) && wide(out, dv) && f->starts_stride[1] < (int64_t)1 << 24;
     const int64_t block = batch_block(f->batch, f->heads);
-    const WalkPlan p = walk_plan(f->dtype, block * f->heads, f->steps, dk, dv, vec);
-    const WalkWork w = walk_work(p, block * f->heads, dv, workspace);
+    WalkPlan p = walk_plan(f->dtype, block * f->heads, f->steps, dk, dv, vec);
+    const bool given = shared && shared->nk;
+    if (given) {
+        p.segs = shared->segs;
+        p.seg_steps = shared->seg_steps;
+    } else if (shared) {                        // (of the two plans the one of fewer segments)
+        const WalkPlan other = walk_plan(f->dtype, block * f->heads, f->steps, dv, dk, vec);
+        if (other.segs > 1 && other.segs < p.segs) {
+            p.segs = other.segs;
+            p.seg_steps = other.seg_steps;
+        }
+    }
+    const WalkWork w = walk_work(p, block * f->heads, dv, given ? shared->carry : nullptr, (char*)workspace + (given ? shared->bytes : 0));
+    if (shared && !given && p.segs > 1) *shared = Shared{p.nk, p.segs, p.seg_steps, w.carry, w.bytes};
     ChunkArgs a{q, k, v, out, f->log_decay, f->starts, f->starts_stride[0], f->starts_stride[1], state, state_out, f->steps, f->heads, dk, dv, state_t, exact_state,
-                      (float)read_scale, (float)write_scale, p.slices, p.segs, p.seg_steps, w.carry, w.through, w.odd};
+                      (float)read_scale, (float)write_scale, p.slices, p.segs, p.seg_steps, w.carry, w.through, w.odd, given ? shared->nk : 0};
     int64_t pairs = 0;
     auto run = [&](auto tk, auto tv, auto rows) {
         const dim3 grid((unsigned)(pairs * p.slices * p.segs));
         constexpr int NK = decltype(tk)::value, NV = decltype(tv)::value;
         constexpr bool VEC = decltype(rows)::value;
         int rc = 0;
-        if (p.segs > 1) {
+        if (p.segs > 1 && !given) {
             // without outputs narrow slices fit two waves on a SIMD (16381 steps, 8 heads of 128 x 128: 26 us, with 4 tiles 44)
             constexpr int LV = NK >= 5 ? 2 : NV;
             const int per = NK * 256, col_tiles = (int)ceil_div(dv, 16);
