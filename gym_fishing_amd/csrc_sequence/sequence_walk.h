@@ -524,24 +524,26 @@ __global__ void __launch_bounds__(64, waves_a_simd(NK, NV, VEC, LOCAL)) chunk_ke
 }
 
 // the states behind a pair's segments, chained: carry[s] = through[s] carry[s - 1] + carry[s]
-static __global__ void __launch_bounds__(256) chain_kernel(float* carry, const float* through, int32_t segs, int32_t per, int32_t col_tiles) {
+static __global__ void __launch_bounds__(64) chain_kernel(float* carry, const float* through, int32_t segs, int32_t per, int32_t col_tiles) {
     const int64_t group = blockIdx.y;
-    const int at = blockIdx.x * 256 + threadIdx.x;
-    if (at >= per) return;
-    float* c = carry + group * segs * per + at;
+    f32x4* c = (f32x4*)(carry + group * segs * per) + blockIdx.x * 64 + threadIdx.x;
+    per /= 4;
     const float* p = through + group / col_tiles * segs;
-    float s = c[0];
+    f32x4 s = c[0];
     int x = 1;
     auto batch = [&](auto n) {                  // loads sent together: behind a store to the same array the compiler sends none ahead
         constexpr int U = decltype(n)::value;
         for (; x + U <= segs - 1; x += U) {
-            float next[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u) next[u] = c[(int64_t)(x + u) * per];
+            f32x4 next[U];
+            float f[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const float f = p[x + u];
-                s = (f == 0.0f ? 0.0f : f * s) + next[u];
+                next[u] = c[(int64_t)(x + u) * per];
+                f[u] = p[x + u];
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                s = f[u] == 0.0f ? next[u] : f[u] * s + next[u];
                 c[(int64_t)(x + u) * per] = s;
             }
         }
@@ -738,7 +740,7 @@ int walk(const FishingDecayAttention* f, Strided q, Strided k, Strided v, const 
             ChunkArgs local = a;
             local.slices = (int)ceil_div(dv, LV * 16);
             rc = launch(chunk_kernel<T, NK, LV, BACK, VEC, true>, dim3((unsigned)(pairs * local.slices * p.segs)), dim3(64), stream, local);
-            if (!rc) rc = launch(chain_kernel, dim3((unsigned)ceil_div(per, 256), (unsigned)(pairs * col_tiles)), dim3(256), stream, w.carry, w.through, p.segs, per, col_tiles);
+            if (!rc) rc = launch(chain_kernel, dim3((unsigned)(per / 256), (unsigned)(pairs * col_tiles)), dim3(64), stream, w.carry, w.through, p.segs, per, col_tiles);
         }
         return rc ? rc : launch(chunk_kernel<T, NK, NV, BACK, VEC, false>, grid, dim3(64), stream, a);
     };
