@@ -338,7 +338,9 @@ __global__ void __launch_bounds__(64, waves_a_simd(NK, NV, VEC, LOCAL)) chunk_ke
             }
     }
 
-    float odd = 0.0f, through = 1.0f;
+    // S is kept as a multiple: the state is sigma * S.  A chunk's decay then costs one factor, not one per element (and none of the
+    // moves between register files that those cost); past 2^-8 or 2^8, and where a start cuts, S is multiplied out.
+    float odd = 0.0f, through = 1.0f, sigma = 1.0f;
     for (int x = 0; x < chunks; ++x) {
         const int64_t t0 = front(x);
         const int rows = count(t0);
@@ -372,6 +374,15 @@ __global__ void __launch_bounds__(64, waves_a_simd(NK, NV, VEC, LOCAL)) chunk_ke
             }
         }
         through = st ? 0.0f : through * pass;
+        const float decayed = __int_as_float(uniform(__float_as_int(sigma * pass)));
+        const bool kept = decayed >= 0x1p-8f && decayed <= 0x1p8f;
+        const float scale = kept ? 1.0f / decayed : 1.0f;
+#pragma unroll
+        for (int t = 0; t < TS; ++t) {
+            w[t] *= scale;
+            into[t] *= sigma;
+        }
+        sigma = kept ? decayed : 1.0f;
 
         T* o_front = op + t0 * a.out.step;
         const auto o_rows = __builtin_amdgcn_make_buffer_rsrc(o_front, 0, 0x7fffffff, 0x00020000);
@@ -466,6 +477,10 @@ __global__ void __launch_bounds__(64, waves_a_simd(NK, NV, VEC, LOCAL)) chunk_ke
                 }
             }
             __builtin_amdgcn_sched_barrier(0);
+            if (!kept) {
+#pragma unroll
+                for (int c = 0; c < NK; ++c) S[c][m] *= decayed;
+            }
             f32x4 rest[TS];
             Quad y[TS];
 #pragma unroll
@@ -474,7 +489,7 @@ __global__ void __launch_bounds__(64, waves_a_simd(NK, NV, VEC, LOCAL)) chunk_ke
                 y[t] = L::round(rest[t]);
             }
 #pragma unroll
-            for (int c = 0; c < NK; ++c) S[c][m] = L::over_steps(kc[c], y, S[c][m] * pass);
+            for (int c = 0; c < NK; ++c) S[c][m] = L::over_steps(kc[c], y, S[c][m]);
             if (L::SPLIT) {
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
@@ -497,7 +512,7 @@ __global__ void __launch_bounds__(64, waves_a_simd(NK, NV, VEC, LOCAL)) chunk_ke
         for (int c = 0; c < NK; ++c)
 #pragma unroll
             for (int m = 0; m < NV; ++m)
-                if (col0 / 16 + m < col_tiles) *(f32x4*)(to + (m * a.segs * NK + c) * 256 + lane * 4) = S[c][m];
+                if (col0 / 16 + m < col_tiles) *(f32x4*)(to + (m * a.segs * NK + c) * 256 + lane * 4) = S[c][m] * sigma;
         if (lane == 0 && slice == 0) a.through[pair * a.segs + seg] = through;
         return;
     }
@@ -511,11 +526,12 @@ __global__ void __launch_bounds__(64, waves_a_simd(NK, NV, VEC, LOCAL)) chunk_ke
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
                     if (col < cols && row + r < a.dk) {
-                        odd += S[c][m][r] * 0.0f;
+                        const float x = S[c][m][r] * sigma;
+                        odd += x * 0.0f;
                         if (a.state_t)
-                            s1[(int64_t)(col0 + col) * a.dk + row + r] = S[c][m][r];
+                            s1[(int64_t)(col0 + col) * a.dk + row + r] = x;
                         else
-                            s1[(int64_t)(row + r) * a.dv + col0 + col] = S[c][m][r];
+                            s1[(int64_t)(row + r) * a.dv + col0 + col] = x;
                     }
             }
     }

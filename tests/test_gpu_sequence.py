@@ -588,3 +588,19 @@ def test_every_count_of_tiles(dk, dv, dtype):
         want, bound = ref.attention(*args), ref.attention_bounds(*args)
         for name, x in zip(("out", "state", "dq", "dk", "dv", "dstate"), list(got) + list(grads)):
             ref.check(x, want[name], bound[name], name)
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+def test_decays_that_grow_and_change_little(dtype):
+    """Factors above one, and horizons from under a step to thousands, over whole chunks and segments; the bounds are relative to
+    the same sums of magnitudes, which grow alike."""
+    for batch, steps in ((2, 100), (1, 600)):
+        q, k, v, _, cut, s0, g, gs = make(batch, steps, 5, 32, 48, dtype, False, 0.01, True, seed=steps)
+        ld = torch.tensor([0.05, 0.1, -0.0003, -0.17, -3.0], device="cuda")
+        leaves = [x.detach().requires_grad_() for x in (q, k, v, s0)]
+        got = sequence.decay_attention(*leaves[:3], ld, starts=cut, state=leaves[3], scale=0.2, return_state=True)
+        grads = torch.autograd.grad(got, leaves, [g, gs])
+        args = (q, k, v, ld, cut, s0, 0.2, g, gs)
+        want, bound = ref.attention(*args), ref.attention_bounds(*args)
+        for name, x in zip(("out", "state", "dq", "dk", "dv", "dstate"), list(got) + list(grads)):
+            ref.check(x, want[name], bound[name], name)
