@@ -30,6 +30,7 @@ from ._capi import DTYPE_BF16, DTYPE_F32, FishingDecayAttention, FishingLibraryE
 MAX_HEAD_DIM, MAX_HEADS = 128, 65536
 _DTYPES = {torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16}
 _RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_DEVICE = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)      # (behind a tensor on the device: initialised)
 
 
 def _stream(index):
@@ -39,7 +40,7 @@ def _stream(index):
 def _call(fn, device, *args):
     """The C entry on `device`'s current stream, with that device the current one."""
     index = device.index
-    if torch.cuda.current_device() == index:
+    if _DEVICE() == index:
         rc = fn(*args, _stream(index))
     else:
         with torch.cuda.device(index):
@@ -55,7 +56,7 @@ def _tensor(x, name, dims=None, dtypes=None, device=None):
         raise ValueError("%s must have %d dimensions, got shape %s" % (name, dims, tuple(x.shape)))
     if dtypes is not None and x.dtype not in dtypes:
         raise TypeError("%s must be %s, got %s" % (name, " or ".join(str(d) for d in dtypes), x.dtype))
-    if x.device.type != "cuda":
+    if not x.is_cuda:
         raise FishingLibraryError("%s must live on a HIP ('cuda') device, got %s: there is no CPU backend" % (name, x.device))
     if device is not None and x.device != device:
         raise ValueError("%s is on %s, the other operands on %s" % (name, x.device, device))
@@ -207,26 +208,27 @@ def _check_heads(q, k, v, log_decay, state, dims):
     dev = q.device
     _tensor(k, "k", dims, (q.dtype,), dev)
     _tensor(v, "v", dims, (q.dtype,), dev)
-    if k.shape != q.shape:
-        raise ValueError("k must have q's shape %s, got %s" % (tuple(q.shape), tuple(k.shape)))
-    if v.shape[:-1] != q.shape[:-1]:
-        raise ValueError("v must have q's leading shape %s, got %s" % (tuple(q.shape[:-1]), tuple(v.shape)))
-    heads, dk, dv = q.shape[-2], q.shape[-1], v.shape[-1]
+    qs, vs = q.shape, v.shape
+    if k.shape != qs:
+        raise ValueError("k must have q's shape %s, got %s" % (tuple(qs), tuple(k.shape)))
+    if vs[:-1] != qs[:-1]:
+        raise ValueError("v must have q's leading shape %s, got %s" % (tuple(qs[:-1]), tuple(vs)))
+    heads, dk, dv = qs[-2], qs[-1], vs[-1]
     if not (1 <= dk <= MAX_HEAD_DIM and 1 <= dv <= MAX_HEAD_DIM):
         raise ValueError("head dimensions must be in 1 .. %d, got q, k: %d and v: %d" % (MAX_HEAD_DIM, dk, dv))
     if not 1 <= heads <= MAX_HEADS:
         raise ValueError("1 .. %d heads are needed, got %d" % (MAX_HEADS, heads))
     _tensor(log_decay, "log_decay", 1, (torch.float32,), dev)
-    if log_decay.shape[0] != heads:
-        raise ValueError("log_decay must hold one value for each of %d heads, got %d" % (heads, log_decay.shape[0]))
+    if log_decay.numel() != heads:
+        raise ValueError("log_decay must hold one value for each of %d heads, got %d" % (heads, log_decay.numel()))
     if torch.is_grad_enabled() and log_decay.requires_grad:
         raise ValueError("log_decay has no gradient here: a head's decay is a fixed horizon (detach it)")
-    if q.shape[0] * heads > 0x7FFFFFFF:
+    if qs[0] * heads > 0x7FFFFFFF:
         raise ValueError("at most 2^31 - 1 (batch, head) pairs a call")
-    shape = (q.shape[0], heads, dk, dv)
+    shape = (qs[0], heads, dk, dv)
     if state is not None:
         _tensor(state, "state", 4, (torch.float32,), dev)
-        if tuple(state.shape) != shape:
+        if state.shape != shape:
             raise ValueError("state must be [batch, heads, dk, dv] = %s, got %s" % (shape, tuple(state.shape)))
     return shape
 
@@ -307,10 +309,8 @@ def decay_attention_step(q, k, v, log_decay, state, starts=None, scale=None, out
     a.scale = dk ** -0.5 if scale is None else float(scale)
     a.q, a.k, a.v, a.log_decay = q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr()
     a.state, a.state_out, a.out = state.data_ptr(), state_out.data_ptr(), out.data_ptr()
-    a.q_stride[:] = (q.stride(0), 0, q.stride(1))
-    a.k_stride[:] = (k.stride(0), 0, k.stride(1))
-    a.v_stride[:] = (v.stride(0), 0, v.stride(1))
-    a.out_stride[:] = (out.stride(0), 0, out.stride(1))
+    for to, x in ((a.q_stride, q), (a.k_stride, k), (a.v_stride, v), (a.out_stride, out)):
+        to[0], to[2], _ = x.stride()
     if starts is not None:
         a.starts = starts.data_ptr()
         a.starts_stride[0] = starts.stride(0)
