@@ -604,3 +604,31 @@ def test_decays_that_grow_and_change_little(dtype):
         want, bound = ref.attention(*args), ref.attention_bounds(*args)
         for name, x in zip(("out", "state", "dq", "dk", "dv", "dstate"), list(got) + list(grads)):
             ref.check(x, want[name], bound[name], name)
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("n,vocab,dim", [(2048, 16, 512), (2047, 3, 40), (2048, 70000, 24), (1500, 131072, 8), (2048, 1, 64), (700, 2049, 1030), (2, 40000, 300), (1999, 33000, 7), (3000, (1 << 22) + 9, 1)])
+def test_embedding_gradient_of_few_tokens(n, vocab, dim, dtype):
+    tokens, table = tokens_of(n, vocab, n + dim, torch.int64 if dim % 2 else torch.int32), torch.zeros((vocab, dim), dtype=dtype, device="cuda", requires_grad=True)
+    tokens[:2] = torch.tensor([vocab - 1, 0])[: len(tokens[:2])]
+    grad = rand(n, dim + 3, seed=2, dtype=dtype)[:, :dim] if n % 2 else rand(n, dim, seed=2, dtype=dtype)
+    got = torch.autograd.grad(sequence.embedding(tokens, table, scale=0.7), table, grad)[0]
+    assert torch.equal(got, torch.autograd.grad(sequence.embedding(tokens, table, scale=0.7), table, grad)[0])
+    there = (tokens >= 0) & (tokens < vocab)
+    rows = tokens[there].long().cpu()
+    want, size = (torch.zeros((vocab, dim), dtype=torch.float64).index_add_(0, rows, x[there].cpu().double() * 0.7) for x in (grad, grad.abs()))
+    most = int(torch.bincount(rows, minlength=1).max())
+    ref.check(got, want, size * ((most + 4) * 2.0 ** -24) + ref.STEP[dtype] * want.abs() * 1.01, "table")
+
+
+@pytest.mark.parametrize("vocab,dim", [(101, 64), (2048, 33), (4, 300)])
+@pytest.mark.parametrize("n", [4096, 4097])
+def test_embedding_gradient_listed_or_sorted(n, vocab, dim):
+    """Either side of the number of tokens from which on they are sorted: whole numbers, so both are exact."""
+    tokens = tokens_of(n, vocab, n, torch.int64)
+    table = torch.zeros((vocab, dim), device="cuda", requires_grad=True)
+    grad = torch.randint(-9, 10, (n, dim), generator=torch.Generator().manual_seed(n)).float().cuda()
+    got = torch.autograd.grad(sequence.embedding(tokens, table), table, grad)[0]
+    there = (tokens >= 0) & (tokens < vocab)
+    want = torch.zeros((vocab, dim)).index_add_(0, tokens[there].cpu(), grad[there].cpu())
+    assert torch.equal(got.cpu(), want)
