@@ -39,8 +39,8 @@ static int64_t batch_block(int64_t batch, int heads) {
 // A wave alone needs no barriers; the next chunk's rows are loaded into registers while this one is computed, and the registers (state,
 // rows in flight, operands) leave room for two waves on a SIMD.  What bounds it is those waves' dependent work, not a unit: 2048 x 101
 // steps, 4 heads of 64 x 64, bf16: 112 us a walk, 2.7 TB/s, VALU 37% and matrix cores 17% busy; 97 x 1009 steps, 3 heads of 48 x 80,
-// f32: 76 - 95 us and 42 - 51 for the segments' states, matrix cores half busy; 16381 steps, 8 heads of 128 x 128, bf16, one wave a
-// SIMD: 65 us, states 28, chain 16.  (A third wave a SIMD spilled: 2.3 times slower.)
+// f32: 78 - 100 us and 46 for the segments' states, matrix cores half busy; 16381 steps, 8 heads of 128 x 128, bf16, one wave a
+// SIMD: 61 us, states 27, chain 11.  (A third wave a SIMD spilled: 2.3 times slower.)
 
 // The value, not to be worked with ahead of this place: what is computed of lane numbers for the rare chunk would otherwise be
 // computed once and kept, some sixty registers of it
