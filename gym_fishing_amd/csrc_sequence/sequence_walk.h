@@ -655,6 +655,17 @@ __global__ void __launch_bounds__(256) odd_kernel(ChunkArgs a, int64_t pairs) {
     }
 }
 
+// The recurrence for every pair, 32 columns of its state a workgroup, where there are few steps and no more workgroups than the chip
+// holds at once: a chunk would be nearly empty, and in bfloat16 its copy of the state costs a rounding.  16 pairs of 32 x 32: 5 us a
+// step, 7 four, chunks 10; 16384 pairs, four steps: 61 us, chunks 32
+constexpr int64_t kFewSteps = 8, kFewGroups = 2048;
+
+template <typename T, bool BACK>
+__global__ void __launch_bounds__(256) few_steps_kernel(ChunkArgs a) {
+    __shared__ float row[2][kMaxHeadDim];
+    recurrent<T, BACK>(a, blockIdx.x, blockIdx.y * 32, row);
+}
+
 // How a walk over (batch, heads) pairs is cut: column slices of the state, and, where there are few waves and many steps, segments of
 // the steps, whose states are computed first (from k and v alone) and chained.
 struct WalkPlan {
@@ -770,10 +781,14 @@ int walk(const FishingDecayAttention* f, Strided q, Strided k, Strided v, const 
     int rc = 0;
     for (int64_t n = 0; n < f->batch && !rc; n += block) {
         pairs = (f->batch - n < block ? f->batch - n : block) * f->heads;
-        rc = !vec ? tiles(Count<2>{}, std::false_type{}) : p.nv == 2 ? tiles(Count<2>{}, std::true_type{}) : p.nv == 3 ? tiles(Count<3>{}, std::true_type{}) : tiles(Count<4>{}, std::true_type{});
+        if (f->steps <= kFewSteps && pairs * ceil_div(dv, 32) <= kFewGroups) {
+            rc = launch(few_steps_kernel<T, BACK>, dim3((unsigned)pairs, (unsigned)ceil_div(dv, 32)), dim3(256), stream, a);
+        } else {
+            rc = !vec ? tiles(Count<2>{}, std::false_type{}) : p.nv == 2 ? tiles(Count<2>{}, std::true_type{}) : p.nv == 3 ? tiles(Count<3>{}, std::true_type{}) : tiles(Count<4>{}, std::true_type{});
+            const int64_t groups = ceil_div(pairs, kOddGroup);
+            if (!rc) rc = launch(odd_kernel<T, BACK>, dim3((unsigned)(groups < 1024 ? groups : 1024)), dim3(256), stream, a, pairs);
+        }
         if (rc) break;
-        const int64_t groups = ceil_div(pairs, kOddGroup);
-        rc = launch(odd_kernel<T, BACK>, dim3((unsigned)(groups < 1024 ? groups : 1024)), dim3(256), stream, a, pairs);
         // the next block's corners
         for (Strided* s : {&a.q, &a.k, &a.v, &a.out}) s->p = (const T*)s->p + block * s->batch;
         if (a.starts) a.starts += block * a.starts_batch;

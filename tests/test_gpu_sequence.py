@@ -632,3 +632,18 @@ def test_embedding_gradient_listed_or_sorted(n, vocab, dim):
     there = (tokens >= 0) & (tokens < vocab)
     want = torch.zeros((vocab, dim)).index_add_(0, tokens[there].cpu(), grad[there].cpu())
     assert torch.equal(got.cpu(), want)
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("steps", [1, 2, 8, 9])
+@pytest.mark.parametrize("batch,heads,dk,dv", [(1, 5, 18, 90), (1024, 2, 32, 32), (1025, 2, 32, 32), (3, 1, 128, 128)])
+def test_a_few_steps(batch, heads, dk, dv, steps, dtype):
+    """Either side of the sizes up to which the recurrence is run as it stands."""
+    q, k, v, ld, cut, s0, g, gs = make(batch, steps, heads, dk, dv, dtype, False, 0.2, True, seed=steps + dk)
+    leaves = [x.detach().requires_grad_() for x in (q, k, v, s0)]
+    got = sequence.decay_attention(*leaves[:3], ld, starts=cut, state=leaves[3], scale=0.4, return_state=True)
+    grads = torch.autograd.grad(got, leaves, [g, gs])
+    args = (q, k, v, ld, cut, s0, 0.4, g, gs)
+    want, bound = ref.attention(*args), ref.attention_bounds(*args)
+    for name, x in zip(("out", "state", "dq", "dk", "dv", "dstate"), list(got) + list(grads)):
+        ref.check(x, want[name], bound[name], name)
