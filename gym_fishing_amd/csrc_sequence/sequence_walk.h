@@ -33,9 +33,9 @@ static int64_t batch_block(int64_t batch, int heads) {
 // so a chunk is four small products on the matrix cores.  The layouts chain without a shuffle: the tile k q^T has its columns in
 // lanes and four rows y in registers, which is the second operand of v^T (k q^T); a state tile k^T v likewise is the first of S^T q^T;
 // the outputs come as four neighbouring columns of one step per lane.  k and v are read by columns through the transposing LDS read
-// (bf16) or element reads (f32).  bf16: the products need scores, the state and the decayed v in bf16.  The state's copy is rounded
-// once, as the output is; the scores go as two bf16 terms (16 bits) and the decayed v as two or, where the state is an answer in
-// float32, three: every one of them rounded once would add up to 2x the output's own rounding, this way it is 1.0 - 1.4x.
+// (bf16) or element reads (f32).  bf16: the products need scores, the state and the decayed v in bf16.  The state's copy and the scores
+// go as two bf16 terms (16 bits) and the decayed v as two or, where the state is an answer in float32, three: what comes before an
+// output's own rounding is then too small to show in it (a copy of the state in one term: up to 1.4x that rounding, 2 - 3% less time).
 // A wave alone needs no barriers; the next chunk's rows are loaded into registers while this one is computed, and the registers (state,
 // rows in flight, operands) leave room for two waves on a SIMD.  What bounds it is those waves' dependent work, not a unit: 2048 x 101
 // steps, 4 heads of 64 x 64, bf16: 112 us a walk, 2.7 TB/s, VALU 37% and matrix cores 17% busy; 97 x 1009 steps, 3 heads of 48 x 80,
@@ -453,8 +453,12 @@ __global__ void __launch_bounds__(64, waves_a_simd(NK, NV, VEC, LOCAL)) chunk_ke
                 for (int c = 0; c < NK - 1; c += 2) {
                     const Quad s0 = L::round(S[c][m]), s1 = L::round(S[c + 1][m]);
 #pragma unroll
-                    for (int t = 0; t < TS; ++t)
-                        o[t] = L::mma(s0, s1, q[t][c], q[t][c + 1], o[t]);
+                    for (int t = 0; t < TS; ++t) o[t] = L::mma(s0, s1, q[t][c], q[t][c + 1], o[t]);
+                    if (L::SPLIT) {
+                        const Quad r0 = L::round(S[c][m] - L::wide(s0)), r1 = L::round(S[c + 1][m] - L::wide(s1));
+#pragma unroll
+                        for (int t = 0; t < TS; ++t) o[t] = L::mma(r0, r1, q[t][c], q[t][c + 1], o[t]);
+                    }
                 }
                 if constexpr (NK & 1) o[0] = L::over_steps({S[NK - 1][m]}, {q[0][NK - 1]}, o[0]);
 #pragma unroll
@@ -656,8 +660,8 @@ __global__ void __launch_bounds__(256) odd_kernel(ChunkArgs a, int64_t pairs) {
 }
 
 // The recurrence for every pair, 32 columns of its state a workgroup, where there are few steps and no more workgroups than the chip
-// holds at once: a chunk would be nearly empty, and in bfloat16 its copy of the state costs a rounding.  16 pairs of 32 x 32: 5 us a
-// step, 7 four, chunks 10; 16384 pairs, four steps: 61 us, chunks 32
+// holds at once: a chunk would be nearly empty.  16 pairs of 32 x 32: 5 us a step, 7 four, chunks 10; 16384 pairs, four steps: 61 us,
+// chunks 32
 constexpr int64_t kFewSteps = 8, kFewGroups = 2048;
 
 template <typename T, bool BACK>

@@ -93,3 +93,21 @@ def check(got, want, bound, what=""):
     assert torch.isfinite(got).all(), what
     over = ((got - want).abs() - bound)
     assert (over <= 1e-30).all(), "%s: off by %.3g where %.3g is allowed" % (what, (got - want).abs().flatten()[over.argmax()], bound.flatten()[over.argmax()])
+
+
+def check_once_rounded(got, want, what="", low=1 << 11):
+    """A bfloat16 result whose only rounding worth speaking of is its last: its error in the 2-norm is at most 1.1 times that of `want`
+    rounded once.  What comes before keeps 16 bits or more: terms off by at most 2^-16 of themselves, two thousandths of the last
+    rounding's 2^-8 each, whose errors add up like the terms they belong to.  The last rounding's own error is spread over a step, so its
+    norm over n values is known to about 0.45 n^-1/2 (2048 values: 1%).  One more rounding to bfloat16 on the way makes it 1.4."""
+    got = got.detach().cpu()
+    assert got.dtype == torch.bfloat16 and got.numel() >= low, (what, got.dtype, got.numel())
+    once = (want.to(torch.bfloat16).to(F64) - want).norm()
+    off = (got.to(F64) - want).norm()
+    assert off <= 1.1 * once, "%s: off by %.3g, one rounding by %.3g" % (what, off, once)
+
+
+def state_bound(size, steps):
+    """How far a float32 state may be off, `size` the state of the operands' magnitudes: a product of bfloat16 values is exact in float32; the
+    decays weigh it as a product of float32 factors, one a chunk or step, and are exp2 of a rounded exponent; v's three bfloat16 terms leave 2^-26."""
+    return (2 * steps + 64) * 2.0 ** -24 * size
