@@ -36,8 +36,8 @@ __global__ void __launch_bounds__(256) step_kernel_recurrent(Strided q, Strided 
         }
     }
     __syncthreads();
-    const bool keep = !(starts && live && starts[n * starts_stride]);
     const float a = expf(log_decay_of(log_decay, h));
+    const bool keep = !(starts && live && starts[n * starts_stride]) && a != 0.0f;       // (a decay of zero drops NaN too, as over whole episodes)
     const int cols = dv / V, wide = cols < 64 ? cols : 64, rows = 64 / wide;
     const int r = lane / wide, c0 = lane - r * wide;
     const float* from = state + pair * (int64_t)dk * dv;

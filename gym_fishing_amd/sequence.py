@@ -245,7 +245,7 @@ def decay_attention(q, k, v, log_decay, starts=None, state=None, scale=None, ret
 
     q, k: [batch, steps, heads, dk], v: [batch, steps, heads, dv], float32 or bfloat16, dk and dv in 1 .. 128; any strides (a
     time-major record's `x.transpose(0, 1)` is read in place and answered in the same order; a last axis with gaps is copied).
-    log_decay: float32 [heads], a head's horizon (-inf: none; no gradient).  starts: bool [batch, steps], True where an episode
+    log_decay: float32 [heads], a head's horizon (no gradient; -inf, or where float32's exp is 0: nothing is kept, not even NaN).  starts: bool [batch, steps], True where an episode
     begins -- the done flags of the step before (SB3's `episode_starts`): nothing passes from before it, not even NaN.
     state: float32 [batch, heads, dk, dv], the memory from earlier steps (None: zeros).  scale: dk ** -0.5 by default.
     Returns out [batch, steps, heads, dv], or (out, state behind the last step) with return_state.

@@ -400,6 +400,7 @@ int fishing_embedding_backward(int32_t dtype, int32_t index_bytes, int64_t n, in
 
 /* Linear attention with a decay for each head.  For every batch row and head, over steps t:
  *   S_t = a_t S_{t-1} + k_t v_t^T     a_t = exp(log_decay[h]), 0 where starts[batch, t] (an episode begins at t)
+ * (a_t = 0 lets nothing through, not even NaN)
  *   out_t = scale * q_t S_t
  * q, k: [batch, steps, heads, dk], v, out: [batch, steps, heads, dv] with unit stride in the last axis and the element strides
  * {batch, step, head} given; starts: bytes with strides {batch, step}, nullable; state, state_out: float32 [batch, heads, dk, dv]
