@@ -13,7 +13,8 @@ tests/test-PPO.py:10-21) cannot use it.  These are the operators of one that can
 `policies.memory` is the policy built on them.  Everything runs in hand-written HIP kernels behind the C ABI
 (include/fishing_hip.h) on torch's current stream of the tensors' device; there is no CPU fallback.  Values are float32 or
 bfloat16 (float16's range is too narrow for the products of states and for dz); sums, softmax statistics and states are float32.
-The same inputs give the same bits.
+The same inputs give the same bits.  Derivatives are reverse-mode and of the first order: an operand or gradient that carries a
+forward-mode tangent is refused.
 
 Tensors made on another stream are the caller's to order, as for any torch operator.  Captured into a hipGraph, an operator
 takes its workspace from the graph's memory pool, so graphs share none.  torch's own rule holds for a captured backward(): no
@@ -22,6 +23,7 @@ eager autograd graph over the same leaves may be alive while it is captured (use
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _capi
@@ -49,9 +51,16 @@ def _call(fn, device, *args):
         _capi.check(rc, fn.__name__)
 
 
+def _no_tangent(x, name):
+    """A kernel sees a dual tensor's value alone: its derivative would come out as zero."""
+    if getattr(forward_ad, "_current_level", 0) >= 0 and forward_ad.unpack_dual(x).tangent is not None:
+        raise NotImplementedError("%s carries a forward-mode tangent: the sequence operators have no forward-mode derivative" % name)
+
+
 def _tensor(x, name, dims=None, dtypes=None, device=None):
     if not isinstance(x, torch.Tensor):
         raise TypeError("%s must be a torch.Tensor, got %s" % (name, type(x).__name__))
+    _no_tangent(x, name)
     if dims is not None and x.dim() != dims:
         raise ValueError("%s must have %d dimensions, got shape %s" % (name, dims, tuple(x.shape)))
     if dtypes is not None and x.dtype not in dtypes:
@@ -96,6 +105,7 @@ class _Embedding(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, grad):
         tokens, = ctx.saved_tensors
+        _no_tangent(grad, "the gradient")
         vocab, dim = ctx.shape
         lib, n = _capi.lib(), tokens.numel()
         grad = _rows(grad.reshape(n, dim))
@@ -190,6 +200,9 @@ class _DecayAttention(torch.autograd.Function):
         q, k, v, state, log_decay, starts = ctx.saved_tensors
         if dout is None and dlast is None:
             return (None,) * 8
+        for x in (dout, dlast):
+            if x is not None:
+                _no_tangent(x, "the gradient")
         lib, dev = _capi.lib(), q.device
         dout = _unit(dout) if dout is not None else torch.zeros(q.shape[:3] + v.shape[3:], dtype=q.dtype, device=dev)
         dlast = dlast.contiguous() if dlast is not None else None
@@ -347,6 +360,7 @@ class _CrossEntropy(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, grad):
         hidden, head, target, lse = ctx.saved_tensors
+        _no_tangent(grad, "the gradient")
         rows, dim = hidden.shape
         levels = head.shape[0]
         lib, dev = _capi.lib(), hidden.device

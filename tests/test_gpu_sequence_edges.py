@@ -4,6 +4,7 @@ import sys
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
 import sequence_reference as ref  # noqa: E402
@@ -35,3 +36,24 @@ def test_a_decay_of_zero_lets_nothing_through_not_even_nan(batch, dk, dv, dtype)
     for got, what in ((last, "whole"), (state, "step")):
         ref.check(got[:, :3], want["state"][:, :3], bound["state"][:, :3], what)
         assert torch.isnan(got[0, 3]).all()
+
+
+def test_forward_mode_tangents_are_refused_in_every_operand_and_gradient():
+    q, k, v, ld, _, s0, g, gs = make(2, 5, 2, 8, 12, torch.float32, False, 0.0, True)
+    table, hidden, head, i = rand(5, 8), rand(3, 8), rand(5, 8), torch.zeros(3, dtype=torch.int64, device="cuda")
+    calls = [(sequence.embedding, dict(tokens=i, table=table)), (sequence.cross_entropy, dict(hidden=hidden, head=head, target=i)),
+             (sequence.decay_attention, dict(q=q, k=k, v=v, log_decay=ld, state=s0)),
+             (sequence.decay_attention_step, dict(q=q[:, 0], k=k[:, 0], v=v[:, 0], log_decay=ld, state=s0, state_out=s0.clone(), out=g[:, 0].contiguous()))]
+    for f, kw in calls:
+        for name, x in kw.items():
+            if x.is_floating_point():
+                with forward_ad.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
+                    f(**{**kw, name: forward_ad.make_dual(x, torch.ones_like(x))})
+    t, w, h = table.requires_grad_(), head.requires_grad_(), hidden.requires_grad_()
+    leaf = q.detach().requires_grad_()
+    with forward_ad.dual_level():
+        out, last = sequence.decay_attention(leaf, k, v, ld, state=s0, return_state=True)
+        for y, x in ((sequence.embedding(i, t), t), (sequence.cross_entropy(h, w, i), w), (out, leaf), (last, leaf)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                torch.autograd.grad(y, x, forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y)), retain_graph=True)
+            assert torch.autograd.grad(y, x, torch.ones_like(y), retain_graph=True)[0].shape == x.shape

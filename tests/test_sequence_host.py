@@ -126,3 +126,24 @@ def test_large_calls_have_a_plan_that_fits(lib):
     assert lib.fishing_decay_attention_workspace(a, 1) == need < 1 << 28
     a.heads, a.batch = 65537, 1
     assert lib.fishing_decay_attention_workspace(a, 0) == -4 and lib.fishing_decay_attention_step(a, None) == -4
+
+
+def test_forward_mode_tangents_are_refused():
+    """Before anything else is looked at: a kernel would see the value alone, and the derivative would come out as zero."""
+    from torch.autograd import forward_ad
+    f, i = torch.ones, torch.zeros(3, dtype=torch.int64)
+    with forward_ad.dual_level():
+        def dual(*shape):
+            return forward_ad.make_dual(f(*shape), f(*shape))
+        seq, one = [f(1, 2, 1, 4)] * 3, [f(1, 1, 4)] * 3
+        calls = [lambda: sequence.embedding(i, dual(5, 8)), lambda: sequence.cross_entropy(dual(3, 8), f(5, 8), i)]
+        calls += [lambda a=a: sequence.decay_attention(*a, f(1)) for a in ([dual(1, 2, 1, 4)] + seq[1:],)]
+        calls += [lambda a=a: sequence.decay_attention_step(*a, f(1), f(1, 1, 4, 4)) for a in ([dual(1, 1, 4)] + one[1:],)]
+        for call in calls:
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+            with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+    sequence._no_tangent(f(3), "x")                       # outside a level, and without a tangent inside one
+    with forward_ad.dual_level():
+        sequence._no_tangent(f(3), "x")
