@@ -57,3 +57,61 @@ def test_forward_mode_tangents_are_refused_in_every_operand_and_gradient():
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 torch.autograd.grad(y, x, forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y)), retain_graph=True)
             assert torch.autograd.grad(y, x, torch.ones_like(y), retain_graph=True)[0].shape == x.shape
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("dk,dv", [(17, 33), (33, 65), (49, 5), (65, 127), (81, 50), (127, 97)])
+def test_segments_of_rows_that_are_not_whole_accesses(dk, dv, dtype):
+    """Long histories of few rows whose loads cannot be wide: their states are computed in segments too, and dv's walk starts from dk's."""
+    steps = 600 if dtype == torch.float32 else 1100
+    q, k, v, ld, cut, s0, g, gs = make(1, steps, 2, dk, dv, dtype, dk % 4 == 1, 0.004, True, seed=dk * dv)
+    leaves = [x.detach().requires_grad_() for x in (q, k, v, s0)]
+    got = sequence.decay_attention(*leaves[:3], ld / 16, starts=cut, state=leaves[3], scale=0.3, return_state=True)
+    grads = torch.autograd.grad(got, leaves, [g, gs])
+    args = (q, k, v, ld / 16, cut, s0, 0.3, g, gs)
+    want, bound = ref.attention(*args), ref.attention_bounds(*args)
+    size = ref.attention(*[x.abs() for x in args[:3]], *args[3:5], s0.abs(), 0.3, g.abs(), gs.abs())
+    for name, x in zip(("out", "state", "dq", "dk", "dv", "dstate"), list(got) + list(grads)):
+        ref.check(x, want[name], bound[name], name)
+        if x.dtype == torch.bfloat16:
+            ref.check_once_rounded(x, want[name], name)
+        elif name.endswith("state"):
+            ref.check(x, want[name], ref.state_bound(size[name], steps), name)
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("dk,dv", [(32, 48), (33, 47), (64, 128)])
+def test_nothing_passes_a_start_across_segments(dk, dv, dtype):
+    """NaN and infinities in a long history stay in their episode, whichever segment it lies in and however many it spans, in both
+    directions of time; and a head whose decay is zero keeps them to their step."""
+    steps = 700 if dtype == torch.float32 else 1300
+    q, k, v, ld, _, s0, g, gs = make(1, steps, 3, dk, dv, dtype, False, 0.0, True, seed=dk)
+    ld = torch.tensor([-0.02, -0.3, float("-inf")], device="cuda")
+    cut = torch.zeros((1, steps), dtype=torch.bool, device="cuda")
+    cut[:, [20, 300, steps - 250, steps - 90]] = True
+    clean = [x.clone() for x in (q, k, v, g)]
+    # the first episode (the state carried in), one that spans segments, and the last (the gradient of the state handed out)
+    s0[0], gs[0] = float("nan"), float("inf")
+    q[0, 200], k[0, 150], v[0, 170], g[0, 280] = float("nan"), float("inf"), float("-inf"), float("nan")
+    k[0, steps - 50] = float("nan")
+    leaves = [x.detach().requires_grad_() for x in (q, k, v, s0)]
+    got = sequence.decay_attention(*leaves[:3], ld, starts=cut, state=leaves[3], return_state=True)
+    grads = torch.autograd.grad(got, leaves, [g, gs])
+    args = (*clean[:3], torch.nan_to_num(ld, neginf=-200.0), cut, torch.zeros_like(s0), dk ** -0.5, clean[3], torch.zeros_like(gs))
+    want, bound = ref.attention(*args), ref.attention_bounds(*args)
+    got = dict(zip(("out", "state", "dq", "dk", "dv", "dstate"), list(got) + list(grads)))
+    for name in ("out", "dq", "dk", "dv"):
+        for at in (slice(300, steps - 250), slice(steps - 250, steps - 90)):
+            ref.check(got[name][:, at], want[name][:, at], bound[name][:, at], name)
+        dirty = torch.zeros(steps, dtype=torch.bool)         # of the head that forgets: these steps and no other
+        dirty[[200, 150, 170, 280, steps - 50]] = True
+        if name in ("dk", "dv"):
+            dirty[-1] = True
+        ref.check(got[name][:, ~dirty, 2], want[name][:, ~dirty, 2], bound[name][:, ~dirty, 2], name + " without memory")
+    # forwards what comes later does not reach back, backwards what came before does not reach on
+    ref.check(got["out"][:, 20:150, :2], want["out"][:, 20:150, :2], bound["out"][:, 20:150, :2], "out")
+    ref.check(got["out"][:, steps - 90:steps - 50], want["out"][:, steps - 90:steps - 50], bound["out"][:, steps - 90:steps - 50], "out")
+    ref.check(got["dk"][:, 281:300, :2], want["dk"][:, 281:300, :2], bound["dk"][:, 281:300, :2], "dk")
+    assert not torch.isfinite(got["out"][0, :20, :2]).any() and not torch.isfinite(got["out"][0, 170:300, :2]).any()
+    assert torch.isnan(got["state"][0]).any() and torch.isfinite(got["state"][0, 2]).all()
+    ref.check(got["dstate"][:, 2], want["dstate"][:, 2], bound["dstate"][:, 2], "dstate")
