@@ -740,7 +740,7 @@ int walk(const FishingDecayAttention* f, Strided q, Strided k, Strided v, const 
     auto wide = [&](const Strided& s, int d) {
         return d % V == 0 && aligned16(s.p) && s.batch % V == 0 && s.step % V == 0 && s.head % V == 0 && s.step >= d && s.step < (int64_t)1 << 24;
     };
-    const bool vec = wide(q, dk) && wide(k, dk) && wide(v, dv) && wide(out, dv) && f->starts_stride[1] < (int64_t)1 << 24;
+    const bool vec = wide(q, dk) && wide(k, dk) && wide(v, dv) && wide(out, dv) && f->starts_stride[1] >= 0 && f->starts_stride[1] < (int64_t)1 << 24;
     const int64_t block = batch_block(f->batch, f->heads);
     WalkPlan p = walk_plan(f->dtype, block * f->heads, f->steps, dk, dv, vec);
     const bool given = shared && shared->nk;

@@ -9,7 +9,7 @@ from torch.autograd import forward_ad
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
 import sequence_reference as ref  # noqa: E402
 from test_gpu_sequence import make, rand  # noqa: E402
-from gym_fishing_amd import sequence  # noqa: E402
+from gym_fishing_amd import _capi, sequence  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 BOTH = [torch.float32, torch.bfloat16]
@@ -115,3 +115,22 @@ def test_nothing_passes_a_start_across_segments(dk, dv, dtype):
     assert not torch.isfinite(got["out"][0, :20, :2]).any() and not torch.isfinite(got["out"][0, 170:300, :2]).any()
     assert torch.isnan(got["state"][0]).any() and torch.isfinite(got["state"][0, 2]).all()
     ref.check(got["dstate"][:, 2], want["dstate"][:, 2], bound["dstate"][:, 2], "dstate")
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+def test_the_entry_takes_starts_that_run_backwards(dtype):
+    """A negative step stride of `starts`, which the C entry allows: read from the last byte down, never beyond them."""
+    q, k, v, ld, cut, s0, _, _ = make(3, 77, 2, 32, 32, dtype, False, 0.1, True, seed=4)
+    want = sequence.decay_attention(q, k, v, ld, starts=cut, state=s0)
+    back = cut.flip(1).contiguous()
+    out = torch.empty_like(v)
+    a = sequence._attention_args(q, k, v, ld, back, s0, 32 ** -0.5)
+    a.starts += back.shape[1] - 1
+    a.starts_stride[1] = -1
+    a.out = out.data_ptr()
+    a.out_stride[:] = out.stride()[:3]
+    lib = _capi.lib()
+    work = torch.empty(lib.fishing_decay_attention_workspace(a, 0), dtype=torch.uint8, device="cuda")
+    assert lib.fishing_decay_attention_forward(a, work.data_ptr(), work.numel(), torch.cuda.current_stream().cuda_stream) == 0
+    bound = ref.attention_bounds(q, k, v, ld, cut, s0, 32 ** -0.5)["out"]
+    ref.check(out, want.cpu().double(), 2 * bound, "out")        # (another width of access: the same sums in another order)
