@@ -275,18 +275,35 @@ def decay_attention(q, k, v, log_decay, starts=None, state=None, scale=None, ret
     return (out, last) if return_state else out
 
 
+def _span(x):
+    """The addresses from x's first element to behind its last."""
+    at = x.data_ptr()
+    return at, at + (x.nbytes if x.is_contiguous() else x.element_size() + x.element_size() * sum((n - 1) * s for n, s in zip(x.shape, x.stride())))
+
+
 def _overlap(x, y):
     """Whether the memory between x's first and last element meets y's."""
     if x.numel() == 0 or y.numel() == 0:
         return False
-    (a0, a1), (b0, b1) = ((z.data_ptr(), z.data_ptr() + z.element_size() * (1 + sum((n - 1) * s for n, s in zip(z.shape, z.stride())))) for z in (x, y))
+    (a0, a1), (b0, b1) = _span(x), _span(y)
     return a0 < b1 and b0 < a1
+
+
+def _check_written(x, name, operands):
+    """What a call writes (contiguous) may not lie where it reads: its workgroups run in any order."""
+    lo = x.data_ptr()
+    hi = lo + x.nbytes
+    for y in operands:
+        if y is not None:
+            at = y.data_ptr()
+            if at < hi and (at >= lo or _span(y)[1] > lo) and lo < hi and y.numel():
+                raise ValueError("%s overlaps an operand" % name)
 
 
 def decay_attention_step(q, k, v, log_decay, state, starts=None, scale=None, out=None, state_out=None):
     """One step of decay_attention for a batch: q, k [batch, heads, dk], v [batch, heads, dv], starts bool [batch] (the done flags of
     the step before).  `state` (float32 [batch, heads, dk, dv], contiguous) moves on in place, or into `state_out` (which may be
-    `state` itself; it may not overlap it otherwise).  Returns out [batch, heads, dv] (written into `out` if given).
+    `state` itself; it may not overlap it otherwise); neither it nor `out` may overlap another operand.  Returns out [batch, heads, dv] (written into `out` if given).
     Acting, not training: there is no gradient, and operands that require one are refused while gradients are recorded."""
     if state is None:
         raise TypeError("state must be a torch.Tensor: the memory that moves on")
@@ -299,6 +316,7 @@ def decay_attention_step(q, k, v, log_decay, state, starts=None, scale=None, out
         _check_starts(starts, (batch,), dev)
     if not state.is_contiguous():
         raise ValueError("state must be contiguous: it moves on in place")
+    operands = (q, k, v, log_decay, starts)
     if state_out is None:
         state_out = state
     else:
@@ -307,14 +325,14 @@ def decay_attention_step(q, k, v, log_decay, state, starts=None, scale=None, out
             raise ValueError("state_out must be contiguous %s, got %s" % (shape, tuple(state_out.shape)))
         if state_out.data_ptr() != state.data_ptr() and _overlap(state, state_out):
             raise ValueError("state_out overlaps state without being it")
+    _check_written(state_out, "the state that moves on", operands)
     if out is None:
         out = torch.empty((batch, heads, dv), dtype=q.dtype, device=dev)
     else:
         _tensor(out, "out", 3, (q.dtype,), dev)
         if tuple(out.shape) != (batch, heads, dv) or not out.is_contiguous():
             raise ValueError("out must be contiguous %s, got %s, strides %s" % ((batch, heads, dv), tuple(out.shape), out.stride()))
-        if any(_overlap(out, x) for x in (q, k, v, state, state_out)):
-            raise ValueError("out overlaps an operand")
+        _check_written(out, "out", operands + (state, state_out))
     q, k, v = _unit(q), _unit(k), _unit(v)
     log_decay = log_decay.contiguous()
     a = FishingDecayAttention()

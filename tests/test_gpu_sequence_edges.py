@@ -134,3 +134,26 @@ def test_the_entry_takes_starts_that_run_backwards(dtype):
     assert lib.fishing_decay_attention_forward(a, work.data_ptr(), work.numel(), torch.cuda.current_stream().cuda_stream) == 0
     bound = ref.attention_bounds(q, k, v, ld, cut, s0, 32 ** -0.5)["out"]
     ref.check(out, want.cpu().double(), 2 * bound, "out")        # (another width of access: the same sums in another order)
+
+
+def test_the_step_writes_nowhere_it_reads():
+    """The state that moves on and `out` may lie neither in q, k, v nor in the decays or the starts: another workgroup may not have read them yet."""
+    batch, heads, d = 4, 2, 8
+    pool = torch.zeros(4096, device="cuda")
+    state = pool[512:512 + batch * heads * d * d].view(batch, heads, d, d)
+    end = 512 + state.numel()
+    q, k, v = (rand(batch, heads, d, seed=i) for i in range(3))
+    ld, starts, other = torch.tensor([-0.1, -0.2], device="cuda"), torch.zeros(batch, dtype=torch.bool, device="cuda"), torch.zeros_like(state)
+    inside, bits = pool[600:600 + batch * heads * d].view(batch, heads, d), pool.view(torch.bool)
+    fine = dict(q=q, k=k, v=v, log_decay=ld, state=state, starts=starts)
+    for bad in (dict(q=inside), dict(k=inside), dict(v=inside), dict(log_decay=pool[end - 1:end + 1]), dict(starts=bits[4 * end - 1:4 * end + 3])):
+        for kw in (dict(), dict(state=other, state_out=state)):
+            with pytest.raises(ValueError, match="overlaps"):
+                sequence.decay_attention_step(**{**fine, **bad, **kw})
+        if not set(bad) & {"q", "k", "v"}:                # `out` in the same place
+            with pytest.raises(ValueError, match="overlaps"):
+                sequence.decay_attention_step(**{**fine, **bad, "state": other, "out": pool[end - batch * heads * d:end].view(batch, heads, d)})
+    beside = pool[end:end + batch * heads * d].view(batch, heads, d)         # next to it is not in it
+    sequence.decay_attention_step(**{**fine, "q": beside, "out": pool[512 - batch * heads * d:512].view(batch, heads, d)})
+    wide = pool[:512].view(batch, 128)[:, 100:116].view(batch, heads, d)       # rows that end before it, with gaps
+    sequence.decay_attention_step(**{**fine, "q": wide})
