@@ -303,14 +303,15 @@ def _check_written(x, name, operands):
 def decay_attention_step(q, k, v, log_decay, state, starts=None, scale=None, out=None, state_out=None):
     """One step of decay_attention for a batch: q, k [batch, heads, dk], v [batch, heads, dv], starts bool [batch] (the done flags of
     the step before).  `state` (float32 [batch, heads, dk, dv], contiguous) moves on in place, or into `state_out` (which may be
-    `state` itself; it may not overlap it otherwise); neither it nor `out` may overlap another operand.  Returns out [batch, heads, dv] (written into `out` if given).
-    Acting, not training: there is no gradient, and operands that require one are refused while gradients are recorded."""
+    `state` itself; it may not overlap it otherwise); neither it nor `out` may overlap another operand.  Returns out [batch, heads, dv]
+    (written into `out` if given).  Acting, not training: there is no gradient, and while gradients are recorded tensors that require one
+    are refused, to read or to write."""
     if state is None:
         raise TypeError("state must be a torch.Tensor: the memory that moves on")
     shape = _check_heads(q, k, v, log_decay, state, 3)
     batch, heads, dk, dv = shape
     dev = q.device
-    if torch.is_grad_enabled() and any(x.requires_grad for x in (q, k, v, state)):
+    if torch.is_grad_enabled() and any(getattr(x, "requires_grad", False) for x in (q, k, v, state, out, state_out)):
         raise ValueError("the single step has no gradient: call it under torch.no_grad(), or train with decay_attention")
     if starts is not None:
         _check_starts(starts, (batch,), dev)

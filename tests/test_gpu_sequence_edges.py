@@ -157,3 +157,13 @@ def test_the_step_writes_nowhere_it_reads():
     sequence.decay_attention_step(**{**fine, "q": beside, "out": pool[512 - batch * heads * d:512].view(batch, heads, d)})
     wide = pool[:512].view(batch, 128)[:, 100:116].view(batch, heads, d)       # rows that end before it, with gaps
     sequence.decay_attention_step(**{**fine, "q": wide})
+
+
+def test_the_step_does_not_write_into_what_requires_a_gradient():
+    q, k, v = (rand(2, 1, 8, seed=i) for i in range(3))
+    ld, state = torch.tensor([-0.1], device="cuda"), rand(2, 1, 8, 8, seed=4)
+    for bad in (dict(out=torch.zeros((2, 1, 8), device="cuda", requires_grad=True)), dict(state_out=torch.zeros_like(state).requires_grad_())):
+        with pytest.raises(ValueError, match="no gradient"):
+            sequence.decay_attention_step(q, k, v, ld, state, **bad)
+        with torch.no_grad():
+            sequence.decay_attention_step(q, k, v, ld, state, **bad)
