@@ -233,15 +233,28 @@ __global__ void __launch_bounds__(G::THREADS, 2)
     }
 }
 
-// ---- out[n][m] (+)= sum_k A[m, k] B[n, k] over a share of k: float32 slabs (one per share, added to across pieces) or the type ----
-template <typename T, typename O, typename G, int BM, int BN>
+// ---- out[n][m] (+)= sum_k A[m, k] B[n, k] over a share of k: float32 slabs (one per share, added to across pieces) or the type.  PADDED:
+// rows n of padded targets are zeros, whatever A holds (their dz is zero, and zero times NaN is NaN) ----
+struct Targets {
+    const void* target;
+    int bytes;
+    int64_t levels;
+};
+
+template <typename T, typename O, typename G, int BM, int BN, bool PADDED>
 __global__ void __launch_bounds__(G::THREADS, 2)
-    product_kernel(Operand<T> a, Operand<T> b, int64_t k, int64_t share, int64_t m, int64_t n, int64_t tiles_m, int64_t tiles_n, bool add, O* out, int64_t ld, int64_t slab) {
+    product_kernel(Operand<T> a, Operand<T> b, int64_t k, int64_t share, int64_t m, int64_t n, int64_t tiles_m, int64_t tiles_n, bool add, O* out, int64_t ld, int64_t slab,
+                   Targets y) {
     __shared__ __attribute__((aligned(16))) char lds0[G::BYTES];
     __shared__ __attribute__((aligned(16))) char lds1[G::BYTES];
     int64_t tm, tn;
     tile_of(blockIdx.x, tiles_m, tiles_n, tm, tn);
     const int64_t lo = blockIdx.y * share, hi = lo + share < k ? lo + share : k;
+    __shared__ bool gone[PADDED ? BN : 1];                // read behind the product's barriers (an empty share has none, and sums of zero)
+    if (PADDED && threadIdx.x < BN) {
+        const int64_t row = tn * BN + threadIdx.x, t = row < n ? target_of(y.target, y.bytes, row) : -1;
+        gone[threadIdx.x] = t < 0 || t >= y.levels;
+    }
     f32x4 acc[G::MT][G::NT];
     G::run(lds0, lds1, a, tm * BM, b, tn * BN, lo, hi, acc);
     const int64_t left_n = n - tn * BN, left_m = m - tm * BM;
@@ -250,6 +263,7 @@ __global__ void __launch_bounds__(G::THREADS, 2)
     const bool whole = (ld & 3) == 0 && (((uintptr_t)out) & (4 * sizeof(O) - 1)) == 0;
     G::each(acc, [&](int r, int c, f32x4 x) {
         if (c >= n_here || r >= m_here) return;
+        if (PADDED && gone[c]) x = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         O* p = to + c * ld + r;
         if (whole && r + 4 <= m_here) {
             Pack<O, 4> y;
@@ -489,13 +503,14 @@ static int loss_forward(int64_t rows, int64_t levels, int64_t dim, const T* h, i
     return rc;
 }
 
-template <typename T, typename O, bool A_MAJOR, bool B_MAJOR>
-static int product(const Operand<T>& a, const Operand<T>& b, const Tiling& t, int64_t k, int64_t m, int64_t n, bool add, O* out, int64_t ld, int64_t slab, hipStream_t stream) {
+template <typename T, typename O, bool A_MAJOR, bool B_MAJOR, bool PADDED>
+static int product(const Operand<T>& a, const Operand<T>& b, const Tiling& t, int64_t k, int64_t m, int64_t n, bool add, O* out, int64_t ld, int64_t slab, const Targets& y,
+                   hipStream_t stream) {
     return with_tile<T, A_MAJOR, B_MAJOR>(t.b, [&](auto tile) {
         typedef decltype(tile) Tile;
         const int64_t tm = ceil_div(m, Tile::EDGE), tn = ceil_div(n, Tile::EDGE);
-        return launch(product_kernel<T, O, typename Tile::G, Tile::EDGE, Tile::EDGE>, dim3((unsigned)(tm * tn), (unsigned)t.shares), dim3(Tile::G::THREADS), stream, a, b, k, t.share,
-                      m, n, tm, tn, add, out, ld, slab);
+        return launch(product_kernel<T, O, typename Tile::G, Tile::EDGE, Tile::EDGE, PADDED>, dim3((unsigned)(tm * tn), (unsigned)t.shares), dim3(Tile::G::THREADS), stream, a, b, k,
+                      t.share, m, n, tm, tn, add, out, ld, slab, y);
     });
 }
 
@@ -511,6 +526,7 @@ static int loss_backward(int64_t rows, int64_t levels, int64_t dim, const T* h, 
     for (int64_t r0 = 0; r0 < rows && !rc; r0 += p.block) {
         const int64_t here = rows - r0 < p.block ? rows - r0 : p.block, here_p = round_up(here, p.bk);
         const void* y = (const char*)target + r0 * target_bytes;
+        const Targets targets{y, target_bytes, levels};
         const Operand<T> a{k.h, p.dim_p, here, here};
         rc = pads(PadJob<T>{h + r0 * h_ld, h_ld, here, k.h, y}, r0 ? PadJob<T>{} : w_job, p, dim, target_bytes, levels, stream);
         for (int64_t v0 = 0; v0 < levels && !rc; v0 += p.piece) {
@@ -529,21 +545,21 @@ static int loss_backward(int64_t rows, int64_t levels, int64_t dim, const T* h, 
                 t.share = round_up(ceil_div(width_p, p.dh.shares), p.bk);
                 t.shares = ceil_div(width_p, t.share);
             }
-            rc = k.dh ? product<T, float, true, true>(wd, zr, t, width_p, dim, here, v0 > 0, k.dh, dim, k.dh_slab, stream)
-                      : product<T, T, true, true>(wd, zr, t, width_p, dim, here, false, dh + r0 * dim, dim, 0, stream);
+            rc = k.dh ? product<T, float, true, true, true>(wd, zr, t, width_p, dim, here, v0 > 0, k.dh, dim, k.dh_slab, targets, stream)
+                      : product<T, T, true, true, true>(wd, zr, t, width_p, dim, here, false, dh + r0 * dim, dim, 0, targets, stream);
             if (rc) break;
             // dW[v][d]: m = d, n = v, k = rows; h's rows beyond the last meet zeros of dz.  (A share behind the last block's rows adds
             // nothing to its slab.)
             const Operand<T> hd{k.h, p.dim_p, p.dim_p, here}, zv{k.dzt, here_p, width, width};
             t = k.dw_slab ? whole : dw_tiling<T>(p, width, dim);
             if (k.dw_slab) {
-                rc = product<T, float, true, false>(hd, zv, t, here_p, dim, width, r0 > 0, k.dw + v0 * dim, dim, k.dw_slab, stream);
+                rc = product<T, float, true, false, false>(hd, zv, t, here_p, dim, width, r0 > 0, k.dw + v0 * dim, dim, k.dw_slab, targets, stream);
             } else if (t.shares > 1) {
                 const int64_t slab = round_up(width * dim, 4);
-                rc = product<T, float, true, false>(hd, zv, t, here_p, dim, width, false, k.dw, dim, slab, stream);
+                rc = product<T, float, true, false, false>(hd, zv, t, here_p, dim, width, false, k.dw, dim, slab, targets, stream);
                 if (!rc) rc = slab_sum<T>(k.dw, slab, t.shares, dw + v0 * dim, width * dim, stream);
             } else {
-                rc = product<T, T, true, false>(hd, zv, t, here_p, dim, width, false, dw + v0 * dim, dim, 0, stream);
+                rc = product<T, T, true, false, false>(hd, zv, t, here_p, dim, width, false, dw + v0 * dim, dim, 0, targets, stream);
             }
         }
         if (!rc && k.dh) rc = slab_sum<T>(k.dh, k.dh_slab, p.dh.shares, dh + r0 * dim, here * dim, stream);

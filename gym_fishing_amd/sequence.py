@@ -394,7 +394,7 @@ class _CrossEntropy(torch.autograd.Function):
 def cross_entropy(hidden, head, target):
     """loss[r] = logsumexp_v(hidden[r] . head[v]) - hidden[r] . head[target[r]], float32 [rows]: minus the log probability of the
     level taken.  hidden: [rows, dim], head: [levels, dim], float32 or bfloat16; target: int32 / int64 [rows], one outside
-    [0, levels) is padding: loss 0, no gradient, whatever its row of `hidden` holds.  The logits are computed in pieces of the
+    [0, levels) is padding: loss 0, no gradient, whatever its row of `hidden` or the head hold.  The logits are computed in pieces of the
     levels and never kept.  Differentiable in hidden and head, with any gradient of the rows (weights, advantages)."""
     _tensor(hidden, "hidden", 2, _DTYPES)
     dev = hidden.device

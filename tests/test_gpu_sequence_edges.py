@@ -167,3 +167,20 @@ def test_the_step_does_not_write_into_what_requires_a_gradient():
             sequence.decay_attention_step(q, k, v, ld, state, **bad)
         with torch.no_grad():
             sequence.decay_attention_step(q, k, v, ld, state, **bad)
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("rows,levels,dim", [(200, 100, 40), (64, 20001, 16), (9, 5, 300)])
+def test_padding_takes_no_gradient_whatever_the_head_holds(rows, levels, dim, dtype):
+    hidden, head = rand(rows, dim, seed=1, dtype=dtype).requires_grad_(), rand(levels, dim, seed=2, dtype=dtype, scale=dim ** -0.5)
+    head[levels // 2, 0], head[levels - 1, dim - 1] = float("nan"), float("inf")
+    head.requires_grad_()
+    target = torch.arange(rows, device="cuda") % levels
+    gone = torch.arange(0, rows, 4, device="cuda")
+    target[gone] = torch.tensor([-1, levels], device="cuda")[torch.arange(len(gone), device="cuda") % 2]
+    loss = sequence.cross_entropy(hidden, head, target)
+    dhidden, dhead = torch.autograd.grad(loss.sum(), (hidden, head))
+    assert (loss[gone] == 0).all() and (dhidden[gone] == 0).all()
+    there = torch.ones(rows, dtype=torch.bool, device="cuda")
+    there[gone] = False
+    assert torch.isnan(loss[there]).all() and torch.isnan(dhidden[there]).all()          # and what is not padding does not hide it
