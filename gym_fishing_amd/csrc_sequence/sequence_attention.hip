@@ -137,6 +137,7 @@ static int attention_backward(const FishingDecayAttention* a, void* work, hipStr
     // dq: read with do the state that (v, k) build;  dk, dv: read with v, k the state's gradient that (do, q), (q, do) build backwards,
     // in segments from the same states
     Shared both;
+    both.exact = a->dstate != nullptr;
     int rc = walk<T, false>(a, g, v, k, a->state, nullptr, strided((const void*)a->dq, a->dq_stride), a->dv, a->dk, true, false, a->scale, 1.0, nullptr, work, stream);
     if (!rc) rc = walk<T, true>(a, v, g, q, a->dstate_out, nullptr, strided((const void*)a->dk_out, a->dk_stride), a->dv, a->dk, true, false, 1.0, a->scale, &both, work, stream);
     if (!rc)

@@ -726,6 +726,7 @@ static WalkWork walk_work(const WalkPlan& p, int64_t pairs, int dv, float* carry
 
 // What a walk in segments leaves to one whose state is its own transposed, from the same terms: the states it starts its segments from
 struct Shared {
+    bool exact = false;        // the other's state is an answer
     int nk = 0, segs = 1;
     int64_t seg_steps = 0;
     float* carry = nullptr;
@@ -755,7 +756,7 @@ int walk(const FishingDecayAttention* f, Strided q, Strided k, Strided v, const 
         }
     }
     const WalkWork w = walk_work(p, block * f->heads, dv, given ? shared->carry : nullptr, (char*)workspace + (given ? shared->bytes : 0));
-    if (shared && !given && p.segs > 1) *shared = Shared{p.nk, p.segs, p.seg_steps, w.carry, w.bytes};
+    if (shared && !given && p.segs > 1) *shared = Shared{shared->exact, p.nk, p.segs, p.seg_steps, w.carry, w.bytes};
     ChunkArgs a{q, k, v, out, f->log_decay, f->starts, f->starts_stride[0], f->starts_stride[1], state, state_out, f->steps, f->heads, dk, dv, state_t, exact_state,
                       (float)read_scale, (float)write_scale, p.slices, p.segs, p.seg_steps, w.carry, w.through, w.odd, given ? shared->nk : 0};
     int64_t pairs = 0;
@@ -770,6 +771,7 @@ int walk(const FishingDecayAttention* f, Strided q, Strided k, Strided v, const 
             const int per = NK * 256, col_tiles = (int)ceil_div(dv, 16);
             ChunkArgs local = a;
             local.slices = (int)ceil_div(dv, LV * 16);
+            local.exact_state = exact_state || (shared && shared->exact);
             rc = launch(chunk_kernel<T, NK, LV, BACK, VEC, true>, dim3((unsigned)(pairs * local.slices * p.segs)), dim3(64), stream, local);
             if (!rc) rc = launch(chain_kernel, dim3((unsigned)(per / 256), (unsigned)(pairs * col_tiles)), dim3(64), stream, w.carry, w.through, p.segs, per, col_tiles);
         }

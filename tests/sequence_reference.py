@@ -111,3 +111,12 @@ def state_bound(size, steps):
     """How far a float32 state may be off, `size` the state of the operands' magnitudes: a product of bfloat16 values is exact in float32; the
     decays weigh it as a product of float32 factors, one a chunk or step, and are exp2 of a rounded exponent; v's three bfloat16 terms leave 2^-26."""
     return (2 * steps + 64) * 2.0 ** -24 * size
+
+
+def check_state_norm(got, want, steps, what=""):
+    """A float32 state that nothing decays, in the 2-norm: each of `steps` additions rounds its partial sum by up to 2^-24 of it, 2^-24 / sqrt 3 in
+    the mean; partial sums of terms of random sign grow like the root of their count: 2^-24 sqrt(steps / 6) of the whole, and 4 units of 2^-24 for
+    scaling the terms and what is left.  Terms of 16 bits (two of bfloat16) are off by 2^-19.3."""
+    got = got.detach().cpu().to(F64)
+    off, most = (got - want).norm(), (0.41 * steps ** 0.5 + 4) * 2.0 ** -24 * want.norm()
+    assert off <= most, "%s: off by %.3g where %.3g is allowed" % (what, off, most)

@@ -35,3 +35,17 @@ def test_outputs_are_rounded_once_and_states_are_float32(batch, steps, heads, dk
         size = ref.attention(q.abs(), k.abs(), v.abs(), ld, cut, s0.abs(), 0.3, g.abs(), gs.abs())
         ref.check(got[1], want["state"], ref.state_bound(size["state"], steps), "state")
         ref.check(grads[3], want["dstate"], ref.state_bound(size["dstate"], steps), "dstate")
+
+
+@pytest.mark.parametrize("dk,dv", [(64, 64), (48, 112), (33, 65)])
+@pytest.mark.parametrize("steps", [32, 704])
+def test_states_that_nothing_decays_are_float32_sums(steps, dk, dv):
+    """Whole and in segments, whose states the gradient's walk takes over from another's."""
+    q, k, v, _, _, s0, g, gs = make(1, steps, 2, dk, dv, torch.bfloat16, False, 0.0, True, seed=dk)
+    ld = torch.zeros(2, device="cuda")
+    leaf, s0 = q.detach().requires_grad_(), s0.requires_grad_()
+    out, last = sequence.decay_attention(leaf, k, v, ld, state=s0, scale=0.3, return_state=True)
+    dstate = torch.autograd.grad((out, last), s0, (g, gs))[0]
+    want = ref.attention(q, k, v, ld, None, s0, 0.3, g, gs)
+    ref.check_state_norm(last, want["state"], steps, "state")
+    ref.check_state_norm(dstate, want["dstate"], steps, "dstate")

@@ -63,3 +63,17 @@ def test_forms_with_too_few_bits_fail_and_one_with_enough_passes(steps, d):
     ref.check_once_rounded(scored(q, k, v, ld, 0.3, 2), want, "scores of 16 bits")
     with pytest.raises(AssertionError):
         ref.check_once_rounded(scored(q, k, v, ld, 0.3, 1), want, "scores of 8 bits")
+
+
+def test_a_state_made_of_terms_of_16_bits_fails():
+    g = torch.Generator().manual_seed(2)
+    k, v = (torch.randn((704, 64), generator=g).to(torch.bfloat16) for _ in range(2))
+    w = v.float() * 0.3
+    want = k.double().t() @ v.double() * 0.3
+    S = torch.zeros((64, 64))
+    for t in range(704):
+        S = S + k[t].float()[:, None] * w[t][None]
+    ref.check_state_norm(S, want, 704)
+    two = short(w) + short(w - short(w))
+    with pytest.raises(AssertionError):
+        ref.check_state_norm(k.double().t() @ two.double(), want, 704)
