@@ -13,7 +13,8 @@ namespace fishing {
 namespace seq {
 
 // ---- the single step: a wave owns one (env, head); its state goes through registers once, eight 16-byte loads a lane in flight.
-// Bound by the state's two trips: 65536 envs, 4 heads of 32 x 32: 367 us, 6.2 TB/s.  64 envs: 4 us of the call's 17, which are the host's ----
+// Bound by the state's two trips: 65536 envs, 4 heads of 32 x 32: 374 us a call back to back, 408 on average in a kernel trace (372 at
+// best): 5.6 - 6.1 TB/s.  64 envs: 5 us of the call's 15, which are the host's ----
 template <typename T, int V>
 __global__ void __launch_bounds__(256) step_kernel_recurrent(Strided q, Strided k, Strided v, const float* log_decay, const uint8_t* starts, int64_t starts_stride,
                                                              const float* state, float* state_out, T* out, int64_t out_batch, int64_t out_head, int64_t pairs,

@@ -7,12 +7,14 @@
 // joined afterwards.  Backward: per piece of the levels the logits are computed again and turned into dz (rounded to the operands'
 // type: it is a factor of the two products that follow; sums stay in float32), kept for the piece as dz^T [level][row], where four
 // rows of a lane's accumulator are one store, and multiplied twice: k-major for dh, k-contiguous for dW.  In bf16 that rounding of dz
-// makes the gradients' error 1.4 times their own last rounding's; for a handful of rows, whose dh is mostly one term, up to twice.
+// makes the gradients' error 1.4 times their own last rounding's; for a handful of rows, whose dh is mostly one term, up to twice.  As
+// two terms dz would double both products: at 8192 x 32771 x 1024 another 2 x (283 + 256) us.
 //
-// 8192 x 32771 x 1024, bf16: forward 634 us (870 TFLOP/s), and a piece of 16384 levels dz 312 (880), dW 290 (950), dh 260 (1060); a
-// library's product of that shape reaches 1100.  Bound by LDS: a step's 128 KiB of fragments and 64 KiB of staging fill its 128 bytes
-// a cycle for three quarters of what the matrix cores need; the forward's and dz's exponentials come on top.  float32 products run on
-// the float32 matrix cores (5001 x 1009 x 200: 33 us each, the matrix cores 60% busy); as three bf16 terms, six products, 34 - 42.
+// 8192 x 32771 x 1024, bf16: forward 626 us (880 TFLOP/s), and a piece of 16384 levels dz 302 (910), dW 283 (970), dh 256 (1070); a
+// library's product of that shape reaches 1100.  Bound by LDS: a step's 192 KiB of fragments (eight waves, 8 + 4 of 1 KiB, twice) and 64 KiB
+// of staging take 2048 cycles of its 128 bytes, as many as the matrix cores need; the forward's and dz's exponentials come on top.
+// float32 products run on the float32 matrix cores (5001 x 1009 x 200: 33 us each, the matrix cores 60% busy); as three bf16 terms, six
+// products, 34 - 42.
 // 103424 x 100 x 128, bf16: 20 us forward, 20 dz, 31 dh, 19 dW, 13 the clean copy of h: bound by bytes and launches.
 #include "sequence_gemm.h"
 

@@ -38,9 +38,11 @@ static int64_t batch_block(int64_t batch, int heads) {
 // output's own rounding is then too small to show in it (a copy of the state in one term: up to 1.4x that rounding, 2 - 3% less time).
 // A wave alone needs no barriers; the next chunk's rows are loaded into registers while this one is computed, and the registers (state,
 // rows in flight, operands) leave room for two waves on a SIMD.  What bounds it is those waves' dependent work, not a unit: 2048 x 101
-// steps, 4 heads of 64 x 64, bf16: 112 us a walk, 2.7 TB/s, VALU 37% and matrix cores 17% busy; 97 x 1009 steps, 3 heads of 48 x 80,
-// f32: 78 - 100 us and 46 for the segments' states, matrix cores half busy; 16381 steps, 8 heads of 128 x 128, bf16, one wave a
-// SIMD: 61 us, states 27, chain 11.  (A third wave a SIMD spilled: 2.3 times slower.)
+// steps, 4 heads of 64 x 64, bf16: 117 us a walk, 3.6 TB/s of operands, VALU 42% and matrix cores 18% busy; 97 x 1009 steps, 3 heads of
+// 48 x 80, f32: 76 - 98 us and 44 for the segments' states, matrix cores 44% busy; 16381 steps, 8 heads of 128 x 128, bf16, one wave a
+// SIMD: 67 us, states 27, chain 11.  (A third wave a SIMD spilled: 2.3 times slower.)  Rows that are not whole 16-byte accesses take
+// element loads, and two tiles of columns a wave: 2048 x 101 steps of 63 x 65 instead of 64 x 64 with gradients 2092 us for 479, 97 x 1009 of
+// 47 x 81 f32 1074 for 509 (kernels, captured).
 
 // The value, not to be worked with ahead of this place: what is computed of lane numbers for the rare chunk would otherwise be
 // computed once and kept, some sixty registers of it
@@ -661,7 +663,7 @@ __global__ void __launch_bounds__(256) odd_kernel(ChunkArgs a, int64_t pairs) {
 
 // The recurrence for every pair, 32 columns of its state a workgroup, where there are few steps and no more workgroups than the chip
 // holds at once: a chunk would be nearly empty.  16 pairs of 32 x 32: 5 us a step, 7 four, chunks 10; 16384 pairs, four steps: 61 us,
-// chunks 32
+// chunks 32; 512 pairs of 128 x 128, the most that take this way: four steps as long as chunks, eight 10 us longer
 constexpr int64_t kFewSteps = 8, kFewGroups = 2048;
 
 template <typename T, bool BACK>

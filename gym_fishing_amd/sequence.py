@@ -13,7 +13,9 @@ tests/test-PPO.py:10-21) cannot use it.  These are the operators of one that can
 `policies.memory` is the policy built on them.  Everything runs in hand-written HIP kernels behind the C ABI
 (include/fishing_hip.h) on torch's current stream of the tensors' device; there is no CPU fallback.  Values are float32 or
 bfloat16 (float16's range is too narrow for the products of states and for dz); sums, softmax statistics and states are float32.
-The same inputs give the same bits.  Derivatives are reverse-mode and of the first order: an operand or gradient that carries a
+What comes back in bfloat16 is rounded once, from 16 bits or more, but for cross_entropy's gradients: dz, the logits' gradient that both
+products take as a factor, is rounded to bfloat16 before them (as two terms it would double their work), so they are 1.4 times as far off as
+one rounding, and dhidden of a handful of rows up to twice.  The same inputs give the same bits.  Derivatives are reverse-mode and of the first order: an operand or gradient that carries a
 forward-mode tangent is refused.
 
 Tensors made on another stream are the caller's to order, as for any torch operator.  Captured into a hipGraph, an operator
@@ -258,8 +260,9 @@ def decay_attention(q, k, v, log_decay, starts=None, state=None, scale=None, ret
 
     q, k: [batch, steps, heads, dk], v: [batch, steps, heads, dv], float32 or bfloat16, dk and dv in 1 .. 128; any strides (a
     time-major record's `x.transpose(0, 1)` is read in place and answered in the same order; a last axis with gaps is copied).
-    log_decay: float32 [heads], a head's horizon (no gradient; -inf, or where float32's exp is 0: nothing is kept, not even NaN).  starts: bool [batch, steps], True where an episode
-    begins -- the done flags of the step before (SB3's `episode_starts`): nothing passes from before it, not even NaN.
+    log_decay: float32 [heads], a head's horizon (no gradient; -inf, or where float32's exp is 0: nothing is kept, not even NaN).
+    starts: bool [batch, steps], True where an episode begins -- the done flags of the step before (SB3's `episode_starts`):
+    nothing passes from before it, not even NaN.
     state: float32 [batch, heads, dk, dv], the memory from earlier steps (None: zeros).  scale: dk ** -0.5 by default.
     Returns out [batch, steps, heads, dv], or (out, state behind the last step) with return_state.
     Differentiable in q, k, v and state."""
@@ -395,7 +398,8 @@ def cross_entropy(hidden, head, target):
     """loss[r] = logsumexp_v(hidden[r] . head[v]) - hidden[r] . head[target[r]], float32 [rows]: minus the log probability of the
     level taken.  hidden: [rows, dim], head: [levels, dim], float32 or bfloat16; target: int32 / int64 [rows], one outside
     [0, levels) is padding: loss 0, no gradient, whatever its row of `hidden` or the head hold.  The logits are computed in pieces of the
-    levels and never kept.  Differentiable in hidden and head, with any gradient of the rows (weights, advantages)."""
+    levels and never kept.  Differentiable in hidden and head, with any gradient of the rows (weights, advantages); in bfloat16 with one
+    rounding more than the result's own (of dz, see above)."""
     _tensor(hidden, "hidden", 2, _DTYPES)
     dev = hidden.device
     _tensor(head, "head", 2, (hidden.dtype,), dev)

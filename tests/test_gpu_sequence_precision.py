@@ -8,7 +8,7 @@ import torch
 
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
 import sequence_reference as ref  # noqa: E402
-from test_gpu_sequence import make  # noqa: E402
+from test_gpu_sequence import make, rand  # noqa: E402
 from gym_fishing_amd import sequence  # noqa: E402
 
 pytestmark = pytest.mark.gpu
@@ -49,3 +49,19 @@ def test_states_that_nothing_decays_are_float32_sums(steps, dk, dv):
     want = ref.attention(q, k, v, ld, None, s0, 0.3, g, gs)
     ref.check_state_norm(last, want["state"], steps, "state")
     ref.check_state_norm(dstate, want["dstate"], steps, "dstate")
+
+
+@pytest.mark.parametrize("rows,levels,dim,most", [(4096, 100, 64, 1.6), (2050, 1009, 200, 1.6), (17, 4097, 512, 2.2)])
+def test_loss_gradients_are_rounded_twice(rows, levels, dim, most):
+    """dz, a factor of both products, is rounded once, and each gradient once: two roundings of one size that do not know of each
+    other make sqrt 2 times one's error in the 2-norm (and a tenth for the norm of few values).  A row whose gradient is mostly its target's
+    term takes that term's one error in every column: at worst 2^-8 where the columns' own is 2^-8 / sqrt 3 in the mean, so twice, and a tenth."""
+    hidden = rand(rows, dim, seed=1, dtype=torch.bfloat16).requires_grad_()
+    head = rand(levels, dim, seed=2, dtype=torch.bfloat16, scale=1.5 * dim ** -0.5).requires_grad_()
+    target = torch.randint(0, levels, (rows,), generator=torch.Generator().manual_seed(3)).cuda()
+    grad = rand(rows, seed=4)
+    got = torch.autograd.grad(sequence.cross_entropy(hidden, head, target), (hidden, head), grad)
+    want, _ = ref.loss(hidden, head, target, grad)
+    for name, x in zip(("dhidden", "dhead"), got):
+        once = (want[name].to(torch.bfloat16).double() - want[name]).norm()
+        assert (x.cpu().double() - want[name]).norm() <= most * once, name
